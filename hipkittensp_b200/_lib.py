@@ -12,6 +12,7 @@ E2M3 = 0
 E3M2 = 1
 E4M3 = 2   # MX-FP8
 E5M2 = 3   # MX-FP8
+E2M1 = 4   # MX-FP4
 
 FLAG_B_STATIC = 1
 
@@ -20,7 +21,7 @@ OK, ERR_BAD_ARG, ERR_CUDA, ERR_DEVICE_WAIT, ERR_UNSUPPORTED = 0, 1, 2, 3, 4
 # every symbol include/mxfp6.h declares
 SYMBOLS = ("mxfp6_version", "mxfp6_last_error", "mxfp6_gemm", "mxfp6_gemm_workspace_bytes", "mxfp6_gemm_ws",
            "mxfp6_gemm_noalloc", "mxfp6_gemm_multi", "mxfp6_gemm_copy_gather", "mxfp6_copy_gather_scratch_bytes", "mxfp6_gemm_ex", "mxfp6_gemm_requant", "mxfp6_gemm_scaled",
-           "mxfp6_quantize", "mxfp6_dequantize", "mxfp6_device_status", "mxfp6_debug_tma_dump", "mxfp6_debug_wait_timeout", "mxfp6_debug_option", "mxfp6_debug_plan")
+           "mxfp6_quantize", "mxfp6_dequantize", "mxfp6_dequantize_ex", "mxfp6_device_status", "mxfp6_debug_tma_dump", "mxfp6_debug_wait_timeout", "mxfp6_debug_option", "mxfp6_debug_plan")
 
 
 class Mxfp6Error(RuntimeError):
@@ -68,6 +69,8 @@ def _load() -> ctypes.CDLL:
     lib.mxfp6_quantize.argtypes = [vp, ci, i64, i64, ci, vp, vp, vp]
     lib.mxfp6_dequantize.restype = ci
     lib.mxfp6_dequantize.argtypes = [vp, vp, i64, i64, ci, vp, vp]
+    lib.mxfp6_dequantize_ex.restype = ci
+    lib.mxfp6_dequantize_ex.argtypes = [vp, vp, i64, i64, ci, vp, ci, vp]
     lib.mxfp6_device_status.restype = ci
     lib.mxfp6_device_status.argtypes = [ctypes.POINTER(ci)]
     lib.mxfp6_debug_wait_timeout.restype = ci

@@ -437,9 +437,9 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                 static_assert(OC == 64, "the staging layouts below assume pieces of 64 columns");
                 if (P.q_fmt >= 0) {
                     // The result leaves as an MX operand of the next layer: this thread's 64 columns are two blocks of
-                    // 32.  Their codes (2 x 24 or 2 x 32 bytes) are staged as one dense row of the piece and the piece
+                    // 32.  Their codes (2 x 16, 2 x 24 or 2 x 32 bytes) are staged as one dense row of the piece and the piece
                     // is stored by TMA like a bf16 piece (cmaps.m[0] then describes the code bytes of the output).
-                    const bool fp8 = P.q_fmt == kE4M3 || P.q_fmt == kE5M2;
+                    const bool fp8 = fmt_fp8(P.q_fmt);
                     const int row = my_p0 + prow;
                     uint32_t sbs = 0;
 #pragma unroll
@@ -452,7 +452,8 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                         if (P.q_fmt == kE2M3) sb = quant_block32<kE2M3>(f, w);
                         else if (P.q_fmt == kE3M2) sb = quant_block32<kE3M2>(f, w);
                         else if (P.q_fmt == kE4M3) sb = quant_block32<kE4M3>(f, w);
-                        else sb = quant_block32<kE5M2>(f, w);
+                        else if (P.q_fmt == kE5M2) sb = quant_block32<kE5M2>(f, w);
+                        else sb = quant_block32<kE2M1>(f, w);
                         sbs |= (uint32_t)sb << (8 * hb);
                         if (fp8) {
                             // 64-byte rows, 64-byte swizzle: 16-byte chunk c sits at c ^ ((row / 2) % 4)
@@ -461,6 +462,10 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                                          ::"r"(ra + (((2 * hb) ^ sw8) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                                          ::"r"(ra + (((2 * hb + 1) ^ sw8) << 4)), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+                        } else if (P.q_fmt == kE2M1) {
+                            // 32-byte rows, no swizzle
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(buf + prow * 32 + 16 * hb), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                         } else {
                             // 48-byte rows, no swizzle
                             const uint32_t ra = buf + prow * 48 + 24 * hb;
@@ -475,7 +480,7 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                     fence_proxy_async_smem();
                     asm volatile("bar.sync 1, 128;" ::: "memory");
                     if (etid == 0) {
-                        tma_store_2d_hint(&cmaps.m[0], buf, (fp8 ? 64 : 48) * (col / 64), my_p0, pol_st);
+                        tma_store_2d_hint(&cmaps.m[0], buf, 2 * fmt_block_bytes(P.q_fmt) * (col / 64), my_p0, pol_st);
                         bulk_commit_group();
                     }
                     ++n_out;

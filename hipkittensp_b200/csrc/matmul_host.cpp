@@ -5,7 +5,7 @@
 // fp32 accumulation in k order and one rounding to bf16 (|c - ref| <= 1 % of |ref|, the reference's criterion with
 // the absolute value it lacks, plus the row-normalised bound of this repository's parity tests).
 //
-//   matmul_host [M N K [fmt [warmup iters [check_rows]]]]        fmt 0 = E2M3, 1 = E3M2, 2 = E4M3, 3 = E5M2
+//   matmul_host [M N K [fmt [warmup iters [check_rows]]]]        fmt 0 = E2M3, 1 = E3M2, 2 = E4M3, 3 = E5M2, 4 = E2M1
 //
 // Operands are drawn on the host (normal distribution, seeded per copy), quantised on the GPU by mxfp6_quantize
 // and, for the check, read back through mxfp6_dequantize: the harness needs no number-format code of its own.
@@ -49,7 +49,7 @@ struct Operand {                // one quantised operand on the device
     uint8_t* scales = nullptr;
 };
 
-size_t code_bytes(int64_t rows, int64_t K, int fmt) { return (size_t)rows * (fmt >= 2 ? K : K * 3 / 4); }
+size_t code_bytes(int64_t rows, int64_t K, int fmt) { return (size_t)rows * (fmt == MXFP4_E2M1 ? K / 2 : fmt >= 2 ? K : K * 3 / 4); }
 
 // fp32 -> bf16 (round to nearest even) -> fp32
 float round_bf16(float x) {
@@ -89,7 +89,7 @@ int main(int argc, char** argv) {
     if (argc >= 5) fmt = std::atoi(argv[4]);
     if (argc >= 7) { warmup = std::atoi(argv[5]); iters = std::atoi(argv[6]); }
     if (argc >= 8) check_rows = std::atoi(argv[7]);
-    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || iters <= 0 || fmt < 0 || fmt > 3) {
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128 || iters <= 0 || fmt < 0 || fmt > 4) {
         std::fprintf(stderr, "usage: %s [M N K [fmt [warmup iters [check_rows]]]]   (K a multiple of 128)\n", argv[0]);
         return 2;
     }

@@ -20,6 +20,7 @@
 #include <utility>
 #include <vector>
 
+#include "dequantize_kernel.cuh"
 #include "gemm_kernel_2cta.cuh"
 #include "quantize_kernel.cuh"
 
@@ -156,6 +157,24 @@ static int ensure_smem_attr(DeviceState& d, const void* kern, int bytes) {
     return MXFP6_OK;
 }
 
+// One launch with programmatic stream serialisation: the kernel may begin while the preceding one drains and waits for it
+// (griddepcontrol.wait) before its first global access.
+template <typename... Params, typename... Args>
+static int launch_pdl(void (*kern)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t lc{};
+    lc.gridDim = dim3(grid, 1, 1);
+    lc.blockDim = dim3(block, 1, 1);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = st;
+    lc.attrs = &attr;
+    lc.numAttrs = options().pdl ? 1 : 0;
+    CUDA_TRY(cudaLaunchKernelEx(&lc, kern, args...));
+    return MXFP6_OK;
+}
+
 // ---------------------------------------------------------------------------------- tensor maps
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -184,6 +203,8 @@ static int get_encode_fn(EncodeTiledFn* out) {
 // kind 5: quantiser source, bf16 viewed as [blocks, 32] (64-byte rows), box 32 x box_rows, 64-byte swizzle
 // kind 6: re-quantised fp6 output bytes [rows, 3N/4] (inner = bytes per row), box 48 x box_rows, no swizzle
 // kind 7: re-quantised fp8 output bytes [rows, N], box 64 x box_rows, 64-byte swizzle
+// kind 8: packed 4-bit operand [rows, K] (inner = K elements) spread to 8-bit slots (16 codes in the first 8 bytes of each 16), box 128 x box_rows, 128-byte swizzle
+// kind 9: re-quantised fp4 output bytes [rows, N/2] (inner = bytes per row), box 32 x box_rows, no swizzle
 // Encoded maps are kept inside the launch recipe of the call that uses them; a small per-thread table of recent
 // encodings serves callers that alternate between a few buffers with otherwise new argument combinations.
 struct MapKey {
@@ -224,6 +245,8 @@ static int make_map(const void* ptr, int64_t rows, int64_t inner, int box_rows, 
         case 5: strides[0] = 64; box[0] = 32; dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; sw = CU_TENSOR_MAP_SWIZZLE_64B; break;
         case 6: strides[0] = (cuuint64_t)inner; box[0] = 48; sw = CU_TENSOR_MAP_SWIZZLE_NONE; break;
         case 7: strides[0] = (cuuint64_t)inner; box[0] = 64; sw = CU_TENSOR_MAP_SWIZZLE_64B; break;
+        case 8: strides[0] = (cuuint64_t)(inner / 2); dt = CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B; break;
+        case 9: strides[0] = (cuuint64_t)inner; box[0] = 32; sw = CU_TENSOR_MAP_SWIZZLE_NONE; break;
         default: return fail(MXFP6_ERR_BAD_ARG, "make_map: unknown kind %d", kind);
     }
     CUresult r = encode(out, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
@@ -236,11 +259,16 @@ static int make_map(const void* ptr, int64_t rows, int64_t inner, int box_rows, 
 }
 
 // ---------------------------------------------------------------------------------- operand formats
-static bool fmt_valid(int f) { return f == MXFP6_E2M3 || f == MXFP6_E3M2 || f == MXFP8_E4M3 || f == MXFP8_E5M2; }
-static bool fmt_is_fp8(int f) { return f == MXFP8_E4M3 || f == MXFP8_E5M2; }
-static int fmt_row_bytes_per_128(int f) { return fmt_is_fp8(f) ? 128 : 96; }   // bytes of 128 elements in HBM
+static_assert(kE2M3 == MXFP6_E2M3 && kE3M2 == MXFP6_E3M2 && kE4M3 == MXFP8_E4M3 && kE5M2 == MXFP8_E5M2 && kE2M1 == MXFP4_E2M1, "format codes");
+#define MXFP6_FORMATS "MXFP6_E2M3 (0), MXFP6_E3M2 (1), MXFP8_E4M3 (2), MXFP8_E5M2 (3) or MXFP4_E2M1 (4)"
+static bool fmt_valid(int f) { return f >= MXFP6_E2M3 && f <= MXFP4_E2M1; }
+static bool fmt_is_fp8(int f) { return fmt_fp8(f); }
+static int fmt_row_bytes_per_128(int f) { return 4 * fmt_block_bytes(f); }   // bytes of 128 elements in HBM
+static int64_t fmt_row_bytes(int64_t n, int f) { return n / 32 * fmt_block_bytes(f); }   // bytes of n elements (n % 32 == 0)
+static int fmt_map_kind(int f) { return fmt_is_fp8(f) ? 3 : f == MXFP4_E2M1 ? 8 : 0; }   // tensor map of an operand of kind::mxf8f6f4
+static int fmt_out_map_kind(int f) { return fmt_is_fp8(f) ? 7 : f == MXFP4_E2M1 ? 9 : 6; }   // tensor map of a re-quantised result
 static uint32_t fmt_mma_code(int f) {      // operand format field of kind::mxf8f6f4
-    return f == MXFP6_E2M3 ? kFmtE2M3 : f == MXFP6_E3M2 ? kFmtE3M2 : f == MXFP8_E4M3 ? 0u : 1u;
+    return f == MXFP6_E2M3 ? kFmtE2M3 : f == MXFP6_E3M2 ? kFmtE3M2 : f == MXFP8_E4M3 ? kFmtE4M3 : f == MXFP8_E5M2 ? kFmtE5M2 : kFmtE2M1;
 }
 
 // ---------------------------------------------------------------------------------- GEMM dispatch
@@ -533,7 +561,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     if (M < 0 || N < 0 || K < 0) return fail(MXFP6_ERR_BAD_ARG, "negative dimension (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
     if (K % 128 != 0) return fail(MXFP6_ERR_BAD_ARG, "K=%lld must be a multiple of 128", (long long)K);
     if (!fmt_valid(fmt_a) || !fmt_valid(fmt_b))
-        return fail(MXFP6_ERR_BAD_ARG, "format must be MXFP6_E2M3 (0), MXFP6_E3M2 (1), MXFP8_E4M3 (2) or MXFP8_E5M2 (3)");
+        return fail(MXFP6_ERR_BAD_ARG, "format must be " MXFP6_FORMATS);
     if (M > 0x7fffff00LL || N > 0x7fffff00LL || K > 0x7fffff00LL) return fail(MXFP6_ERR_BAD_ARG, "dimension too large");
     if (M == 0 || N == 0) return MXFP6_OK;
     if (!c) return fail(MXFP6_ERR_BAD_ARG, "null C");
@@ -550,7 +578,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     }
     if (!a || !b || !sfa || !sfb) return fail(MXFP6_ERR_BAD_ARG, "null operand pointer");
     if (((uintptr_t)a & (fmt_is_fp8(fmt_a) ? 15 : 31)) || ((uintptr_t)b & (fmt_is_fp8(fmt_b) ? 15 : 31)))
-        return fail(MXFP6_ERR_BAD_ARG, "operands must be 32-byte aligned (fp6) / 16-byte aligned (fp8)");
+        return fail(MXFP6_ERR_BAD_ARG, "operands must be 32-byte aligned (fp6, fp4) / 16-byte aligned (fp8)");
     if (((uintptr_t)sfa & 3) || ((uintptr_t)sfb & 3)) return fail(MXFP6_ERR_BAD_ARG, "scale arrays must be 4-byte aligned");
 
     DeviceState* dp = nullptr;
@@ -590,10 +618,10 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     const int fp = pl.swap ? fmt_b : fmt_a, fq = pl.swap ? fmt_a : fmt_b;
 
     const int p_box = pl.pair ? 128 : pl.p_tile, q_box = pl.pair ? 128 : pl.q_tile;      // rows one operand load brings
-    if ((rc = make_map(pp, prow, K, p_box, fmt_is_fp8(fp) ? 3 : 0, &r.tp))) return rc;
-    if ((rc = make_map(qp, qrow, K, q_box, fmt_is_fp8(fq) ? 3 : 0, &r.tq))) return rc;
+    if ((rc = make_map(pp, prow, K, p_box, fmt_map_kind(fp), &r.tp))) return rc;
+    if ((rc = make_map(qp, qrow, K, q_box, fmt_map_kind(fq), &r.tq))) return rc;
     r.tq_tail = r.tq;
-    if (pl.pair && pl.tail_split > 1 && (rc = make_map(qp, qrow, K, 128 / pl.tail_split, fmt_is_fp8(fq) ? 3 : 0, &r.tq_tail))) return rc;
+    if (pl.pair && pl.tail_split > 1 && (rc = make_map(qp, qrow, K, 128 / pl.tail_split, fmt_map_kind(fq), &r.tq_tail))) return rc;
     if (sf_tma) {
         if ((rc = make_map(sp, prow, K / 32, p_box, 1, &r.tsp))) return rc;
         if ((rc = make_map(sq, qrow, K / 32, pl.q_tile, 1, &r.tsq))) return rc;   // pair kernel: all 256 Q rows per CTA
@@ -636,7 +664,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     P.idesc = make_idesc_m(fmt_mma_code(fp), fmt_mma_code(fq), pl.pair ? 256u : 128u, mma_n);
     P.sf_tma = sf_tma ? 1 : 0;
     P.sf_ld = (int)(K / 32);
-    // bytes a stage's two loads credit to its mbarrier: the global bytes of the boxes (fp6: 96 per 128 elements)
+    // bytes a stage's two loads credit to its mbarrier: the global bytes of the boxes (fp6: 96, fp4: 64 per 128 elements)
     P.stage_tx_bytes = p_box * fmt_row_bytes_per_128(fp) + q_box * fmt_row_bytes_per_128(fq);
     P.tail_first = pl.tail_first; P.tail_split = pl.tail_split;
     P.stage_tx_bytes_tail = p_box * fmt_row_bytes_per_128(fp) + (128 / pl.tail_split) * fmt_row_bytes_per_128(fq);
@@ -652,7 +680,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     P.c_tma_last = (!pl.pair && !pl.swap && o.c_tma_last && q_fmt < 0 && dst.n == 1 && dest_by_tma(dst) &&
                     (pl.p_tile == 128 || pl.tiles_p == 1)) ? 1 : 0;
     P.q_out = (uint8_t*)q_out; P.q_scales = (uint8_t*)q_scales; P.q_fmt = q_fmt;
-    P.q_ld = q_fmt < 0 ? 0 : (fmt_is_fp8(q_fmt) ? N : N * 3 / 4);
+    P.q_ld = q_fmt < 0 ? 0 : fmt_row_bytes(N, q_fmt);
     P.ws_counter = (unsigned int*)ws;
     P.ws_partial = ws ? (float*)((uint8_t*)ws + pl.ws_counter_bytes) : nullptr;
     P.ws_slots = pl.ws_slots;
@@ -682,7 +710,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
         for (int i = 0; i < 8; ++i) {
             if (i >= dst.n) { r.cm.m[i] = r.cm.m[0]; continue; }     // unused slots hold a valid map all the same
             if (q_fmt >= 0) {       // the pieces of a re-quantised result are code bytes, not bf16
-                if ((rc = make_map(q_out, M, fmt_is_fp8(q_fmt) ? N : N * 3 / 4, 128, fmt_is_fp8(q_fmt) ? 7 : 6, &r.cm.m[i]))) return rc;
+                if ((rc = make_map(q_out, M, fmt_row_bytes(N, q_fmt), 128, fmt_out_map_kind(q_fmt), &r.cm.m[i]))) return rc;
             } else if (!P.c_tma) {
                 r.cm.m[i] = r.tp;       // plain stores: the slot only has to hold a valid map
             } else if ((rc = make_map(dst.c[i], M, N, 128, 2, &r.cm.m[i], dst.ldc * 2))) return rc;
@@ -733,7 +761,7 @@ template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bflo
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ src, int64_t n_quads, uint32_t* __restrict__ packed_words,
                                                        uint8_t* __restrict__ scales) {
-    constexpr int EMAX = FMT == MXFP6_E2M3 ? 2 : FMT == MXFP6_E3M2 ? 4 : FMT == MXFP8_E4M3 ? 8 : 15;
+    constexpr int EMAX = FMT == MXFP6_E2M3 || FMT == MXFP4_E2M1 ? 2 : FMT == MXFP6_E3M2 ? 4 : FMT == MXFP8_E4M3 ? 8 : 15;
     constexpr bool FP8 = FMT == MXFP8_E4M3 || FMT == MXFP8_E5M2;
     const int lane = threadIdx.x & 31;
     // n_quads is a multiple of 8, so whole warps share the loop trip count up to the tail handled by `live`;
@@ -764,6 +792,10 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ src
         if constexpr (FP8) {
             // one byte per element: this thread's 4 codes are one 32-bit word of the operand
             if (live) packed_words[q] = w;
+        } else if constexpr (FMT == MXFP4_E2M1) {
+            // two lanes hold 2 x 16 bits = one word
+            const uint32_t wn = __shfl_down_sync(0xffffffffu, w, 1);
+            if (live && (lane & 1) == 0) packed_words[q >> 1] = w | (wn << 16);
         } else {
             // 4 lanes hold 4 x 24 bits = three 32-bit words of the packed stream
             const uint32_t wn = __shfl_down_sync(0xffffffffu, w, 1);
@@ -771,41 +803,6 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ src
             if (live && i4 < 3) packed_words[(q >> 2) * 3 + i4] = (w >> (8 * i4)) | (wn << (24 - 8 * i4));
         }
         if (live && (lane & 7) == 0) scales[q >> 3] = (uint8_t)sb;
-    }
-}
-
-template <int FMT>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ packed, const uint8_t* __restrict__ scales,
-                                                         int64_t n_quads, float* __restrict__ out) {
-    constexpr bool FP8 = FMT == MXFP8_E4M3 || FMT == MXFP8_E5M2;
-    constexpr int BITS = FP8 ? 8 : 6;
-    constexpr int MB = (FMT == MXFP6_E2M3 || FMT == MXFP8_E4M3) ? 3 : 2;
-    constexpr int EB = BITS - 1 - MB;
-    constexpr int BIAS = FMT == MXFP6_E2M3 ? 1 : FMT == MXFP6_E3M2 ? 3 : FMT == MXFP8_E4M3 ? 7 : 15;
-    for (int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; q < n_quads; q += (int64_t)gridDim.x * blockDim.x) {
-        uint32_t w;
-        if constexpr (FP8) {
-            w = *reinterpret_cast<const uint32_t*>(packed + q * 4);
-        } else {
-            const uint8_t* p = packed + q * 3;
-            w = (uint32_t)p[0] | ((uint32_t)p[1] << 8) | ((uint32_t)p[2] << 16);
-        }
-        const uint32_t sbyte = scales[q >> 3];
-        // 2^(sbyte-127) as fp32 (sbyte 0 -> 2^-127, an fp32 subnormal)
-        const float s = sbyte == 255 ? __uint_as_float(0x7fc00000u) : sbyte == 0 ? __uint_as_float(0x00400000u) : __uint_as_float(sbyte << 23);
-        float4 o;
-        float* of = reinterpret_cast<float*>(&o);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t c = (w >> (BITS * i)) & ((1u << BITS) - 1);
-            const uint32_t e = (c >> MB) & ((1u << EB) - 1), m = c & ((1u << MB) - 1);
-            float mag = e ? __uint_as_float(((e - BIAS + 127) << 23) | (m << (23 - MB)))
-                          : (float)m * __uint_as_float((uint32_t)(1 - BIAS - MB + 127) << 23);
-            if (FMT == MXFP8_E4M3 && e == 15 && m == 7) mag = __uint_as_float(0x7fc00000u);
-            if (FMT == MXFP8_E5M2 && e == 31) mag = m ? __uint_as_float(0x7fc00000u) : __uint_as_float(0x7f800000u);
-            of[i] = ((c >> (BITS - 1)) ? -mag : mag) * s;
-        }
-        *reinterpret_cast<float4*>(out + q * 4) = o;
     }
 }
 
@@ -884,7 +881,7 @@ extern "C" int mxfp6_gemm_requant(const void* a, const void* sfa, const void* b,
     if ((uintptr_t)out & 15) return fail(MXFP6_ERR_BAD_ARG, "requant: output must be 16-byte aligned");
     if ((uintptr_t)out_scales & 1) return fail(MXFP6_ERR_BAD_ARG, "requant: out_scales must be 2-byte aligned");
     if (K == 0 && M > 0 && N > 0) {   // all-zero result: codes 0, scale byte 0
-        CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)M * (fmt_is_fp8(out_fmt) ? N : N * 3 / 4), (cudaStream_t)stream));
+        CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)(M * fmt_row_bytes(N, out_fmt)), (cudaStream_t)stream));
         CUDA_TRY(cudaMemsetAsync(out_scales, 0, (size_t)M * (N / 32), (cudaStream_t)stream));
         return MXFP6_OK;
     }
@@ -1134,10 +1131,12 @@ extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int6
         } while (0)
         if (src_dtype == 0) {
             if (fmt == MXFP6_E2M3) QT(float, MXFP6_E2M3); else if (fmt == MXFP6_E3M2) QT(float, MXFP6_E3M2);
-            else if (fmt == MXFP8_E4M3) QT(float, MXFP8_E4M3); else QT(float, MXFP8_E5M2);
+            else if (fmt == MXFP8_E4M3) QT(float, MXFP8_E4M3); else if (fmt == MXFP8_E5M2) QT(float, MXFP8_E5M2);
+            else QT(float, MXFP4_E2M1);
         } else {
             if (fmt == MXFP6_E2M3) QT(__nv_bfloat16, MXFP6_E2M3); else if (fmt == MXFP6_E3M2) QT(__nv_bfloat16, MXFP6_E3M2);
-            else if (fmt == MXFP8_E4M3) QT(__nv_bfloat16, MXFP8_E4M3); else QT(__nv_bfloat16, MXFP8_E5M2);
+            else if (fmt == MXFP8_E4M3) QT(__nv_bfloat16, MXFP8_E4M3); else if (fmt == MXFP8_E5M2) QT(__nv_bfloat16, MXFP8_E5M2);
+            else QT(__nv_bfloat16, MXFP4_E2M1);
         }
 #undef QT
         CUDA_TRY(cudaGetLastError());
@@ -1146,37 +1145,56 @@ extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int6
 #define QK(T, F) quantize_kernel<T, F><<<(unsigned)blocks, 256, 0, st>>>((const T*)src, nq, (uint32_t*)packed, (uint8_t*)scales)
     if (src_dtype == 0) {
         if (fmt == MXFP6_E2M3) QK(float, MXFP6_E2M3); else if (fmt == MXFP6_E3M2) QK(float, MXFP6_E3M2);
-        else if (fmt == MXFP8_E4M3) QK(float, MXFP8_E4M3); else QK(float, MXFP8_E5M2);
+        else if (fmt == MXFP8_E4M3) QK(float, MXFP8_E4M3); else if (fmt == MXFP8_E5M2) QK(float, MXFP8_E5M2);
+        else QK(float, MXFP4_E2M1);
     } else {
         if (fmt == MXFP6_E2M3) QK(__nv_bfloat16, MXFP6_E2M3); else if (fmt == MXFP6_E3M2) QK(__nv_bfloat16, MXFP6_E3M2);
-        else if (fmt == MXFP8_E4M3) QK(__nv_bfloat16, MXFP8_E4M3); else QK(__nv_bfloat16, MXFP8_E5M2);
+        else if (fmt == MXFP8_E4M3) QK(__nv_bfloat16, MXFP8_E4M3); else if (fmt == MXFP8_E5M2) QK(__nv_bfloat16, MXFP8_E5M2);
+        else QK(__nv_bfloat16, MXFP4_E2M1);
     }
 #undef QK
     CUDA_TRY(cudaGetLastError());
     return MXFP6_OK;
 }
 
-extern "C" int mxfp6_dequantize(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out_f32,
-                                void* stream) {
+template <int F, typename T>
+static int launch_dequantize(const DeviceState& d, const uint8_t* packed, const uint8_t* scales, int64_t n_oct, T* out, cudaStream_t st) {
+    // four octets per thread; the grid covers the device eight times over at most
+    int64_t blocks = (n_oct + 4 * 256 - 1) / (4 * 256);
+    if (blocks > (int64_t)d.sm_count * 8) blocks = (int64_t)d.sm_count * 8;
+    constexpr int B = fmt_block_bytes(F) / 4;       // code bytes of an octet: loaded whole when the pointer allows it
+    const uintptr_t need = B == 6 ? 1 : (uintptr_t)(B - 1);
+    const bool vec = !((uintptr_t)packed & need) && !((uintptr_t)out & 31);
+    return launch_pdl(vec ? dequantize_kernel<F, T, true> : dequantize_kernel<F, T, false>, (unsigned)blocks, 256, 0, st, packed, scales, n_oct, out);
+}
+
+extern "C" int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out,
+                                   int out_dtype, void* stream) {
     if (rows < 0 || K < 0 || K % 32) return fail(MXFP6_ERR_BAD_ARG, "dequantize: rows=%lld K=%lld (K must be a multiple of 32)", (long long)rows, (long long)K);
     if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "dequantize: bad format %d", fmt);
+    if (out_dtype != 0 && out_dtype != 1) return fail(MXFP6_ERR_BAD_ARG, "dequantize: out_dtype must be 0 (fp32) or 1 (bf16)");
     if (rows == 0 || K == 0) return MXFP6_OK;
-    if (!packed || !scales || !out_f32) return fail(MXFP6_ERR_BAD_ARG, "dequantize: null pointer");
-    if ((uintptr_t)out_f32 & 15) return fail(MXFP6_ERR_BAD_ARG, "dequantize: output must be 16-byte aligned");
+    if (!packed || !scales || !out) return fail(MXFP6_ERR_BAD_ARG, "dequantize: null pointer");
+    if ((uintptr_t)out & 15) return fail(MXFP6_ERR_BAD_ARG, "dequantize: output must be 16-byte aligned");
     DeviceState* d = nullptr;
     int rc = get_device_state(&d);
     if (rc) return rc;
-    const int64_t nq = rows * K / 4;
-    int64_t blocks = (nq + 255) / 256;
-    const int64_t cap = (int64_t)d->sm_count * 16;
-    if (blocks > cap) blocks = cap;
     cudaStream_t st = (cudaStream_t)stream;
-#define DQ(F) dequantize_kernel<F><<<(unsigned)blocks, 256, 0, st>>>((const uint8_t*)packed, (const uint8_t*)scales, nq, (float*)out_f32)
-    if (fmt == MXFP6_E2M3) DQ(MXFP6_E2M3); else if (fmt == MXFP6_E3M2) DQ(MXFP6_E3M2);
-    else if (fmt == MXFP8_E4M3) DQ(MXFP8_E4M3); else DQ(MXFP8_E5M2);
+    const int64_t n_oct = rows * K / 8;
+    const uint8_t *p = (const uint8_t*)packed, *s = (const uint8_t*)scales;
+#define DQ(F) (out_dtype == 0 ? launch_dequantize<F>(*d, p, s, n_oct, (float*)out, st) : launch_dequantize<F>(*d, p, s, n_oct, (__nv_bfloat16*)out, st))
+    switch (fmt) {
+        case MXFP6_E2M3: return DQ(MXFP6_E2M3);
+        case MXFP6_E3M2: return DQ(MXFP6_E3M2);
+        case MXFP8_E4M3: return DQ(MXFP8_E4M3);
+        case MXFP8_E5M2: return DQ(MXFP8_E5M2);
+        default: return DQ(MXFP4_E2M1);
+    }
 #undef DQ
-    CUDA_TRY(cudaGetLastError());
-    return MXFP6_OK;
+}
+
+extern "C" int mxfp6_dequantize(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out_f32, void* stream) {
+    return mxfp6_dequantize_ex(packed, scales, rows, K, fmt, out_f32, 0, stream);
 }
 
 extern "C" int mxfp6_device_status(int* status_out) {

@@ -200,7 +200,7 @@ __device__ __forceinline__ uint64_t smem_desc_sf(uint32_t saddr) {
 }
 
 // Operand format codes of kind::mxf8f6f4
-constexpr uint32_t kFmtE2M3 = 3, kFmtE3M2 = 4;
+constexpr uint32_t kFmtE4M3 = 0, kFmtE5M2 = 1, kFmtE2M3 = 3, kFmtE3M2 = 4, kFmtE2M1 = 5;
 
 // Instruction descriptor for the block-scaled MMA: M=128, N=n, both operands K-major, E8M0 scales,
 // fp32 accumulate.  sf_id (0..3) selects which byte of the 32-bit scale column this K=32 step uses.

@@ -9,14 +9,23 @@
 namespace mxfp6 {
 
 // format codes of the C ABI
-constexpr int kE2M3 = 0, kE3M2 = 1, kE4M3 = 2, kE5M2 = 3;
+constexpr int kE2M3 = 0, kE3M2 = 1, kE4M3 = 2, kE5M2 = 3, kE2M1 = 4;
 
-__device__ __forceinline__ int quant_emax(int fmt) { return fmt == kE2M3 ? 2 : fmt == kE3M2 ? 4 : fmt == kE4M3 ? 8 : 15; }
+__host__ __device__ constexpr bool fmt_fp8(int fmt) { return fmt == kE4M3 || fmt == kE5M2; }
+// operand bytes of one block of 32 elements: 8, 6 or 4 bits each
+__host__ __device__ constexpr int fmt_block_bytes(int fmt) { return fmt_fp8(fmt) ? 32 : fmt == kE2M1 ? 16 : 24; }
+
+__device__ __forceinline__ int quant_emax(int fmt) { return fmt == kE2M3 || fmt == kE2M1 ? 2 : fmt == kE3M2 ? 4 : fmt == kE4M3 ? 8 : 15; }
 
 // Hardware conversion of two fp32 values at once (round to nearest even, saturate to the largest finite value):
-// returns code(x0) | code(x1) << 8, fp6 codes in the low 6 bits of their byte.
+// returns code(x0) | code(x1) << 8, fp6 codes in the low 6 bits of their byte; for E2M1 code(x0) | code(x1) << 4.
 template <int FMT>
 __device__ __forceinline__ uint32_t cvt_pair(float x0, float x1) {
+    if constexpr (FMT == kE2M1) {
+        uint32_t b;
+        asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(b) : "f"(x1), "f"(x0));
+        return b;
+    }
     uint16_t r;
     if constexpr (FMT == kE2M3) asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x1), "f"(x0));
     else if constexpr (FMT == kE3M2) asm("cvt.rn.satfinite.e3m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x1), "f"(x0));
@@ -24,16 +33,29 @@ __device__ __forceinline__ uint32_t cvt_pair(float x0, float x1) {
     else asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(x1), "f"(x0));
     return r;
 }
+// eight values -> eight E2M1 codes in one word, lowest nibble first
+__device__ __forceinline__ uint32_t cvt_oct_e2m1(const float* x) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+    return r;
+}
 __device__ __forceinline__ uint32_t mad_u32(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
-// four values -> 4 codes: fp8 one per byte (32 bits), fp6 6 bits each (24 bits)
+// four values -> 4 codes: fp8 one per byte (32 bits), fp6 6 bits each (24 bits), fp4 4 bits each (16 bits)
 template <int FMT>
 __device__ __forceinline__ uint32_t cvt_quad(float x0, float x1, float x2, float x3) {
     const uint32_t lo = cvt_pair<FMT>(x0, x1), hi = cvt_pair<FMT>(x2, x3);
     if constexpr (FMT == kE4M3 || FMT == kE5M2) return lo | (hi << 16);          // one code per byte
+    if constexpr (FMT == kE2M1) return lo | (hi << 8);
     // a pair is c0 + 256*c1; the 12-bit form c0 + 64*c1 is pair - 192*(pair >> 8), and two 12-bit forms join by
     // one more multiply-add: integer multiply-adds run on the FMA pipe, which this code leaves idle, not on the ALU
     const uint32_t lo12 = mad_u32(lo >> 8, 0xffffff40u, lo), hi12 = mad_u32(hi >> 8, 0xffffff40u, hi);
@@ -69,7 +91,7 @@ __device__ __forceinline__ float amax32(const float* v) {
     return amax3(amax3(a, b, c), m[9], m[10]);
 }
 
-// v[0..31] (fp32) with largest magnitude amax -> out[0..5] (fp6: 24 bytes) or out[0..7] (fp8: 32 bytes); returns
+// v[0..31] (fp32) with largest magnitude amax -> out[0..3] (fp4: 16 bytes), out[0..5] (fp6: 24 bytes) or out[0..7] (fp8: 32 bytes); returns
 // the scale byte
 template <int FMT>
 __device__ __forceinline__ int quant_block32_amax(const float* v, float amax, uint32_t* out) {
@@ -82,6 +104,14 @@ __device__ __forceinline__ int quant_block32_amax(const float* v, float amax, ui
 #pragma unroll
         for (int g = 0; g < 8; ++g)
             out[g] = cvt_quad<FMT>(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+    } else if constexpr (FMT == kE2M1) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float s[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = v[8 * g + i] * f;
+            out[g] = cvt_oct_e2m1(s);
+        }
     } else {
         uint32_t w24[8];
 #pragma unroll
@@ -109,14 +139,16 @@ __device__ __forceinline__ uint32_t cvt_one(float x, int fmt) {
     if (fmt == kE2M3) r = cvt_pair<kE2M3>(x, 0.f);
     else if (fmt == kE3M2) r = cvt_pair<kE3M2>(x, 0.f);
     else if (fmt == kE4M3) r = cvt_pair<kE4M3>(x, 0.f);
-    else r = cvt_pair<kE5M2>(x, 0.f);
+    else if (fmt == kE5M2) r = cvt_pair<kE5M2>(x, 0.f);
+    else r = cvt_pair<kE2M1>(x, 0.f);
     return r & 0xffu;
 }
 __device__ __forceinline__ uint32_t cvt_quad_rt(float x0, float x1, float x2, float x3, int fmt) {
     if (fmt == kE2M3) return cvt_quad<kE2M3>(x0, x1, x2, x3);
     if (fmt == kE3M2) return cvt_quad<kE3M2>(x0, x1, x2, x3);
     if (fmt == kE4M3) return cvt_quad<kE4M3>(x0, x1, x2, x3);
-    return cvt_quad<kE5M2>(x0, x1, x2, x3);
+    if (fmt == kE5M2) return cvt_quad<kE5M2>(x0, x1, x2, x3);
+    return cvt_quad<kE2M1>(x0, x1, x2, x3);
 }
 __device__ __forceinline__ float quant_inv_scale(int sb) {          // 2^-(sb-127)
     const int e = sb - 127;
@@ -125,7 +157,7 @@ __device__ __forceinline__ float quant_inv_scale(int sb) {          // 2^-(sb-12
 
 // A block of 32 consecutive columns of output row `row` whose elements sit one per lane of a warp (lane = column
 // within the block): scale from the warp-wide largest magnitude, one conversion per lane, and the codes leave as
-// 32 bytes (fp8) or, gathered by four lanes at a time, as six 32-bit words (fp6).  Whole warp, converged.
+// 32 bytes (fp8) or, gathered by several lanes at a time, as six (fp6) or four (fp4) 32-bit words.  Whole warp, converged.
 __device__ __forceinline__ void quant_store_lanes(float x, int fmt, uint8_t* q_out, size_t q_ld, uint8_t* q_scales,
                                                   int n_cols, int row, int col0, bool row_valid) {
     const int lane = threadIdx.x & 31;
@@ -135,6 +167,12 @@ __device__ __forceinline__ void quant_store_lanes(float x, int fmt, uint8_t* q_o
     const bool fp8 = fmt == kE4M3 || fmt == kE5M2;
     if (fp8) {
         if (row_valid) q_out[(size_t)row * q_ld + col0 + lane] = (uint8_t)code;
+    } else if (fmt == kE2M1) {
+        // every eighth lane gathers eight nibbles
+        uint32_t w = code | (__shfl_down_sync(0xffffffffu, code, 1) << 4);
+        w |= __shfl_down_sync(0xffffffffu, w, 2) << 8;
+        w |= __shfl_down_sync(0xffffffffu, w, 4) << 16;
+        if (row_valid && (lane & 7) == 0) reinterpret_cast<uint32_t*>(q_out + (size_t)row * q_ld + col0 / 2)[lane >> 3] = w;
     } else {
         // lanes 4j: 24 bits of the four codes 4j..4j+3; then lanes 4j, 4j+1, 4j+2 of every 16 write one word each
         uint32_t w = code | (__shfl_down_sync(0xffffffffu, code, 1) << 6) | (__shfl_down_sync(0xffffffffu, code, 2) << 12) |
@@ -165,6 +203,9 @@ __device__ __forceinline__ void quant_store_lanes4(const float (&x)[4], int fmt,
     const int j = lane & 7;                                   // this lane's 4 columns: col0 + 4j ..
     if (fp8) {
         if (row_valid) reinterpret_cast<uint32_t*>(q_out + (size_t)row * q_ld + col0)[j] = w;
+    } else if (fmt == kE2M1) {
+        const uint32_t wn = __shfl_down_sync(0xffffffffu, w, 1);
+        if (row_valid && (j & 1) == 0) reinterpret_cast<uint32_t*>(q_out + (size_t)row * q_ld + col0 / 2)[j >> 1] = w | (wn << 16);
     } else {
         // lanes 4g..4g+3 hold 4 x 24 bits = three 32-bit words of the packed stream
         const uint32_t wn = __shfl_down_sync(0xffffffffu, w, 1);
@@ -188,13 +229,14 @@ __device__ __forceinline__ void quant_store32(const uint32_t* vbits, int fmt, ui
     if (fmt == kE2M3) sb = quant_block32<kE2M3>(v, w);
     else if (fmt == kE3M2) sb = quant_block32<kE3M2>(v, w);
     else if (fmt == kE4M3) sb = quant_block32<kE4M3>(v, w);
-    else sb = quant_block32<kE5M2>(v, w);
-    uint8_t* dst = q_out + (size_t)row * q_ld + (fp8 ? col : col / 4 * 3);
-    // 24 (fp6) or 32 (fp8) bytes; 8-byte aligned in both cases when q_ld % 8 == 0 and col % 32 == 0
+    else if (fmt == kE5M2) sb = quant_block32<kE5M2>(v, w);
+    else sb = quant_block32<kE2M1>(v, w);
+    uint8_t* dst = q_out + (size_t)row * q_ld + col / 32 * fmt_block_bytes(fmt);
+    // 16 (fp4), 24 (fp6) or 32 (fp8) bytes; 8-byte aligned in all cases when q_ld % 8 == 0 and col % 32 == 0
     uint2* d2 = reinterpret_cast<uint2*>(dst);
     d2[0] = make_uint2(w[0], w[1]);
     d2[1] = make_uint2(w[2], w[3]);
-    d2[2] = make_uint2(w[4], w[5]);
+    if (fmt != kE2M1) d2[2] = make_uint2(w[4], w[5]);
     if (fp8) d2[3] = make_uint2(w[6], w[7]);
     q_scales[(size_t)row * (n_cols / 32) + col / 32] = (uint8_t)sb;
 }

@@ -1,15 +1,15 @@
 // Block quantiser fp32 / bf16 [rows, K] -> MX operand bytes + E8M0 scales, as a streaming kernel: HBM-bound
-// byte work (reads 4 or 2 bytes per element, writes 0.78 or 1.03).
+// byte work (reads 4 or 2 bytes per element, writes 0.53, 0.78 or 1.03).
 //
 // The source is one long run of 32-element blocks (K % 32 == 0, rows contiguous), the outputs are one run of
-// 24- or 32-byte code groups and one run of scale bytes, so the kernel is one-dimensional over blocks:
+// 16-, 24- or 32-byte code groups and one run of scale bytes, so the kernel is one-dimensional over blocks:
 //
 //   warp 0      one elected thread TMA-loads tiles of 128 blocks (16 KB of fp32 / 8 KB of bf16) into a ring of
 //               shared-memory stages; the tensor map views the source as [blocks, 32] with the 128-byte (fp32) or
 //               64-byte (bf16) swizzle, so that 128 threads can each read their own block without bank conflicts
 //   warps 1-4   thread t quantises block t of the tile (amax, scale byte, hardware cvt, 6-bit packing), stores its
-//               scale byte, writes its 24/32 code bytes to a staging buffer, and one lane per warp sends the warp's
-//               768 / 1024 code bytes with one bulk copy; the warps never wait for each other
+//               scale byte, writes its 16/24/32 code bytes to a staging buffer, and one lane per warp sends the warp's
+//               512 / 768 / 1024 code bytes with one bulk copy; the warps never wait for each other
 //
 // Persistent: four (fp32) or seven (bf16: what registers and shared memory allow; 35.4 us against 37.1 us with six for
 // an 8192 x 8192 source) CTAs per SM (a single group of four consumer warps cannot hide its own latencies), tiles dealt
@@ -35,9 +35,9 @@ struct QuantCfg {
     // several CTAs per SM: one group of four consumer warps cannot hide its own latencies
     static constexpr int CTAS_PER_SM = sizeof(T) == 4 ? 4 : 7;
     static constexpr int STAGES = 3;                                 // per SM 192 KB (fp32) / 168 KB (bf16) of loads in flight
-    static constexpr bool FP8 = FMT == kE4M3 || FMT == kE5M2;
-    static constexpr int OUT_ROW = FP8 ? 32 : 24;                    // code bytes of one block
-    static constexpr int OUT_BYTES = TILE_BLOCKS * OUT_ROW;          // 4 KB or 3 KB, a multiple of 16
+    static constexpr bool FP8 = fmt_fp8(FMT);
+    static constexpr int OUT_ROW = fmt_block_bytes(FMT);             // code bytes of one block
+    static constexpr int OUT_BYTES = TILE_BLOCKS * OUT_ROW;          // 4, 3 or 2 KB, a multiple of 16
     static constexpr int OUT_BUFS = 2;
     static constexpr int THREADS = 32 + TILE_BLOCKS;
     static constexpr int SMEM_BYTES = STAGES * IN_BYTES + OUT_BUFS * OUT_BYTES + 2 * STAGES * 8 + 16;
@@ -115,7 +115,7 @@ quantize_tma_kernel(const __grid_constant__ CUtensorMap tm_src, long long n_bloc
     } else {
         // ------------------------------------------------------------------ consumers: thread t <-> block t of the tile
         // The four consumer warps never wait for each other: each takes its 32 blocks from the stage, and sends its own
-        // 768 / 1024 code bytes with one bulk copy from its own slice of the staging buffers.
+        // 512 / 768 / 1024 code bytes with one bulk copy from its own slice of the staging buffers.
         const int t = threadIdx.x - 32;
         const int cw = t >> 5;                               // consumer warp 0..3
         uint32_t n = 0, s = 0, phase = 0;
@@ -168,7 +168,7 @@ quantize_tma_kernel(const __grid_constant__ CUtensorMap tm_src, long long n_bloc
                 uint2* o = reinterpret_cast<uint2*>(smem_gen + out_off + ob * Cfg::OUT_BYTES + t * Cfg::OUT_ROW);
                 o[0] = make_uint2(w[0], w[1]);
                 o[1] = make_uint2(w[2], w[3]);
-                o[2] = make_uint2(w[4], w[5]);
+                if constexpr (Cfg::OUT_ROW >= 24) o[2] = make_uint2(w[4], w[5]);
                 if constexpr (Cfg::FP8) o[3] = make_uint2(w[6], w[7]);
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -182,7 +182,7 @@ quantize_tma_kernel(const __grid_constant__ CUtensorMap tm_src, long long n_bloc
                 uint2* o = reinterpret_cast<uint2*>(packed + blk * Cfg::OUT_ROW);
                 o[0] = make_uint2(w[0], w[1]);
                 o[1] = make_uint2(w[2], w[3]);
-                o[2] = make_uint2(w[4], w[5]);
+                if constexpr (Cfg::OUT_ROW >= 24) o[2] = make_uint2(w[4], w[5]);
                 if constexpr (Cfg::FP8) o[3] = make_uint2(w[6], w[7]);
             }
         }

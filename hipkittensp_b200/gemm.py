@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import E2M3, E3M2, E4M3, E5M2, check, lib
+from ._lib import E2M1, E2M3, E3M2, E4M3, E5M2, check, lib
 
 
 def _accept(t, name: str, dtype) -> None:
@@ -30,12 +30,19 @@ def _accept(t, name: str, dtype) -> None:
 
 
 def _k_of(t, fmt: int, name: str) -> int:
-    """K of an operand [rows, bytes]: 4 elements per 3 bytes for fp6, 1 per byte for fp8."""
+    """K of an operand [rows, bytes]: 4 elements per 3 bytes for fp6, 1 per byte for fp8, 2 per byte for fp4."""
     if fmt in (E4M3, E5M2):
         return t.shape[1]
+    if fmt == E2M1:
+        return 2 * t.shape[1]
     if t.shape[1] % 3:
         raise RuntimeError(f"{name}.shape[1] must be 3K/4 bytes")
     return t.shape[1] // 3 * 4
+
+
+def row_bytes(K: int, fmt: int) -> int:
+    """Bytes of an operand row of K elements."""
+    return K if fmt in (E4M3, E5M2) else K // 2 if fmt == E2M1 else K * 3 // 4
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -69,8 +76,8 @@ def _on_device_of(t):
 def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None = None, b_static: bool = False) -> None:
     """C[M,N] (bf16, in place) = A[M,K] @ B[N,K]^T.
 
-    A [M,3K/4] u8 and B [N,3K/4] u8 are packed fp6, or [rows,K] u8 for the fp8 formats (format `fmt`; `fmt_b` if
-    B differs),
+    A [M,3K/4] u8 and B [N,3K/4] u8 are packed fp6, [rows,K] u8 for the fp8 formats or [rows,K/2] u8 for fp4 (format
+    `fmt`; `fmt_b` if B differs),
     scale_A [M,K/32] u8 and scale_B [N,K/32] u8 are E8M0 bytes.  M is taken from A, N from C,
     K from A, as the reference does (256_256_64_32_with16x32.cpp:52-54).  b_static=True promises that B and
     scale_B are not written by the work queued just before this call (see MXFP6_FLAG_B_STATIC)."""
@@ -87,7 +94,7 @@ def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None
     if C.shape[0] != M:
         raise RuntimeError("C.shape[0] must equal A.shape[0]")
     if B.shape[0] != N or _k_of(B, fb, "B") != K:
-        raise RuntimeError("B must be [N, 3K/4] (fp6) or [N, K] (fp8) with the K of A")
+        raise RuntimeError("B must be [N, 3K/4] (fp6), [N, K] (fp8) or [N, K/2] (fp4) with the K of A")
     if tuple(scale_A.shape) != (M, K // 32) or tuple(scale_B.shape) != (N, K // 32):
         raise RuntimeError("scales must be [rows, K/32]")
     if len({t.device for t in (A, B, C, scale_A, scale_B)}) != 1:
@@ -161,7 +168,7 @@ def dispatch_copy_gather(A, B, dests, col_offset: int, scale_A, scale_B, scratch
 
 
 def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out_fmt: int = E2M3):
-    """C = A @ B^T delivered as an MX operand for the next layer: (operand bytes [M, 3N/4 | N], scales [M, N/32]),
+    """C = A @ B^T delivered as an MX operand for the next layer: (operand bytes [M, 3N/4 | N | N/2], scales [M, N/32]),
     quantised in the GEMM epilogue from the fp32 accumulators (blocks of 32 along N)."""
     _accept(A, "A", torch.uint8)
     _accept(B, "B", torch.uint8)
@@ -173,7 +180,7 @@ def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = No
         raise RuntimeError("A and B disagree on K")
     if N % 64:
         raise RuntimeError("N must be a multiple of 64")
-    out = torch.empty((M, N if out_fmt in (E4M3, E5M2) else N * 3 // 4), dtype=torch.uint8, device=A.device)
+    out = torch.empty((M, row_bytes(N, out_fmt)), dtype=torch.uint8, device=A.device)
     scales = torch.empty((M, N // 32), dtype=torch.uint8, device=A.device)
     with _on_device_of(A):
         check(lib.mxfp6_gemm_requant(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
@@ -224,7 +231,8 @@ def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=
 
 
 def quantize(x: torch.Tensor, fmt: int = E2M3):
-    """fp32 or bf16 [rows,K] on the GPU -> (operand bytes u8 [rows,3K/4] for fp6 / [rows,K] for fp8, scales u8 [rows,K/32])."""
+    """fp32 or bf16 [rows,K] on the GPU -> (operand bytes u8 [rows,3K/4] for fp6 / [rows,K] for fp8 / [rows,K/2] for fp4,
+    scales u8 [rows,K/32])."""
     if x.device.type == "cpu":
         raise RuntimeError("Tensor must be on CUDA device")
     if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() != 2 or not x.is_contiguous():
@@ -232,7 +240,7 @@ def quantize(x: torch.Tensor, fmt: int = E2M3):
     rows, K = x.shape
     if K % 32:
         raise RuntimeError("K must be a multiple of 32")
-    packed = torch.empty((rows, K if fmt in (E4M3, E5M2) else K * 3 // 4), dtype=torch.uint8, device=x.device)
+    packed = torch.empty((rows, row_bytes(K, fmt)), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, K // 32), dtype=torch.uint8, device=x.device)
     with _on_device_of(x):
         check(lib.mxfp6_quantize(x.data_ptr(), 0 if x.dtype == torch.float32 else 1, rows, K, fmt,
@@ -240,14 +248,21 @@ def quantize(x: torch.Tensor, fmt: int = E2M3):
     return packed, scales
 
 
-def dequantize(packed: torch.Tensor, scales: torch.Tensor, fmt: int = E2M3) -> torch.Tensor:
-    """(packed, scales) on the GPU -> fp32 [rows,K]."""
+def dequantize(packed: torch.Tensor, scales: torch.Tensor, fmt: int = E2M3, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """(packed, scales) on the GPU -> fp32 or bf16 [rows,K]."""
     _accept(packed, "packed", torch.uint8)
     _accept(scales, "scales", torch.uint8)
     rows, K = packed.shape[0], _k_of(packed, fmt, "packed")
-    out = torch.empty((rows, K), dtype=torch.float32, device=packed.device)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError("dtype must be torch.float32 or torch.bfloat16")
+    if K % 32 or tuple(scales.shape) != (rows, K // 32):
+        raise RuntimeError("scales must be [rows, K/32]")
+    if scales.device != packed.device:
+        raise RuntimeError("all tensors must be on the same device")
+    out = torch.empty((rows, K), dtype=dtype, device=packed.device)
     with _on_device_of(packed):
-        check(lib.mxfp6_dequantize(packed.data_ptr(), scales.data_ptr(), rows, K, fmt, out.data_ptr(), _stream_ptr()))
+        check(lib.mxfp6_dequantize_ex(packed.data_ptr(), scales.data_ptr(), rows, K, fmt, out.data_ptr(),
+                                      0 if dtype == torch.float32 else 1, _stream_ptr()))
     return out
 
 

@@ -132,11 +132,11 @@ def main(argv=None) -> None:
     ap.add_argument("--check", action="store_true", help="asserting run instead of the timing sweep")
     ap.add_argument("--quantize", action="store_true", help="time the block quantiser instead of the GEMM")
     ap.add_argument("--edge", action="store_true", help="time shapes off the preferred multiples instead of the reference's list")
-    ap.add_argument("--fmt", choices=["e2m3", "e3m2", "e4m3", "e5m2"], default="e2m3")
+    ap.add_argument("--fmt", choices=["e2m3", "e3m2", "e4m3", "e5m2", "e2m1"], default="e2m3")
     ap.add_argument("--warmup", type=int, default=500)
     ap.add_argument("--iters", type=int, default=500)
     args = ap.parse_args(argv)
-    fmt = {"e2m3": F.E2M3, "e3m2": F.E3M2, "e4m3": F.E4M3, "e5m2": F.E5M2}[args.fmt]
+    fmt = {"e2m3": F.E2M3, "e3m2": F.E3M2, "e4m3": F.E4M3, "e5m2": F.E5M2, "e2m1": F.E2M1}[args.fmt]
     torch.manual_seed(0)
     if args.quantize:
         print_title(f"MX {args.fmt} block quantiser (B200)")

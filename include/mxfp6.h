@@ -1,5 +1,5 @@
 /*
- * mxfp6.h -- C ABI of the B200 (sm_100a) MX-FP6 GEMM path.
+ * mxfp6.h -- C ABI of the B200 (sm_100a) MX-FP6 GEMM path (with MX-FP8 and MX-FP4 operands and the layer norm in front of it).
  *
  *   C[M,N] (bf16) = A[M,K] * B[N,K]^T
  *
@@ -42,6 +42,11 @@ extern "C" {
  * (The reference's main-branch GEMMs are fp8: kernels/gemm/fp8fp32/FP8_8wave/8_wave.cu.) */
 #define MXFP8_E4M3 2
 #define MXFP8_E5M2 3
+/* MX-FP4 operands (E2M1: +-0, 0.5, 1, 1.5, 2, 3, 4, 6): two codes per byte, the lower element in the low nibble, row-major
+ * [rows, K/2], 32-byte aligned, same E8M0 scale per 32 elements.  Every entry point that takes a format takes this one.
+ * The nibbles are spread to 8-bit slots on the way into shared memory and multiplied by kind::mxf8f6f4.
+ * (No counterpart in the reference.) */
+#define MXFP4_E2M1 4
 
 #define MXFP6_OK 0
 #define MXFP6_ERR_BAD_ARG 1      /* shape / alignment / format / null pointer */
@@ -61,8 +66,8 @@ const char* mxfp6_last_error(void);
  * (kernels/gemm/bf16fp32/256_256_64_32_with16x32.cpp:383-387) with the operand set of
  * micro_globals (:47-58) extended by the two scale tensors in the argument order of the
  * reference's scale-taking kernel (kernels/torch_scaled/scaled_matmul.cu:17-18).
- *   a   [M, 3K/4] u8 (fp6) or [M, K] u8 (fp8)   sfa [M, K/32] u8    fmt_a one of the four format codes
- *   b   [N, 3K/4] u8 (fp6) or [N, K] u8 (fp8)   sfb [N, K/32] u8    fmt_b likewise
+ *   a   [M, 3K/4] u8 (fp6), [M, K] u8 (fp8) or [M, K/2] u8 (fp4)   sfa [M, K/32] u8    fmt_a one of the five format codes
+ *   b   [N, 3K/4] u8 (fp6), [N, K] u8 (fp8) or [N, K/2] u8 (fp4)   sfb [N, K/32] u8    fmt_b likewise
  *   c   [M, N] bf16, written in place
  * Shapes that split output tiles along K use a per-device scratch buffer that the library
  * allocates on first need (cudaMalloc) and keeps; concurrent calls on different streams of one
@@ -91,7 +96,7 @@ int mxfp6_gemm_ex(const void* a, const void* sfa, const void* b, const void* sfb
 
 /*
  * The GEMM with its result handed to the next layer already quantised: instead of bf16 C the epilogue writes
- * C as an MX operand, blocks of 32 along N (the next layer's K): out [M, 3N/4] (fp6) or [M, N] (fp8) bytes and
+ * C as an MX operand, blocks of 32 along N (the next layer's K): out [M, 3N/4] (fp6), [M, N] (fp8) or [M, N/2] (fp4) bytes and
  * out_scales [M, N/32] E8M0 bytes, quantised from the fp32 accumulators with the rule of mxfp6_quantize
  * (so a 2-byte round trip of C through HBM and a quantiser launch disappear).  N % 64 == 0, out 16-byte
  * aligned, out_scales 2-byte aligned (two scale bytes are stored at a time).  (No counterpart in the reference; the nearest is the epilogue scaling of
@@ -186,16 +191,19 @@ int mxfp6_gemm_noalloc(const void* a, const void* sfa, const void* b, const void
 
 /*
  * Block quantiser: src [rows, K] (src_dtype 0 = fp32, 1 = bf16), K % 32 == 0  ->
- * packed [rows, 3K/4] (fp6) or [rows, K] (fp8) + scales [rows, K/32].  Scale exponent = floor(log2(amax)) - 2
- * (E2M3), - 4 (E3M2), - 8 (E4M3) or - 15 (E5M2); elements rounded to nearest even and saturated.  The step in front of the GEMM; the
+ * packed [rows, 3K/4] (fp6), [rows, K] (fp8) or [rows, K/2] (fp4) + scales [rows, K/32].  Scale exponent = floor(log2(amax)) - 2
+ * (E2M3, E2M1), - 4 (E3M2), - 8 (E4M3) or - 15 (E5M2); elements rounded to nearest even and saturated.  The step in front of the GEMM; the
  * reference's fp8 harness does it on the host (kernels/gemm/fp8fp32/FP8_8wave/8_wave.cu:258-268).
  */
 int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt,
                    void* packed, void* scales, void* stream);
 
-/* Inverse, to fp32 [rows, K]: decode(code) * 2^(scale-127).  Test aid. */
+/* Inverse, to fp32 [rows, K]: decode(code) * 2^(scale-127).  The _ex form also delivers bf16 (out_dtype 1; 0 = fp32), which
+ * changes no value inside bf16's normal range (the elements have at most four significant bits).  out 16-byte aligned. */
 int mxfp6_dequantize(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt,
                      void* out_f32, void* stream);
+int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt,
+                        void* out, int out_dtype, void* stream);
 
 /*
  * Synchronises the current device and reports the device-side status word of the kernels launched

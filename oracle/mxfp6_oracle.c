@@ -52,12 +52,14 @@ static inline float pow2i(int e) {
 /* ---- format parameters ---------------------------------------------------- */
 #define MXFP8_E4M3 2
 #define MXFP8_E5M2 3
+#define MXFP4_E2M1 4
 typedef struct { int bits, mbits, bias, emax; float maxv; int maxcode; } fmt_t;
 static fmt_t fmt_of(int fmt) {
     switch (fmt) {
         case MXFP6_E2M3: { fmt_t f = {6, 3, 1, 2, 7.5f, 0x1f}; return f; }
         case MXFP6_E3M2: { fmt_t f = {6, 2, 3, 4, 28.0f, 0x1f}; return f; }
         case MXFP8_E4M3: { fmt_t f = {8, 3, 7, 8, 448.0f, 0x7e}; return f; }   /* 0x7f is NaN */
+        case MXFP4_E2M1: { fmt_t f = {4, 1, 1, 2, 6.0f, 0x7}; return f; }
         default:         { fmt_t f = {8, 2, 15, 15, 57344.0f, 0x7b}; return f; } /* exponent 31 is inf/nan */
     }
 }
@@ -151,7 +153,7 @@ void mxfp6_unpack(const uint8_t* packed, int64_t n, uint8_t* codes) {
 }
 
 /* ---- block quantiser ------------------------------------------------------ */
-/* src [rows,K] fp32 row-major, K % 32 == 0 -> operand bytes (fp6: packed [rows,3K/4]; fp8: [rows,K]),
+/* src [rows,K] fp32 row-major, K % 32 == 0 -> operand bytes (fp6: packed [rows,3K/4]; fp8: [rows,K]; fp4: [rows,K/2]),
  * scales [rows,K/32] */
 void mxfp6_quantize(const float* src, int64_t rows, int64_t K, int fmt, uint8_t* packed, uint8_t* scales) {
     const int fp8 = fmt_of(fmt).bits == 8;
@@ -170,6 +172,7 @@ void mxfp6_quantize(const float* src, int64_t rows, int64_t K, int fmt, uint8_t*
             float f1 = pow2i(h), f2 = pow2i(-e - h);
             for (int i = 0; i < 32; ++i) codes[i] = mxfp6_encode_elem(x[i] * f1 * f2, fmt);
             if (fp8) memcpy(packed + r * K + kb * 32, codes, 32);
+            else if (fmt == MXFP4_E2M1) for (int i = 0; i < 16; ++i) packed[r * (K / 2) + kb * 16 + i] = (uint8_t)(codes[2 * i] | (codes[2 * i + 1] << 4));
             else mxfp6_pack(codes, 32, packed + r * (K * 3 / 4) + kb * 24);
         }
     }
@@ -179,12 +182,13 @@ void mxfp6_quantize(const float* src, int64_t rows, int64_t K, int fmt, uint8_t*
 void mxfp6_dequantize(const uint8_t* packed, const uint8_t* scales, int64_t rows, int64_t K, int fmt, float* out) {
     const int fp8 = fmt_of(fmt).bits == 8;
     float lut[256];
-    for (int c = 0; c < (fp8 ? 256 : 64); ++c) lut[c] = mxfp6_decode_elem((uint8_t)c, fmt);
+    for (int c = 0; c < (fp8 ? 256 : fmt == MXFP4_E2M1 ? 16 : 64); ++c) lut[c] = mxfp6_decode_elem((uint8_t)c, fmt);
     #pragma omp parallel for schedule(static)
     for (int64_t r = 0; r < rows; ++r) {
         uint8_t codes[32];
         for (int64_t kb = 0; kb < K / 32; ++kb) {
             if (fp8) memcpy(codes, packed + r * K + kb * 32, 32);
+            else if (fmt == MXFP4_E2M1) for (int i = 0; i < 32; ++i) codes[i] = (packed[r * (K / 2) + kb * 16 + i / 2] >> (4 * (i & 1))) & 15;
             else mxfp6_unpack(packed + r * (K * 3 / 4) + kb * 24, 32, codes);
             float s = mxfp6_e8m0_decode(scales[r * (K / 32) + kb]);
             for (int i = 0; i < 32; ++i) out[r * K + kb * 32 + i] = lut[codes[i]] * s;

@@ -27,6 +27,7 @@ E2M3 = 0
 E3M2 = 1
 E4M3 = 2   # MX-FP8, OCP e4m3 ("fn": no infinities, 0x7f/0xff are NaN), one byte per element
 E5M2 = 3   # MX-FP8, OCP e5m2 (IEEE-like: exponent 31 is inf/nan), one byte per element
+E2M1 = 4   # MX-FP4, OCP e2m1, two elements per byte, the lower one in the low nibble
 
 # bits = container width; ncodes = finite non-negative codes (they ascend with the value, so the index of a
 # magnitude in the table of finite magnitudes is its code)
@@ -35,6 +36,7 @@ _FMT = {
     E3M2: dict(bits=6, mbits=2, bias=3, emax=4, maxv=28.0, nfinite=32),
     E4M3: dict(bits=8, mbits=3, bias=7, emax=8, maxv=448.0, nfinite=127),
     E5M2: dict(bits=8, mbits=2, bias=15, emax=15, maxv=57344.0, nfinite=124),
+    E2M1: dict(bits=4, mbits=1, bias=1, emax=2, maxv=6.0, nfinite=8),
 }
 
 
@@ -44,7 +46,7 @@ def is_fp8(fmt: int) -> bool:
 
 # --------------------------------------------------------------------------- tables
 def decode_table(fmt: int) -> np.ndarray:
-    """All 64 (fp6) or 256 (fp8) code -> fp32 values; fp8 NaN/inf codes decode to nan/inf."""
+    """All 16 (fp4), 64 (fp6) or 256 (fp8) code -> fp32 values; fp8 NaN/inf codes decode to nan/inf."""
     p = _FMT[fmt]
     mb, bias, bits = p["mbits"], p["bias"], p["bits"]
     eb = bits - 1 - mb
@@ -122,6 +124,23 @@ def unpack_codes(packed: np.ndarray) -> np.ndarray:
     return out.reshape(*packed.shape[:-1], -1)
 
 
+def pack_nibbles(codes: np.ndarray) -> np.ndarray:
+    """[..., K] uint8 codes -> [..., K/2] bytes, the lower element in the low nibble."""
+    c = np.asarray(codes, dtype=np.uint8)
+    return (c[..., 0::2] | (c[..., 1::2] << 4)).astype(np.uint8)
+
+
+def unpack_nibbles(packed: np.ndarray) -> np.ndarray:
+    """[..., K/2] bytes -> [..., K] uint8 codes."""
+    p = np.asarray(packed, dtype=np.uint8)
+    return np.stack([p & 15, p >> 4], axis=-1).reshape(*p.shape[:-1], -1)
+
+
+def elements_of(nbytes: int, fmt: int) -> int:
+    """K of an operand row of nbytes bytes."""
+    return nbytes * 8 // _FMT[fmt]["bits"]
+
+
 # --------------------------------------------------------------------------- quantise / dequantise
 def quantize(x: np.ndarray, fmt: int):
     """fp32 [rows,K] -> (packed uint8 [rows,3K/4] for fp6 or [rows,K] for fp8, scales uint8 [rows,K/32])."""
@@ -134,12 +153,12 @@ def quantize(x: np.ndarray, fmt: int):
     e = sb.astype(np.int32) - 127
     v = np.ldexp(xb.astype(np.float64), -e[..., None]).astype(np.float32)  # exact power-of-two scaling
     codes = encode_elems(v, fmt).reshape(rows, K)
-    return (codes if is_fp8(fmt) else pack_codes(codes)), sb
+    return (codes if is_fp8(fmt) else pack_nibbles(codes) if fmt == E2M1 else pack_codes(codes)), sb
 
 
 def codes_of(packed: np.ndarray, fmt: int) -> np.ndarray:
     """Operand bytes -> one code per element."""
-    return np.asarray(packed, dtype=np.uint8) if is_fp8(fmt) else unpack_codes(packed)
+    return np.asarray(packed, dtype=np.uint8) if is_fp8(fmt) else unpack_nibbles(packed) if fmt == E2M1 else unpack_codes(packed)
 
 
 def dequantize(packed: np.ndarray, scales: np.ndarray, fmt: int) -> np.ndarray:
@@ -285,7 +304,7 @@ def _p(a, t):
 def c_quantize(x: np.ndarray, fmt: int):
     x = np.ascontiguousarray(x, dtype=np.float32)
     rows, K = x.shape
-    packed = np.empty((rows, K if is_fp8(fmt) else K * 3 // 4), np.uint8)
+    packed = np.empty((rows, K * _FMT[fmt]["bits"] // 8), np.uint8)
     scales = np.empty((rows, K // 32), np.uint8)
     c_oracle().mxfp6_quantize(_p(x, ctypes.c_float), rows, K, fmt, _p(packed, ctypes.c_uint8), _p(scales, ctypes.c_uint8))
     return packed, scales
@@ -294,7 +313,7 @@ def c_quantize(x: np.ndarray, fmt: int):
 def c_dequantize(packed: np.ndarray, scales: np.ndarray, fmt: int) -> np.ndarray:
     packed = np.ascontiguousarray(packed, dtype=np.uint8)
     scales = np.ascontiguousarray(scales, dtype=np.uint8)
-    rows, K = packed.shape[0], (packed.shape[1] if is_fp8(fmt) else packed.shape[1] * 4 // 3)
+    rows, K = packed.shape[0], elements_of(packed.shape[1], fmt)
     out = np.empty((rows, K), np.float32)
     c_oracle().mxfp6_dequantize(_p(packed, ctypes.c_uint8), _p(scales, ctypes.c_uint8), rows, K, fmt, _p(out, ctypes.c_float))
     return out
@@ -309,7 +328,7 @@ def c_gemm_ref(a_packed, sfa, b_packed, sfb, fmt_a=E2M3, fmt_b=None, acc_mode=0,
     sfa = np.ascontiguousarray(sfa, np.uint8)
     sfb = np.ascontiguousarray(sfb, np.uint8)
     M, N = a_packed.shape[0], b_packed.shape[0]
-    K = a_packed.shape[1] if is_fp8(fmt_a) else a_packed.shape[1] * 4 // 3
+    K = elements_of(a_packed.shape[1], fmt_a)
     cb = np.empty((M, N), np.uint16)
     cf = np.empty((M, N), np.float32)
     ad = np.empty((M, N), np.float32) if want_absdot else None
@@ -334,6 +353,9 @@ def dequantize_torch(packed, scales, fmt: int):
     if is_fp8(fmt):
         K = packed.shape[1]
         codes = packed
+    elif fmt == E2M1:
+        K = packed.shape[1] * 2
+        codes = torch.stack([packed & 15, packed >> 4], dim=-1).view(rows, K)
     else:
         K = packed.shape[1] // 3 * 4
         b = packed.view(rows, -1, 3).to(torch.int32)
