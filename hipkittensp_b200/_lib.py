@@ -21,7 +21,8 @@ OK, ERR_BAD_ARG, ERR_CUDA, ERR_DEVICE_WAIT, ERR_UNSUPPORTED = 0, 1, 2, 3, 4
 # every symbol include/mxfp6.h declares
 SYMBOLS = ("mxfp6_version", "mxfp6_last_error", "mxfp6_gemm", "mxfp6_gemm_workspace_bytes", "mxfp6_gemm_ws",
            "mxfp6_gemm_noalloc", "mxfp6_gemm_multi", "mxfp6_gemm_copy_gather", "mxfp6_copy_gather_scratch_bytes", "mxfp6_gemm_ex", "mxfp6_gemm_requant", "mxfp6_gemm_scaled",
-           "mxfp6_quantize", "mxfp6_dequantize", "mxfp6_dequantize_ex", "mxfp6_device_status", "mxfp6_debug_tma_dump", "mxfp6_debug_wait_timeout", "mxfp6_debug_option", "mxfp6_debug_plan")
+           "mxfp6_quantize", "mxfp6_dequantize", "mxfp6_dequantize_ex", "mxfp6_layer_norm", "mxfp6_layer_norm_quantize", "mxfp6_layer_norm_backward",
+           "mxfp6_layer_norm_backward_workspace_bytes", "mxfp6_device_status", "mxfp6_debug_tma_dump", "mxfp6_debug_wait_timeout", "mxfp6_debug_option", "mxfp6_debug_plan")
 
 
 class Mxfp6Error(RuntimeError):
@@ -71,6 +72,14 @@ def _load() -> ctypes.CDLL:
     lib.mxfp6_dequantize.argtypes = [vp, vp, i64, i64, ci, vp, vp]
     lib.mxfp6_dequantize_ex.restype = ci
     lib.mxfp6_dequantize_ex.argtypes = [vp, vp, i64, i64, ci, vp, ci, vp]
+    lib.mxfp6_layer_norm.restype = ci
+    lib.mxfp6_layer_norm.argtypes = [vp, ci, vp, vp, ci, vp, vp, vp, i64, i64, ctypes.c_float, vp]
+    lib.mxfp6_layer_norm_quantize.restype = ci
+    lib.mxfp6_layer_norm_quantize.argtypes = [vp, ci, vp, vp, ci, ci, vp, vp, vp, vp, i64, i64, ctypes.c_float, vp]
+    lib.mxfp6_layer_norm_backward.restype = ci
+    lib.mxfp6_layer_norm_backward.argtypes = [vp, vp, ci, vp, vp, vp, ci, vp, vp, vp, i64, i64, vp, sz, vp]
+    lib.mxfp6_layer_norm_backward_workspace_bytes.restype = sz
+    lib.mxfp6_layer_norm_backward_workspace_bytes.argtypes = [i64, i64]
     lib.mxfp6_device_status.restype = ci
     lib.mxfp6_device_status.argtypes = [ctypes.POINTER(ci)]
     lib.mxfp6_debug_wait_timeout.restype = ci

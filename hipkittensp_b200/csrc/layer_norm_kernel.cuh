@@ -1,0 +1,462 @@
+// Layer norm over the rows of a [rows, H] matrix (fp32 or bf16), its gradient, and the form that hands its result on as an MX
+// operand.  All sums and statistics are fp32.
+//
+//   forward    mean = sum(x) / H,  var = sum((x - mean)^2) / H,  rstd = 1 / sqrt(var + eps),  y = (x - mean) * rstd * w + b
+//   backward   xhat = (x - mean) * rstd,  g = dy * w,
+//              dx = (g - sum(g) / H - xhat * sum(g * xhat) / H) * rstd,   dw = sum over rows(dy * xhat),   db = sum over rows(dy)
+//
+// Both are bound by HBM: forward reads x and writes y once, backward reads x and dy and writes dx once.  A row is held in
+// registers between its passes (the variance is the sum of squared distances from the mean, not E[x^2] - mean^2, which loses
+// every digit of rows whose mean is far above their spread; the second pass also sums the distances themselves, whose mean is
+// what the first pass's rounding left out of the mean).  One warp or one CTA owns a row; CTAs are persistent.
+//
+// The parameter gradients: every CTA sums its rows in registers (each thread owns the same columns of every row) and writes one
+// partial per column; a second kernel adds the partials in a fixed order, so results do not depend on timing.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "ptx.cuh"
+#include "quant.cuh"
+
+namespace mxfp6 {
+
+struct LnParams {
+    const void* x;           // [rows, H]
+    const void* dy;          // backward: [rows, H]
+    void* y;                 // forward: result, [rows, H] in x's type; backward: dx
+    const void* w;           // [H] or null (ones)
+    const void* b;           // [H] or null (zeros)
+    int w_bf16;              // type of w and b: 0 = fp32, 1 = bf16
+    float* mean;             // [rows]; forward: may be null, like rstd
+    float* rstd;             // [rows]
+    float* part;             // backward: [grid][2][H] partial sums of dw and db, or null when they are not wanted
+    uint8_t* q_out;          // forward to an MX operand: codes [rows, H * bits / 8] ...
+    uint8_t* q_scales;       // ... and scales [rows, H / 32]
+    int q_fmt;
+    int64_t rows;
+    int H;
+    float inv_h, eps;
+};
+
+__device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
+// V consecutive elements as they lie in memory (V = 8: one 16- or 32-byte load; V = 1: any alignment).  Data of the row
+// matrices goes past L1, which keeps the weights.
+template <typename T, int V> struct Raw { uint32_t u[V == 8 ? (sizeof(T) == 4 ? 8 : 4) : 1]; };
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> ld_raw(const T* p) {
+    Raw<T, V> r;
+    if constexpr (V == 8 && sizeof(T) == 4) {
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]), "=r"(r.u[4]), "=r"(r.u[5]), "=r"(r.u[6]), "=r"(r.u[7]) : "l"(p) : "memory");
+    } else if constexpr (V == 8) {
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "l"(p) : "memory");
+    } else if constexpr (sizeof(T) == 4) {
+        r.u[0] = *reinterpret_cast<const volatile uint32_t*>(p);
+    } else {
+        r.u[0] = *reinterpret_cast<const volatile uint16_t*>(p);
+    }
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& r, float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = __uint_as_float(r.u[i]);
+    } else if constexpr (V == 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r.u[i]); v[2 * i + 1] = bf16_hi(r.u[i]); }
+    } else {
+        v[0] = bf16_lo(r.u[0]);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void st_row(T* p, const float (&v)[V]) {
+    if constexpr (V == 8 && sizeof(T) == 4) {
+        st_global_v8(p, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]),
+                     __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    } else if constexpr (V == 8) {
+        uint4 q;
+        q.x = pack_bf16x2(v[0], v[1]); q.y = pack_bf16x2(v[2], v[3]); q.z = pack_bf16x2(v[4], v[5]); q.w = pack_bf16x2(v[6], v[7]);
+        *reinterpret_cast<uint4*>(p) = q;
+    } else if constexpr (sizeof(T) == 4) {
+        *p = v[0];
+    } else {
+        *p = __float2bfloat16_rn(v[0]);
+    }
+}
+// V elements of a parameter vector (fill where there is none)
+template <int V>
+__device__ __forceinline__ void ld_param(const void* w, int is_bf16, int col, float fill, float (&v)[V]) {
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fill;
+    } else if (is_bf16) {
+        const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(w) + col;
+        if constexpr (V == 8) {
+            const uint4 q = *reinterpret_cast<const uint4*>(p);
+            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(u[i]); v[2 * i + 1] = bf16_hi(u[i]); }
+        } else {
+            v[0] = __bfloat162float(*p);
+        }
+    } else {
+        const float* p = reinterpret_cast<const float*>(w) + col;
+        if constexpr (V == 8) {
+            const float4 a = *reinterpret_cast<const float4*>(p), c = *reinterpret_cast<const float4*>(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
+        } else {
+            v[0] = *p;
+        }
+    }
+}
+
+// Sums of N values over the WARPS warps that share a row (one warp: shuffles alone).  `red` has N * WARPS floats per call of a
+// row pass; the barrier in front of the reads is the only one a pass needs because consecutive passes use different buffers.
+template <int N, int WARPS>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    if constexpr (WARPS > 1) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        if (lane == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) red[n * WARPS + warp] = v[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float s = lane < WARPS ? red[n * WARPS + lane] : 0.f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                if (o < WARPS) s += __shfl_xor_sync(0xffffffffu, s, o);
+            v[n] = WARPS < 32 ? __shfl_sync(0xffffffffu, s, 0) : s;
+        }
+    }
+}
+
+// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes and scale.
+__device__ __forceinline__ void mx_store8(const float (&v)[8], int fmt, uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
+    float amax = fmaxf(amax3(v[0], v[1], v[2]), fmaxf(amax3(v[3], v[4], v[5]), fmaxf(fabsf(v[6]), fabsf(v[7]))));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int sb = quant_scale_byte(amax, fmt);
+    const float f = quant_inv_scale(sb);
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = v[i] * f;
+    const int j = (col >> 3) & 3;                   // place of these eight in their block
+    if (fmt == kE2M1) {
+        const uint32_t w = cvt_oct_e2m1(s);
+        if (live) *reinterpret_cast<uint32_t*>(codes_row + col / 2) = w;
+    } else if (fmt_fp8(fmt)) {
+        const uint32_t w0 = cvt_quad_rt(s[0], s[1], s[2], s[3], fmt), w1 = cvt_quad_rt(s[4], s[5], s[6], s[7], fmt);
+        if (live) *reinterpret_cast<uint2*>(codes_row + col) = make_uint2(w0, w1);
+    } else {
+        // 48 bits a lane: four lanes hold 24 bytes, which three of them write
+        const uint64_t w = (uint64_t)cvt_quad_rt(s[0], s[1], s[2], s[3], fmt) | ((uint64_t)cvt_quad_rt(s[4], s[5], s[6], s[7], fmt) << 24);
+        const uint64_t nx = (uint64_t)__shfl_down_sync(0xffffffffu, (unsigned long long)w, 1);
+        if (live && j < 3) *reinterpret_cast<uint64_t*>(codes_row + (col / 32) * 24 + 8 * j) = (w >> (16 * j)) | (nx << (48 - 16 * j));
+    }
+    if (live && j == 0) scales_row[col / 32] = (uint8_t)sb;
+}
+
+// ---------------------------------------------------------------------------------- forward
+// WARPS warps own a row, V * C elements per thread.  WARPS = 1: eight warps per CTA with a row each.  MX: the result leaves as codes and scales.
+template <typename T, int V, int C, int WARPS, bool MX>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+layer_norm_kernel(const LnParams P) {
+    constexpr int TPR = 32 * WARPS;
+    constexpr int ROWS = WARPS == 1 ? 8 : 1;                    // rows a CTA works on at a time
+    __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
+    const T* x = reinterpret_cast<const T*>(P.x);
+    Raw<T, V> cur[C];
+    auto load = [&](int64_t r, Raw<T, V> (&dst)[C]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (tid + c * TPR) * V;
+            dst[c] = Raw<T, V>{};
+            if (r < P.rows && col < P.H) dst[c] = ld_raw<T, V>(x + r * P.H + col);
+        }
+    };
+    load(row, cur);
+    for (int par = 0; row < P.rows; row += step, par ^= 1) {
+        // the next row is on its way while this one is worked on
+        Raw<T, V> nxt[C];
+        load(row + step, nxt);
+        float v[C][V];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            unpack<T, V>(cur[c], v[c]);                          // columns past H hold zeros
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] += v[c][i];
+        }
+        row_sum<1, WARPS>(s, red[par]);
+        const float mean0 = s[0] * P.inv_h;
+        float q[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if ((tid + c * TPR) * V < P.H) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) { v[c][i] -= mean0; q[0] = fmaf(v[c][i], v[c][i], q[0]); q[1] += v[c][i]; }
+            }
+        }
+        row_sum<2, WARPS>(q, red2[par]);
+        const float corr = q[1] * P.inv_h, mean = mean0 + corr;
+        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
+        if (tid == 0 && P.mean) P.mean[row] = mean;
+        if (tid == 0 && P.rstd) P.rstd[row] = rstd;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (tid + c * TPR) * V;
+            const bool live = col < P.H;
+            float w[V], b[V], o[V];
+            if (live) { ld_param<V>(P.w, P.w_bf16, col, 1.f, w); ld_param<V>(P.b, P.w_bf16, col, 0.f, b); }
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = live ? fmaf((v[c][i] - corr) * rstd, w[i], b[i]) : 0.f;
+            if constexpr (MX) {
+                mx_store8(o, P.q_fmt, P.q_out + row * (P.H / 32) * fmt_block_bytes(P.q_fmt), P.q_scales + row * (P.H / 32), col, live);
+            } else if (live) {
+                st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) cur[c] = nxt[c];
+    }
+}
+
+// Rows longer than the registers of a CTA hold: a CTA of 1024 threads passes over its row three times (the second and third
+// pass find it in L2).
+template <typename T, int V, bool MX>
+__global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P) {
+    __shared__ float red[32], red2[64];
+    pdl_launch_dependents();
+    pdl_wait();
+    const T* x = reinterpret_cast<const T*>(P.x);
+    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        const T* xr = x + row * P.H;
+        float s[1] = {0.f};
+        for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
+            float v[V];
+            unpack<T, V>(ld_raw<T, V>(xr + col), v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[0] += v[i];
+        }
+        row_sum<1, 32>(s, red);
+        const float mean0 = s[0] * P.inv_h;
+        float q[2] = {0.f, 0.f};
+        for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
+            float v[V];
+            unpack<T, V>(ld_raw<T, V>(xr + col), v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const float d = v[i] - mean0; q[0] = fmaf(d, d, q[0]); q[1] += d; }
+        }
+        row_sum<2, 32>(q, red2);
+        const float corr = q[1] * P.inv_h, mean = mean0 + corr;
+        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
+        if (threadIdx.x == 0 && P.mean) P.mean[row] = mean;
+        if (threadIdx.x == 0 && P.rstd) P.rstd[row] = rstd;
+        // every thread makes the same number of rounds: the lanes of a block exchange their largest magnitudes
+        for (int c0 = 0; c0 < P.H; c0 += 1024 * V) {
+            const int col = c0 + threadIdx.x * V;
+            const bool live = col < P.H;
+            float v[V], w[V], b[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = 0.f;
+            if (live) {
+                unpack<T, V>(ld_raw<T, V>(xr + col), v);
+                ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
+                ld_param<V>(P.b, P.w_bf16, col, 0.f, b);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = fmaf((v[i] - mean0 - corr) * rstd, w[i], b[i]);
+            }
+            if constexpr (MX) {
+                mx_store8(v, P.q_fmt, P.q_out + row * (P.H / 32) * fmt_block_bytes(P.q_fmt), P.q_scales + row * (P.H / 32), col, live);
+            } else if (live) {
+                st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, v);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------- backward
+template <typename T, int V, int C, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+layer_norm_backward_kernel(const LnParams P) {
+    constexpr int TPR = 32 * WARPS;
+    constexpr int ROWS = WARPS == 1 ? 8 : 1;
+    __shared__ float red[2][2 * WARPS];
+    __shared__ float fold[WARPS == 1 ? 8 * 32 * V * C : 1];     // one warp per row: the warps' column sums meet here
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const T* dy = reinterpret_cast<const T*>(P.dy);
+    float dw[C][V], db[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.f;
+    int par = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0); row < P.rows; row += step, par ^= 1) {
+        const float mean = P.mean[row], rstd = P.rstd[row];
+        float xh[C][V], g[C][V];
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (tid + c * TPR) * V;
+            if (col < P.H) {
+                float w[V];
+                unpack<T, V>(ld_raw<T, V>(x + row * P.H + col), xh[c]);
+                unpack<T, V>(ld_raw<T, V>(dy + row * P.H + col), g[c]);
+                ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    xh[c][i] = (xh[c][i] - mean) * rstd;
+                    dw[c][i] = fmaf(g[c][i], xh[c][i], dw[c][i]);
+                    db[c][i] += g[c][i];
+                    g[c][i] *= w[i];
+                    s[0] += g[c][i];
+                    s[1] = fmaf(g[c][i], xh[c][i], s[1]);
+                }
+            }
+        }
+        row_sum<2, WARPS>(s, red[par]);
+        const float m1 = s[0] * P.inv_h, m2 = s[1] * P.inv_h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (tid + c * TPR) * V;
+            if (col < P.H) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[c][i] = (g[c][i] - fmaf(xh[c][i], m2, m1)) * rstd;
+                st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, g[c]);
+            }
+        }
+    }
+    if (!P.part) return;
+    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if constexpr (WARPS == 1) {
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) fold[(threadIdx.x >> 5) * (32 * V * C) + (tid + c * 32) * V + i] = k ? db[c][i] : dw[c][i];
+            __syncthreads();
+            for (int col = threadIdx.x; col < P.H; col += 256) {
+                float a = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) a += fold[r * (32 * V * C) + col];
+                out[(int64_t)k * P.H + col] = a;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int col = (tid + c * TPR) * V;
+                if (col < P.H)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) out[(int64_t)k * P.H + col + i] = k ? db[c][i] : dw[c][i];
+            }
+        }
+    }
+}
+
+// Rows longer than a CTA's registers hold: dx with a second pass over the row, and the parameter gradients by a kernel whose
+// threads own a column each and walk down a share of the rows.
+template <typename T, int V>
+__global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const LnParams P) {
+    __shared__ float red[2][64];
+    pdl_launch_dependents();
+    pdl_wait();
+    int par = 0;
+    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x, par ^= 1) {
+        const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
+        const T* dy = reinterpret_cast<const T*>(P.dy) + row * P.H;
+        const float mean = P.mean[row], rstd = P.rstd[row];
+        float s[2] = {0.f, 0.f};
+        for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
+            float v[V], g[V], w[V];
+            unpack<T, V>(ld_raw<T, V>(x + col), v);
+            unpack<T, V>(ld_raw<T, V>(dy + col), g);
+            ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) { const float gw = g[i] * w[i]; s[0] += gw; s[1] = fmaf(gw, (v[i] - mean) * rstd, s[1]); }
+        }
+        row_sum<2, 32>(s, red[par]);
+        const float m1 = s[0] * P.inv_h, m2 = s[1] * P.inv_h;
+        for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
+            float v[V], g[V], w[V];
+            unpack<T, V>(ld_raw<T, V>(x + col), v);
+            unpack<T, V>(ld_raw<T, V>(dy + col), g);
+            ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) g[i] = (g[i] * w[i] - fmaf((v[i] - mean) * rstd, m2, m1)) * rstd;
+            st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, g);
+        }
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) layer_norm_columns_kernel(const LnParams P) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= P.H) return;
+    const int64_t per = (P.rows + gridDim.y - 1) / gridDim.y;
+    const int64_t r0 = blockIdx.y * per, r1 = r0 + per < P.rows ? r0 + per : P.rows;
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const T* dy = reinterpret_cast<const T*>(P.dy);
+    float dw = 0.f, db = 0.f;
+#pragma unroll 4
+    for (int64_t r = r0; r < r1; ++r) {
+        float v[1], g[1];
+        unpack<T, 1>(ld_raw<T, 1>(x + r * P.H + col), v);
+        unpack<T, 1>(ld_raw<T, 1>(dy + r * P.H + col), g);
+        dw = fmaf(g[0], (v[0] - P.mean[r]) * P.rstd[r], dw);
+        db += g[0];
+    }
+    float* out = P.part + (int64_t)blockIdx.y * 2 * P.H;
+    out[col] = dw;
+    out[P.H + col] = db;
+}
+
+// [parts][2][H] partial sums -> dw [H], db [H] (either may be null): 32 columns per CTA, 32 threads per column, each adding
+// every 32nd partial; the 32 sums meet in shared memory in a fixed order.
+__global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* part, int parts, int H, float* dw, float* db) {
+    __shared__ float s[32][33];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t two_h = 2 * (int64_t)H;
+    const int64_t col = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int lane = threadIdx.x >> 5;
+    float a = 0.f;
+    if (col < two_h) {
+#pragma unroll 8
+        for (int p = lane; p < parts; p += 32) a += __ldcg(part + p * two_h + col);
+    }
+    s[lane][threadIdx.x & 31] = a;
+    __syncthreads();
+    // warp `lane` sums the 32 shares of column `lane`
+    float t = s[threadIdx.x & 31][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    if ((threadIdx.x & 31) == 0 && c < two_h) {
+        if (c < H) { if (dw) dw[c] = t; }
+        else if (db) db[c - H] = t;
+    }
+}
+
+}  // namespace mxfp6

@@ -121,6 +121,7 @@ struct DeviceState {
     size_t ws_bytes = 0;
     std::vector<std::pair<void*, size_t>> ws_all;   // every buffer ever handed out: none is freed, launches and graphs may hold them
     std::map<const void*, bool> smem_attr_set;
+    std::map<const void*, int> ctas_per_sm;
 };
 static std::mutex g_mu;
 static DeviceState g_dev[64];
@@ -269,6 +270,16 @@ static int fmt_map_kind(int f) { return fmt_is_fp8(f) ? 3 : f == MXFP4_E2M1 ? 8 
 static int fmt_out_map_kind(int f) { return fmt_is_fp8(f) ? 7 : f == MXFP4_E2M1 ? 9 : 6; }   // tensor map of a re-quantised result
 static uint32_t fmt_mma_code(int f) {      // operand format field of kind::mxf8f6f4
     return f == MXFP6_E2M3 ? kFmtE2M3 : f == MXFP6_E3M2 ? kFmtE3M2 : f == MXFP8_E4M3 ? kFmtE4M3 : f == MXFP8_E5M2 ? kFmtE5M2 : kFmtE2M1;
+}
+
+// CTAs of a kernel (no dynamic shared memory) that one SM holds, asked once per device
+static int resident_ctas(DeviceState& d, const void* kern, int threads, int* out) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    int& n = d.ctas_per_sm[kern];
+    if (n == 0) CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0));
+    if (n < 1) return fail(MXFP6_ERR_CUDA, "a kernel of %d threads does not fit an SM", threads);
+    *out = n;
+    return MXFP6_OK;
 }
 
 // ---------------------------------------------------------------------------------- GEMM dispatch
@@ -843,6 +854,8 @@ __global__ void wait_probe_kernel(GemmParams P) {
 
 }  // namespace mxfp6
 
+#include "layer_norm_api.cuh"
+
 // ====================================================================================== C ABI
 using namespace mxfp6;
 
@@ -1195,6 +1208,31 @@ extern "C" int mxfp6_dequantize_ex(const void* packed, const void* scales, int64
 
 extern "C" int mxfp6_dequantize(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out_f32, void* stream) {
     return mxfp6_dequantize_ex(packed, scales, rows, K, fmt, out_f32, 0, stream);
+}
+
+extern "C" int mxfp6_layer_norm(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, void* y,
+                                float* mean, float* rstd, int64_t rows, int64_t H, float eps, void* stream) {
+    return ln_forward("layer_norm", x, x_dtype, weight, bias, w_dtype, y, -1, nullptr, nullptr, mean, rstd, rows, H, eps, stream);
+}
+
+extern "C" int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, int fmt,
+                                         void* packed, void* scales, float* mean, float* rstd, int64_t rows, int64_t H, float eps,
+                                         void* stream) {
+    if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "layer_norm_quantize: bad format %d", fmt);
+    return ln_forward("layer_norm_quantize", x, x_dtype, weight, bias, w_dtype, nullptr, fmt, packed, scales, mean, rstd, rows, H, eps, stream);
+}
+
+extern "C" size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H) {
+    if (rows <= 0 || H < 1 || rows > 0x7fffffffLL || H > 0x3fffffffLL) return 0;
+    DeviceState* d = nullptr;
+    if (get_device_state(&d)) return 0;
+    return (size_t)ln_backward_parts(rows, H, d->sm_count) * 2 * (size_t)H * 4;
+}
+
+extern "C" int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,
+                                         const void* weight, int w_dtype, void* dx, float* dweight, float* dbias, int64_t rows,
+                                         int64_t H, void* workspace, size_t workspace_bytes, void* stream) {
+    return ln_backward(dy, x, x_dtype, mean, rstd, weight, w_dtype, dx, dweight, dbias, rows, H, workspace, workspace_bytes, stream);
 }
 
 extern "C" int mxfp6_device_status(int* status_out) {

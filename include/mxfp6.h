@@ -206,6 +206,40 @@ int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, in
                         void* out, int out_dtype, void* stream);
 
 /*
+ * Layer norm over the rows of x [rows, H] (x_dtype 0 = fp32, 1 = bf16), the step in front of a projection:
+ *     mean = sum(x) / H,  rstd = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) * rstd * weight + bias
+ * with all arithmetic in fp32 and one rounding of y to x's type.  weight and bias are [H] vectors of w_dtype (0 = fp32,
+ * 1 = bf16); either may be NULL (ones / zeros).  mean and rstd are fp32 [rows], kept for the backward pass; either may be
+ * NULL.  y may be x itself.  Any H >= 1 and any pointers aligned to their type; 16-byte (bf16) or 32-byte (fp32) aligned rows
+ * take the vector path.
+ *
+ * The _quantize form delivers y as an MX operand instead (blocks of 32 along H: the K of the product that follows), rounded
+ * once from fp32 with the rule of mxfp6_quantize: packed [rows, H/2 | 3H/4 | H] codes and scales [rows, H/32].  H % 32 == 0;
+ * x aligned as for the vector path, weight, bias and packed to 16 bytes.
+ * (Stands next to the reference's fused norm, kernels/layernorm/kernel.cpp, which has neither statistics nor a gradient.)
+ */
+int mxfp6_layer_norm(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, void* y,
+                     float* mean, float* rstd, int64_t rows, int64_t H, float eps, void* stream);
+int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, int fmt,
+                              void* packed, void* scales, float* mean, float* rstd, int64_t rows, int64_t H, float eps,
+                              void* stream);
+
+/*
+ * Gradient of the layer norm.  dy and dx are [rows, H] of x's type, mean and rstd what the forward pass gave.  With
+ * xhat = (x - mean) * rstd and g = dy * weight:
+ *     dx = (g - sum(g) / H - xhat * sum(g * xhat) / H) * rstd
+ *     dweight = sum over rows(dy * xhat),  dbias = sum over rows(dy)       (fp32 [H] each; either may be NULL)
+ * The sums over the rows go through per-CTA partials in `workspace` (at least the given number of bytes, 16-byte aligned, owned
+ * by this call until the stream has passed it; any contents; not needed when dweight and dbias are both NULL) and are added
+ * in a fixed order: equal calls on a device give equal bits.  Two calls that may overlap need a workspace each.
+ * rows = 0 gives zero parameter gradients.  (No counterpart in the reference.)
+ */
+size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H);
+int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,
+                              const void* weight, int w_dtype, void* dx, float* dweight, float* dbias, int64_t rows, int64_t H,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Synchronises the current device and reports the device-side status word of the kernels launched
  * so far (0 = ok; otherwise low byte = role whose wait ran out, upper bits = CTA index), then clears
  * it.  Returns MXFP6_ERR_DEVICE_WAIT if it was non-zero.  The reference ignores launch status
