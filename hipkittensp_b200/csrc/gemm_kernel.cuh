@@ -11,7 +11,7 @@
 //   warp 0   TMA producer: packed 6-bit operand tiles (tensor-map type 16U6_ALIGN16B, 128-byte swizzle)
 //            and raw E8M0 scale slabs into shared-memory rings
 //   warp 1   MMA issuer: copies the scale atoms into TMEM (tcgen05.cp) and issues
-//            tcgen05.mma.kind::mxf8f6f4.block_scale, accumulating in TMEM
+//            tcgen05.mma.kind::mxf8f6f4.block_scale (or kind::mxf4 when both operands are E2M1), accumulating in TMEM
 //   warps 2-3 scale re-tilers: row-major [rows, K/32] scale bytes -> the 32x16-byte atoms the MMA wants,
 //            one group of 4 K-blocks at a time, the two warps alternating
 //   warps 4-7 epilogue: TMEM -> registers -> bf16 -> global (or fp32 partials for split tiles)
@@ -34,7 +34,8 @@ enum : int {
 
 struct GemmParams {
     int p_rows, q_rows;        // valid rows of P and Q
-    int kblocks;               // K / 128
+    int kblocks;               // K-blocks (128 bytes of a row in shared memory): K / 128, or K / 256 rounded up on the 4-bit path
+    int sf_words;              // K / 128: 4-byte words of a scale row, one per 128 elements
     int tiles_p, tiles_q;      // ceil(p_rows/p_tile_rows), ceil(q_rows/q_tile_rows)
     int p_tile_rows;           // rows of P one tile covers (<= 128; 128 unless the rows of a streamed operand are dealt evenly to the CTAs)
     int q_tile_rows;           // rows of Q one tile covers (<= BN)
@@ -45,7 +46,7 @@ struct GemmParams {
     int stage_stride;          // bytes from one stage to the next (a multiple of 1024)
     int q_off;                 // offset of the Q box inside a stage (rows of P rounded up to 8, times 128)
     int load_batch;            // K-blocks the producer requests back to back
-    int k_rot;                 // whole tiles start their K loop at a tile-dependent K-block and wrap around (kblocks % 4 == 0)
+    int k_rot;                 // whole tiles start their K loop at a tile-dependent K-block and wrap around (only with whole scale groups)
     int ldc;                   // row stride of C in elements (= N)
     int c_rows, c_cols;        // M, N
     uint32_t idesc;            // instruction descriptor without scale ids
@@ -152,14 +153,18 @@ __device__ __forceinline__ void affine_chunk(const GemmParams& P, uint32_t (&v)[
 // unswapped tiles at N = 28672, K = 8192.)
 // (A third-size build, leaving room on every SM for a CTA of the next kernel of the stream, was measured and dropped:
 // its shorter ring cost 8 % at M = 16, N = 28672, more than the overlap of consecutive kernels gave back.)
-template <int BN_, bool SWAP_, bool STREAMK_, int CTAS_ = 1>
+// F4 = true: both operands E2M1 on kind::mxf4.  A K-block is 128 bytes of a row in shared memory in every form; here that is 256
+// elements instead of 128, so a scale slab (16 bytes of a row = 512 elements = 4 atoms) covers two K-blocks instead of four.
+template <int BN_, bool SWAP_, bool STREAMK_, int CTAS_ = 1, bool F4_ = false>
 struct GemmCfg {
+    static constexpr bool F4 = F4_;
+    static constexpr int KPG = F4_ ? 2 : 4;              // K-blocks per scale group
     static constexpr int BN = BN_;
     static constexpr bool SWAP = SWAP_;
     static constexpr bool STREAMK = STREAMK_;
     static constexpr int CTAS = CTAS_;
     static constexpr int BM = 128;
-    static constexpr int BK = 128;                       // elements of K per pipeline stage (= bytes in smem)
+    static constexpr int BK = 128;                       // x extent of a pipeline stage in the operands' tensor maps (= bytes in smem)
     static constexpr int P_BYTES = BM * BK;
     static constexpr int Q_BYTES = BN * BK;
     static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES;
@@ -176,8 +181,8 @@ struct GemmCfg {
     static constexpr int RAW_SLOTS = (BN >= 256 || CTAS_ == 2) ? 2 : 4;  // each raw slab covers 4 K-blocks (16 scale bytes per row)
     static constexpr int RAW_Q_ROWS = BN < 32 ? 32 : BN;
     static constexpr int RAW_BYTES = (BM + RAW_Q_ROWS) * 16;
-    static constexpr int ATOM_BYTES = 512 * (1 + QATOMS);  // scale atoms of one K-block: P atom + Q atoms
-    static constexpr int GROUP_BYTES = 4 * ATOM_BYTES;     // a group = the 4 K-blocks one raw slab covers
+    static constexpr int ATOM_BYTES = 512 * (1 + QATOMS);  // scale atoms of 128 elements: P atom + Q atoms
+    static constexpr int GROUP_BYTES = 4 * ATOM_BYTES;     // a group = the KPG K-blocks one raw slab covers
     static constexpr int ATOM_GROUPS = (BN >= 256 || CTAS_ == 2) ? 3 : 4;
     static constexpr bool OVERLAP = BN == 256;           // two 256-column accumulators share 32 columns
     static constexpr int ACC_COL1 = OVERLAP ? 224 : BN;
@@ -265,7 +270,7 @@ struct SegIter {
         } else {
             if (tile >= num_tiles) return false;
             s.tile = tile; s.k0 = 0; s.k1 = P.kblocks; s.nseg = 1; s.segidx = 0;
-            s.kofs = P.k_rot ? (int)(((long long)tile * P.kblocks) / num_tiles) & ~3 : 0;
+            s.kofs = P.k_rot ? (int)(((long long)tile * P.kblocks) / num_tiles) & ~(Cfg::KPG - 1) : 0;
             coords(tile, s.p0, s.q0);
             tile += gridDim.x;
             return true;
@@ -411,12 +416,12 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
             else tma_load_2d_hint(stage_dst + q_off, &tm_q, bar, kblk * Cfg::BK, s.q0, pol_q);
         };
         auto slab_weights = [&](uint32_t slab_dst, uint32_t bar, int kblk, const Segment& s) {
-            if (WQ) tma_load_2d_hint(slab_dst + Cfg::BM * 16, &tm_sfq, bar, (kblk >> 2) * 16, s.q0, pol_q);
-            else tma_load_2d_hint(slab_dst, &tm_sfp, bar, (kblk >> 2) * 16, s.p0, pol_p);
+            if (WQ) tma_load_2d_hint(slab_dst + Cfg::BM * 16, &tm_sfq, bar, kblk / Cfg::KPG * 16, s.q0, pol_q);
+            else tma_load_2d_hint(slab_dst, &tm_sfp, bar, kblk / Cfg::KPG * 16, s.p0, pol_p);
         };
         auto slab_other = [&](uint32_t slab_dst, uint32_t bar, int kblk, const Segment& s) {
-            if (WQ) tma_load_2d_hint(slab_dst, &tm_sfp, bar, (kblk >> 2) * 16, s.p0, pol_p);
-            else tma_load_2d_hint(slab_dst + Cfg::BM * 16, &tm_sfq, bar, (kblk >> 2) * 16, s.q0, pol_q);
+            if (WQ) tma_load_2d_hint(slab_dst, &tm_sfp, bar, kblk / Cfg::KPG * 16, s.p0, pol_p);
+            else tma_load_2d_hint(slab_dst + Cfg::BM * 16, &tm_sfq, bar, kblk / Cfg::KPG * 16, s.q0, pol_q);
         };
         if (early) {
             SegIter<Cfg> it2(P);
@@ -434,7 +439,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                         }
                         continue;
                     }
-                    if (P.sf_tma && (k == s2.k0 || (k & 3) == 0)) {
+                    if (P.sf_tma && (k == s2.k0 || k % Cfg::KPG == 0)) {
                         if (slabs && pre_raw < (uint32_t)Cfg::RAW_SLOTS) {
                             if (elect_one_sync()) {
                                 mbar_arrive_expect_tx(bar_raw_full(pre_raw), (uint32_t)P.raw_tx_bytes);
@@ -467,9 +472,9 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                 for (int k = s2.k0; k < s2.k1 && n_pre < want; ++k, ++n_pre) {
                     if (elect_one_sync()) {
                         // (the scale slab of the group first: the first MMA waits for the re-tiled scales as well)
-                        if (P.sf_tma && (k == s2.k0 || (k & 3) == 0)) {
-                            if (WQ) tma_prefetch_l2_2d(&tm_sfq, (k_at(P, s2, k) >> 2) * 16, s2.q0);
-                            else tma_prefetch_l2_2d(&tm_sfp, (k_at(P, s2, k) >> 2) * 16, s2.p0);
+                        if (P.sf_tma && (k == s2.k0 || k % Cfg::KPG == 0)) {
+                            if (WQ) tma_prefetch_l2_2d(&tm_sfq, k_at(P, s2, k) / Cfg::KPG * 16, s2.q0);
+                            else tma_prefetch_l2_2d(&tm_sfp, k_at(P, s2, k) / Cfg::KPG * 16, s2.p0);
                         }
                         if (WQ) tma_prefetch_l2_2d(&tm_q, k_at(P, s2, k) * Cfg::BK, s2.q0);
                         else tma_prefetch_l2_2d(&tm_p, k_at(P, s2, k) * Cfg::BK, s2.p0);
@@ -486,7 +491,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                 const int nb = min(load_batch, sg.k1 - kb);
                 for (int j = 0; j < nb && ok; ++j) {
                     const int k = kb + j;
-                    if (P.sf_tma && (k == sg.k0 || (k & 3) == 0)) {
+                    if (P.sf_tma && (k == sg.k0 || k % Cfg::KPG == 0)) {
                         const int r = n_raw % Cfg::RAW_SLOTS;
                         const uint32_t ph = (n_raw / Cfg::RAW_SLOTS) & 1;
                         ok = wait_bar_warp(bar_raw_empty(r), ph ^ 1, abort_flag, P, kStatusTimeoutProducer);
@@ -548,28 +553,43 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
             for (int kb = sg.k0; kb < sg.k1; ++kb) {
                 const int s = (int)st_idx;
                 const int g = n_grp % Cfg::ATOM_GROUPS;
-                // the scale atoms arrive per group of 4 K-blocks (one raw slab)
-                if (kb == sg.k0 || (kb & 3) == 0)
+                // the scale atoms arrive per group of KPG K-blocks (one raw slab)
+                if (kb == sg.k0 || kb % Cfg::KPG == 0)
                     ok = wait_bar_warp(bar_atom_full(g), (n_grp / Cfg::ATOM_GROUPS) & 1, abort_flag, P, kStatusTimeoutMma);
                 ok = ok && wait_bar_warp(bar_full(s), st_phase, abort_flag, P, kStatusTimeoutMma);
                 if (!ok) break;
-                const bool group_done = (kb & 3) == 3 || kb == sg.k1 - 1;
+                const bool group_done = kb % Cfg::KPG == Cfg::KPG - 1 || kb == sg.k1 - 1;
                 if (elect_one_sync()) {
-                    const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
-                    const uint32_t sfb = sfa + 4;
-                    const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
-                    {
-                    tc_cp_32x128b_warpx4(sfa, smem_desc_sf(atom));
-#pragma unroll
-                    for (int q = 0; q < Cfg::QATOMS; ++q) tc_cp_32x128b_warpx4(sfb + 4 * q, smem_desc_sf(atom + 512 * (1 + q)));
-                    }
                     const uint32_t sp = stage_base + s * stage_stride;
                     const uint64_t adesc = smem_desc_sw128(sp);
                     const uint64_t bdesc = smem_desc_sw128(sp + q_off);
+                    if constexpr (Cfg::F4) {
+                        // 256 elements: two atoms, each serving two K = 64 instructions (scale bytes 0-1 and 2-3 of its words)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t sfa = tmem_base + Cfg::SF_COL + h * 16;
+                            const uint32_t sfb = sfa + 4;
+                            const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + ((kb & 1) * 2 + h) * Cfg::ATOM_BYTES;
+                            tc_cp_32x128b_warpx4(sfa, smem_desc_sf(atom));
+#pragma unroll
+                            for (int q = 0; q < Cfg::QATOMS; ++q) tc_cp_32x128b_warpx4(sfb + 4 * q, smem_desc_sf(atom + 512 * (1 + q)));
+#pragma unroll
+                            for (uint32_t k = 2 * h; k < 2 * h + 2; ++k)
+                                mma_mxf4(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(P.idesc, 2 * (k & 1)), sfa | ((2 * (k & 1)) << 30),
+                                         sfb | ((2 * (k & 1)) << 30), (kb > sg.k0 || k > 0) ? 1u : 0u);
+                        }
+                    } else {
+                    const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
+                    const uint32_t sfb = sfa + 4;
+                    const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
+                    tc_cp_32x128b_warpx4(sfa, smem_desc_sf(atom));
+#pragma unroll
+                    for (int q = 0; q < Cfg::QATOMS; ++q) tc_cp_32x128b_warpx4(sfb + 4 * q, smem_desc_sf(atom + 512 * (1 + q)));
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k) {
                         mma_mxf8f6f4(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(P.idesc, k),
                                      sfa | (k << 30), sfb | (k << 30), (kb > sg.k0 || k > 0) ? 1u : 0u);
+                    }
                     }
                     tc_commit(bar_empty(s));
                     if (group_done) tc_commit(bar_atom_empty(g));
@@ -586,7 +606,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
         }
     }
     // =========================================================== warps 2-3: scale re-tilers
-    // Each group of 4 K-blocks (one raw slab of 16 scale bytes per row) is handled by one of the two warps,
+    // Each group of KPG K-blocks (one raw slab of 16 scale bytes per row) is handled by one of the two warps,
     // alternately: raw words -> registers -> the 4 x (1+QATOMS) atoms of the group -> one proxy fence ->
     // one arrival.
     else if (warp == 2 || warp == 3) {
@@ -597,9 +617,9 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
         constexpr int QG = (BN + 31) / 32;        // 32-row groups on the Q side
         while (ok && it.next(sg)) {
             for (int kb = sg.k0; kb < sg.k1 && ok;) {
-                const int kb_next = min(sg.k1, (kb | 3) + 1);
+                const int kb_next = min(sg.k1, (kb | (Cfg::KPG - 1)) + 1);
                 if ((int)(n_grp & 1) == warp - 2) {
-                    uint32_t rp[4][4];                  // [32-row group][K-block of the slab]
+                    uint32_t rp[4][4];                  // [32-row group][128 elements of the slab]
                     uint32_t rq[Cfg::QATOMS * 4][4];
                     if (P.sf_tma) {
                         const int r = n_grp % Cfg::RAW_SLOTS;
@@ -626,7 +646,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                         // global memory directly.  Four adjacent lanes read the four words of one row (16 contiguous
                         // bytes), so an instruction touches 8 rows, not 32; each word goes straight to its place in the
                         // atom of its K-block: row (r % 32), 4-byte column (r / 32).
-                        const int kb4 = k_at(P, sg, kb & ~3);
+                        const int kb4 = k_at(P, sg, kb & ~(Cfg::KPG - 1)) / Cfg::KPG * 4;      // first of the group's four scale words
                         const int w = lane & 3;
                         constexpr int NI = 16 + 4 * QG;             // 8 rows per step: 128 rows of P, then the 32-row groups of Q
                         uint32_t v[NI];
@@ -635,7 +655,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                             const int ridx = 8 * i + (lane >> 2);
                             const bool is_p = i < 16;
                             const int row = is_p ? sg.p0 + ridx : sg.q0 + ridx - 128;
-                            const bool live = row < (is_p ? P.p_rows : P.q_rows) && kb4 + w < P.kblocks;
+                            const bool live = row < (is_p ? P.p_rows : P.q_rows) && kb4 + w < P.sf_words;
                             v[i] = live ? __ldg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + (kb4 + w) * 4)) : 0u;
                         }
                         const int g = n_grp % Cfg::ATOM_GROUPS;

@@ -116,12 +116,15 @@ __device__ __forceinline__ bool pair_unit(const GemmParams& P, int it, int clust
     return true;
 }
 
+// F4: both operands E2M1 on kind::mxf4 (a K-block of 128 bytes is 256 elements, a scale slab covers two K-blocks instead of four)
+template <bool F4>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::THREADS, 1)
 mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_q_tail,
                        const __grid_constant__ CUtensorMap tm_sfp, const __grid_constant__ CUtensorMap tm_sfq,
                        const __grid_constant__ CMaps cmaps, const GemmParams P) {
     using Cfg = PairCfg;
+    constexpr int KPG = F4 ? 2 : 4;      // K-blocks per scale group
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -205,15 +208,15 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
             const CUtensorMap* tq = whole ? &tm_q : &tm_q_tail;
             const uint32_t tx = whole ? (uint32_t)P.stage_tx_bytes : (uint32_t)P.stage_tx_bytes_tail;
             for (int kb = 0; kb < P.kblocks && ok; ++kb) {
-                if (P.sf_tma && (kb & 3) == 0) {
+                if (P.sf_tma && kb % KPG == 0) {
                     const int r = n_raw % Cfg::RAW_SLOTS;
                     ok = wait_bar_warp(bar_raw_empty(r), ((n_raw / Cfg::RAW_SLOTS) & 1) ^ 1, abort_flag, P, kStatusTimeoutProducer);
                     if (!ok) break;
                     if (elect_one_sync()) {
                         const uint32_t dst = raw_base + r * Cfg::RAW_BYTES;
                         mbar_arrive_expect_tx(bar_raw_full(r), Cfg::RAW_BYTES);
-                        tma_load_2d(dst, &tm_sfp, bar_raw_full(r), (kb >> 2) * 16, my_p);
-                        tma_load_2d(dst + Cfg::BM * 16, &tm_sfq, bar_raw_full(r), (kb >> 2) * 16, q0);
+                        tma_load_2d(dst, &tm_sfp, bar_raw_full(r), kb / KPG * 16, my_p);
+                        tma_load_2d(dst + Cfg::BM * 16, &tm_sfq, bar_raw_full(r), kb / KPG * 16, q0);
                     }
                     ++n_raw;
                 }
@@ -253,27 +256,42 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                 for (int kb = 0; kb < P.kblocks; ++kb) {
                     const int s = n_kb % Cfg::STAGES;
                     const int g = n_grp % Cfg::ATOM_GROUPS;
-                    if ((kb & 3) == 0)
+                    if (kb % KPG == 0)
                         ok = wait_bar_cluster_warp(bar_atom_full(g), (n_grp / Cfg::ATOM_GROUPS) & 1, abort_flag, P, kStatusTimeoutMma);
                     ok = ok && wait_bar_warp(bar_full(s), (n_kb / Cfg::STAGES) & 1, abort_flag, P, kStatusTimeoutMma);
                     if (!ok) break;
-                    const bool group_done = (kb & 3) == 3 || kb == P.kblocks - 1;
+                    const bool group_done = kb % KPG == KPG - 1 || kb == P.kblocks - 1;
                     if (elect_one_sync()) {
-                        const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
-                        const uint32_t sfb = sfa + 4;
-                        const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
-                        {
-                        tc_cp_32x128b_warpx4_pair(sfa, smem_desc_sf(atom));
-                        tc_cp_32x128b_warpx4_pair(sfb, smem_desc_sf(atom + 512));
-                        tc_cp_32x128b_warpx4_pair(sfb + 4, smem_desc_sf(atom + 1024));
-                        }
                         const uint32_t sp = stage_base + s * Cfg::STAGE_BYTES;
                         const uint64_t adesc = smem_desc_sw128(sp);
                         const uint64_t bdesc = smem_desc_sw128(sp + Cfg::P_BYTES);
+                        if constexpr (F4) {
+                            // 256 elements: two sets of atoms, each serving two K = 64 instructions (scale bytes 0-1 and 2-3 of its words)
+#pragma unroll
+                            for (uint32_t h = 0; h < 2; ++h) {
+                                const uint32_t sfa = tmem_base + Cfg::SF_COL + h * 16;
+                                const uint32_t sfb = sfa + 4;
+                                const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + ((kb & 1) * 2 + h) * Cfg::ATOM_BYTES;
+                                tc_cp_32x128b_warpx4_pair(sfa, smem_desc_sf(atom));
+                                tc_cp_32x128b_warpx4_pair(sfb, smem_desc_sf(atom + 512));
+                                tc_cp_32x128b_warpx4_pair(sfb + 4, smem_desc_sf(atom + 1024));
+#pragma unroll
+                                for (uint32_t k = 2 * h; k < 2 * h + 2; ++k)
+                                    mma_mxf4_pair(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(idesc, 2 * (k & 1)),
+                                                  sfa | ((2 * (k & 1)) << 30), sfb | ((2 * (k & 1)) << 30), (kb > 0 || k > 0) ? 1u : 0u);
+                            }
+                        } else {
+                        const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
+                        const uint32_t sfb = sfa + 4;
+                        const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
+                        tc_cp_32x128b_warpx4_pair(sfa, smem_desc_sf(atom));
+                        tc_cp_32x128b_warpx4_pair(sfb, smem_desc_sf(atom + 512));
+                        tc_cp_32x128b_warpx4_pair(sfb + 4, smem_desc_sf(atom + 1024));
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) {
                             mma_mxf8f6f4_pair(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(idesc, k),
                                               sfa | (k << 30), sfb | (k << 30), (kb > 0 || k > 0) ? 1u : 0u);
+                        }
                         }
                         tc_commit_pair(bar_empty(s), 3);
                         if (group_done) tc_commit_pair(bar_atom_empty(g), 3);
@@ -298,7 +316,7 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
         bool ok = true;
         PairUnit u;
         for (int it = 0; ok && pair_unit(P, it, cluster_id, n_clusters, u); ++it) {
-            for (int kb = 0; kb < P.kblocks && ok; kb += 4, ++n_grp) {
+            for (int kb = 0; kb < P.kblocks && ok; kb += KPG, ++n_grp) {
                 if ((int)(n_grp & 1) != warp - 2) continue;
                 uint32_t rp[4][4], rq[8][4];
                 if (P.sf_tma) {
@@ -323,20 +341,20 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                     // four words of one row (16 contiguous bytes), so an instruction touches 8 rows, not 32; each word goes
                     // straight to its place in the atom of its K-block: row (r % 32), 4-byte column (r / 32).
                     const int p0 = u.p0, q0 = u.q0;
-                    const int w = lane & 3;
+                    const int w = kb / KPG * 4 + (lane & 3);           // scale word of the row: 128 elements
                     uint32_t v[48];
 #pragma unroll
                     for (int i = 0; i < 48; ++i) {
                         const int ridx = 8 * i + (lane >> 2);           // 0..127: my rows of P, 128..383: the unit's rows of Q
                         const bool is_p = i < 16;
                         const int row = is_p ? p0 + 128 * (int)rank + ridx : q0 + ridx - 128;
-                        const bool live = row < (is_p ? P.p_rows : P.q_rows) && kb + w < P.kblocks;
-                        v[i] = live ? __ldg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + (kb + w) * 4)) : 0u;
+                        const bool live = row < (is_p ? P.p_rows : P.q_rows) && w < P.sf_words;
+                        v[i] = live ? __ldg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + w * 4)) : 0u;
                     }
                     const int g = n_grp % Cfg::ATOM_GROUPS;
                     ok = wait_bar_warp(bar_atom_empty(g), ((n_grp / Cfg::ATOM_GROUPS) & 1) ^ 1, abort_flag, P, kStatusTimeoutScale);
                     if (!ok) break;
-                    uint8_t* atom = smem_gen + (atom_base - smem_base) + g * Cfg::GROUP_BYTES + w * Cfg::ATOM_BYTES;
+                    uint8_t* atom = smem_gen + (atom_base - smem_base) + g * Cfg::GROUP_BYTES + (lane & 3) * Cfg::ATOM_BYTES;
 #pragma unroll
                     for (int i = 0; i < 48; ++i) {
                         const int ridx = 8 * i + (lane >> 2);

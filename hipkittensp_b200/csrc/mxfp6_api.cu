@@ -64,6 +64,7 @@ struct Options {
     int l2_ahead = 1;        // MXFP6_L2_AHEAD: the single-CTA kernel asks the weights of its first stages into L2 while it waits for the preceding kernel
     int c_tma_last = 1;      // MXFP6_C_TMA_LAST: the unswapped single-CTA kernel drains the last tile of every CTA through its idle ring and TMA stores
     int c_plain = 0;         // MXFP6_C_PLAIN: the pair kernel writes C with plain stores from its staging buffer even where TMA stores are possible
+    int f4 = 1;              // MXFP6_F4: two E2M1 operands take the 4-bit MMA (0: spread to 8-bit slots like a mixed pair)
     int k_rot = 1;           // MXFP6_K_ROT: the even-rows skinny forms start each tile's K loop at its own K-block
 };
 static Options g_opt;
@@ -85,6 +86,7 @@ static bool set_option(const char* name, const char* v) {
         if (v) sscanf(v, "%d,%d", &g_opt.l2_load, &g_opt.l2_store);
     } else if (!strcmp(name, "MXFP6_TAIL_SPLIT")) g_opt.tail_split = v ? atoi(v) : d.tail_split;
     else if (!strcmp(name, "MXFP6_DECODE_ROWS")) g_opt.decode_rows = v ? atoi(v) : d.decode_rows;
+    else if (!strcmp(name, "MXFP6_F4")) g_opt.f4 = v ? atoi(v) : d.f4;
     else if (!strcmp(name, "MXFP6_K_ROT")) g_opt.k_rot = v ? atoi(v) : d.k_rot;
     else if (!strcmp(name, "MXFP6_C_PLAIN")) g_opt.c_plain = v ? atoi(v) : d.c_plain;
     else if (!strcmp(name, "MXFP6_C_TMA_LAST")) g_opt.c_tma_last = v ? atoi(v) : d.c_tma_last;
@@ -98,7 +100,7 @@ static bool set_option(const char* name, const char* v) {
     return true;
 }
 static const char* const kOptionNames[] = {"MXFP6_FORCE_CFG", "MXFP6_NO_SF_TMA", "MXFP6_PDL", "MXFP6_GROUP_P", "MXFP6_QUANT_PATH",
-                                           "MXFP6_WAIT_MS", "MXFP6_L2", "MXFP6_TAIL_SPLIT", "MXFP6_DECODE_ROWS", "MXFP6_DECODE_RING", "MXFP6_K_ROT", "MXFP6_PUSH_ROTATE", "MXFP6_C_PLAIN", "MXFP6_C_TMA_LAST", "MXFP6_L2_AHEAD"};
+                                           "MXFP6_WAIT_MS", "MXFP6_L2", "MXFP6_TAIL_SPLIT", "MXFP6_DECODE_ROWS", "MXFP6_DECODE_RING", "MXFP6_K_ROT", "MXFP6_PUSH_ROTATE", "MXFP6_C_PLAIN", "MXFP6_C_TMA_LAST", "MXFP6_L2_AHEAD", "MXFP6_F4"};
 static const Options& options() {
     std::call_once(g_opt_once, [] {
         for (const char* n : kOptionNames)
@@ -300,12 +302,13 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Most output tiles a problem may have and still split tiles along K (bounds the counter region).
 constexpr int64_t kMaxSplitTiles = 65536;
 
+// kelems: elements of K per K-block of the kernels (128; 256 on the 4-bit path)
 static Plan make_plan(int64_t M, int64_t N, int64_t K, int sm_count, bool allow_pair = true, bool plain = false,
-                      bool even_rows_ok = true) {
+                      bool even_rows_ok = true, int kelems = 128) {
     Plan p{};
     p.ctas = 1;
     const Options& o = options();
-    const int kb = (int)(K / 128);
+    const int kb = (int)((K + kelems - 1) / kelems);
     const int fbn = o.force_bn, fswap = o.force_swap, fsk = o.force_sk, fpair = o.force_pair;
     // Skinny M: the weights are what is streamed.  Up to M = 32 the swapped form (weights on the 128-row side, K-split
     // work units over all SMs) is fastest.  Above that, whole unswapped 128 x 256 tiles stream 256 weight rows per
@@ -438,11 +441,11 @@ static bool dest_by_tma(const Dest& dst) {
     return ok;
 }
 static Plan plan_for(const void* sfa, const void* sfb, const Dest& dst, int64_t M, int64_t N, int64_t K, int sm_count,
-                     bool requant = false) {
+                     bool requant = false, int kelems = 128) {
     // several destinations are written untransposed from whole tiles; a re-quantised result needs tiles that start on
     // multiples of 32 rows and columns
     (void)sfa; (void)sfb; (void)dst;
-    return make_plan(M, N, K, sm_count, true, dst.n > 1, !requant);
+    return make_plan(M, N, K, sm_count, true, dst.n > 1, !requant, kelems);
 }
 
 // Everything a call passes in.  Two calls with equal keys launch the same kernel with the same arguments, so the
@@ -598,7 +601,9 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     DeviceState& d = *dp;
     const Options& o = options();
     const bool sf_tma = scales_by_tma(sfa, sfb, K);
-    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d.sm_count, q_fmt >= 0);
+    const bool f4 = fmt_a == MXFP4_E2M1 && fmt_b == MXFP4_E2M1 && o.f4;      // the 4-bit MMA takes two E2M1 operands
+    const int kelems = f4 ? 256 : 128;
+    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d.sm_count, q_fmt >= 0, kelems);
 
     Recipe r;
     r.key = key;
@@ -629,10 +634,14 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     const int fp = pl.swap ? fmt_b : fmt_a, fq = pl.swap ? fmt_a : fmt_b;
 
     const int p_box = pl.pair ? 128 : pl.p_tile, q_box = pl.pair ? 128 : pl.q_tile;      // rows one operand load brings
-    if ((rc = make_map(pp, prow, K, p_box, fmt_map_kind(fp), &r.tp))) return rc;
-    if ((rc = make_map(qp, qrow, K, q_box, fmt_map_kind(fq), &r.tq))) return rc;
+    // (the 4-bit MMA wants two elements per byte in shared memory, as they lie in HBM: a map of bytes.  The half K-block past
+    // an odd K / 128 is filled with zeros.)
+    const int64_t k_inner = f4 ? K / 2 : K;
+    const int kind_p = f4 ? 3 : fmt_map_kind(fp), kind_q = f4 ? 3 : fmt_map_kind(fq);
+    if ((rc = make_map(pp, prow, k_inner, p_box, kind_p, &r.tp))) return rc;
+    if ((rc = make_map(qp, qrow, k_inner, q_box, kind_q, &r.tq))) return rc;
     r.tq_tail = r.tq;
-    if (pl.pair && pl.tail_split > 1 && (rc = make_map(qp, qrow, K, 128 / pl.tail_split, fmt_map_kind(fq), &r.tq_tail))) return rc;
+    if (pl.pair && pl.tail_split > 1 && (rc = make_map(qp, qrow, k_inner, 128 / pl.tail_split, kind_q, &r.tq_tail))) return rc;
     if (sf_tma) {
         if ((rc = make_map(sp, prow, K / 32, p_box, 1, &r.tsp))) return rc;
         if ((rc = make_map(sq, qrow, K / 32, pl.q_tile, 1, &r.tsq))) return rc;   // pair kernel: all 256 Q rows per CTA
@@ -643,7 +652,8 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     GemmParams& P = r.P;
     memset(&P, 0, sizeof P);
     P.p_rows = (int)prow; P.q_rows = (int)qrow;
-    P.kblocks = (int)(K / 128);
+    P.kblocks = (int)((K + kelems - 1) / kelems);
+    P.sf_words = (int)(K / 128);
     P.tiles_p = pl.tiles_p; P.tiles_q = pl.tiles_q;
     P.p_tile_rows = pl.p_tile; P.q_tile_rows = pl.q_tile;
     P.raw_tx_bytes = (p_box + pl.q_tile) * 16;
@@ -664,7 +674,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
         if (o.decode_batch >= 1 && o.decode_batch <= ns / 2) P.load_batch = o.decode_batch;
         // the even-rows forms of skinny problems (tiles narrower than a box) rotate their K loops
         const bool even_rows = pl.ctas == 2 || pl.q_tile != pl.bn;
-        P.k_rot = (even_rows && o.k_rot && (K / 128) % 4 == 0) ? 1 : 0;
+        P.k_rot = (even_rows && o.k_rot && K % 512 == 0) ? 1 : 0;      // whole scale groups
     }
     P.ldc = (int)dst.ldc; P.c_rows = (int)M; P.c_cols = (int)N;
     // The instruction's N: the accumulator's width, or, where an unswapped tile is narrower than its accumulator (the
@@ -672,13 +682,14 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     // not multiply the stale rows behind the tile (a fifth of the MMA work and of its power there).
     uint32_t mma_n = (uint32_t)pl.bn;
     if (!pl.pair && !pl.swap && pl.q_tile < pl.bn) mma_n = (uint32_t)((pl.q_tile + 15) / 16 * 16);
-    P.idesc = make_idesc_m(fmt_mma_code(fp), fmt_mma_code(fq), pl.pair ? 256u : 128u, mma_n);
+    P.idesc = make_idesc_m(f4 ? kMxf4E2M1 : fmt_mma_code(fp), f4 ? kMxf4E2M1 : fmt_mma_code(fq), pl.pair ? 256u : 128u, mma_n);
     P.sf_tma = sf_tma ? 1 : 0;
     P.sf_ld = (int)(K / 32);
     // bytes a stage's two loads credit to its mbarrier: the global bytes of the boxes (fp6: 96, fp4: 64 per 128 elements)
-    P.stage_tx_bytes = p_box * fmt_row_bytes_per_128(fp) + q_box * fmt_row_bytes_per_128(fq);
+    const int row_p = f4 ? 128 : fmt_row_bytes_per_128(fp), row_q = f4 ? 128 : fmt_row_bytes_per_128(fq);
+    P.stage_tx_bytes = p_box * row_p + q_box * row_q;
     P.tail_first = pl.tail_first; P.tail_split = pl.tail_split;
-    P.stage_tx_bytes_tail = p_box * fmt_row_bytes_per_128(fp) + (128 / pl.tail_split) * fmt_row_bytes_per_128(fq);
+    P.stage_tx_bytes_tail = p_box * row_p + (128 / pl.tail_split) * row_q;
     P.sfp = (const uint8_t*)sp; P.sfq = (const uint8_t*)sq;
     P.c = (__nv_bfloat16*)c;
     for (int i = 1; i < dst.n; ++i) P.c_more[i - 1] = (__nv_bfloat16*)dst.c[i];
@@ -714,7 +725,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     r.grid = pl.grid;
     r.pair = pl.pair;
     if (pl.pair) {
-        r.func = (const void*)mxfp6_gemm_pair_kernel;
+        r.func = f4 ? (const void*)mxfp6_gemm_pair_kernel<true> : (const void*)mxfp6_gemm_pair_kernel<false>;
         r.threads = PairCfg::THREADS;
         r.smem = PairCfg::SMEM_ALLOC;
         if ((rc = ensure_smem_attr(d, r.func, PairCfg::SMEM_ALLOC))) return rc;
@@ -730,10 +741,12 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
         r.tc = r.tp;            // (the slot only has to hold a valid map when the kernel does not use it)
         if (P.c_tma_last && (rc = make_map(dst.c[0], M, N, 128, 2, &r.tc, dst.ldc * 2))) return rc;
         rc = -1;
-#define MXFP6_CASE(BN_, SWAP_, SK_)                                                              \
-        if (pl.ctas == 1 && pl.bn == BN_ && pl.swap == SWAP_ && pl.streamk == SK_) rc = bind_cfg<GemmCfg<BN_, SWAP_, SK_>>(d, r);
-        if (pl.ctas == 2 && pl.bn == 16 && pl.swap && !pl.streamk) rc = bind_cfg<GemmCfg<16, true, false, 2>>(d, r);
-        if (pl.ctas == 2 && pl.bn == 32 && pl.swap && !pl.streamk) rc = bind_cfg<GemmCfg<32, true, false, 2>>(d, r);
+#define MXFP6_CASE2(BN_, SWAP_, SK_, CTAS_)                                                      \
+        if (pl.ctas == CTAS_ && pl.bn == BN_ && pl.swap == SWAP_ && pl.streamk == SK_)           \
+            rc = f4 ? bind_cfg<GemmCfg<BN_, SWAP_, SK_, CTAS_, true>>(d, r) : bind_cfg<GemmCfg<BN_, SWAP_, SK_, CTAS_>>(d, r);
+#define MXFP6_CASE(BN_, SWAP_, SK_) MXFP6_CASE2(BN_, SWAP_, SK_, 1)
+        MXFP6_CASE2(16, true, false, 2)
+        MXFP6_CASE2(32, true, false, 2)
         MXFP6_CASE(256, false, false)
         MXFP6_CASE(128, false, false)
         MXFP6_CASE(256, false, true)
@@ -747,6 +760,7 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
         MXFP6_CASE(64, true, false)
         MXFP6_CASE(128, true, false)
 #undef MXFP6_CASE
+#undef MXFP6_CASE2
         if (rc == -1) return fail(MXFP6_ERR_BAD_ARG, "no kernel for bn=%d swap=%d streamk=%d", pl.bn, (int)pl.swap, (int)pl.streamk);
         if (rc) return rc;
     }
@@ -872,7 +886,10 @@ extern "C" size_t mxfp6_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
     DeviceState* d = nullptr;
     if (get_device_state(&d)) return 0;
-    return make_plan(M, N, K, d->sm_count).ws_bytes;
+    // the formats are not known here: the 4-bit path splits its (longer) K-blocks a little differently
+    const size_t wide = make_plan(M, N, K, d->sm_count).ws_bytes;
+    const size_t f4 = make_plan(M, N, K, d->sm_count, true, false, true, 256).ws_bytes;
+    return wide > f4 ? wide : f4;
 }
 
 extern "C" int mxfp6_gemm_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,

@@ -16,7 +16,7 @@ FP4 = R.E2M1
 @pytest.fixture(autouse=True)
 def _clean_options():
     yield
-    for name in ("MXFP6_FORCE_CFG", "MXFP6_NO_SF_TMA", "MXFP6_QUANT_PATH"):
+    for name in ("MXFP6_FORCE_CFG", "MXFP6_NO_SF_TMA", "MXFP6_QUANT_PATH", "MXFP6_F4"):
         hk.debug_option(name, None)
 
 
@@ -111,6 +111,28 @@ def _run(M, N, K, fa, fb, force=None, seed=0, config="lognormal"):
 @pytest.mark.parametrize("shape", SHAPES)
 def test_products(shape, pair):
     _run(*shape, *pair, seed=sum(shape))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_products_on_spread_nibbles(shape):
+    """Two E2M1 operands on the 8-bit path of the mixed pairs: the same sums."""
+    hk.debug_option("MXFP6_F4", "0")
+    _run(*shape, FP4, FP4, seed=sum(shape))
+
+
+@pytest.mark.parametrize("shape", [(16, 512, 1024), (64, 640, 384), (130, 200, 1152)])
+def test_caller_workspace(shape):
+    """mxfp6_gemm_ws with exactly the bytes the library asks for, on the 4-bit path and with a mixed pair."""
+    M, N, K = shape
+    need = hk.lib.mxfp6_gemm_workspace_bytes(M, N, K)
+    for fa in (FP4, R.E4M3):
+        pa, sa, pb, sb = quantized_inputs("normal", M, N, K, fa, 1, FP4)
+        t = [torch.from_numpy(x).cuda() for x in (pa, sa, pb, sb)]
+        ws, C = torch.zeros(max(need, 1), dtype=torch.uint8, device="cuda"), torch.empty(M, N, dtype=torch.bfloat16, device="cuda")
+        rc = hk.lib.mxfp6_gemm_ws(*[x.data_ptr() for x in t], C.data_ptr(), M, N, K, fa, FP4, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, hk.lib.mxfp6_last_error()
+        assert hk.device_status() == 0
+        check(C.float().cpu().numpy(), *oracle_f64(pa, sa, pb, sb, fa, FP4))
 
 
 @pytest.mark.parametrize("pair", PAIRS[:2])
