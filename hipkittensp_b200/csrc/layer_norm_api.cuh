@@ -7,56 +7,64 @@ namespace mxfp6 {
 typedef void (*LnKernel)(const LnParams);
 struct LnChoice {
     LnKernel kern;
-    int warps;       // warps that share a row; one: eight rows per CTA
+    int warps;       // warps that share a row; one: eight rows per CTA; none: a CTA of 1024 threads passes over the row again
+    int smem;        // dynamic shared memory
 };
 
-// A thread holds up to 32 elements of a row, sixteen warps a row: 16384 elements; longer rows (warps = 0) are passed over again.
-template <typename T, bool MX>
-static LnChoice ln_forward_kernel(bool vec, int H) {
-    if (vec) {
-        if (H <= 256) return {layer_norm_kernel<T, 8, 1, 1, MX>, 1};
-        if (H <= 512) return {layer_norm_kernel<T, 8, 2, 1, MX>, 1};
-        if (H <= 1024) return {layer_norm_kernel<T, 8, 4, 1, MX>, 1};
-        if (H <= 2048) return {layer_norm_kernel<T, 8, 4, 2, MX>, 2};
-        if (H <= 4096) return {layer_norm_kernel<T, 8, 4, 4, MX>, 4};
-        if (H <= 8192) return {layer_norm_kernel<T, 8, 4, 8, MX>, 8};
-        if (H <= 16384) return {layer_norm_kernel<T, 8, 4, 16, MX>, 16};
-        return {layer_norm_long_kernel<T, 8, MX>, 0};
-    }
-    if constexpr (!MX) {        // (an MX result has whole blocks and aligned pointers)
-        if (H <= 256) return {layer_norm_kernel<T, 1, 8, 1, false>, 1};
-        if (H <= 1024) return {layer_norm_kernel<T, 1, 32, 1, false>, 1};
-        if (H <= 2048) return {layer_norm_kernel<T, 1, 32, 2, false>, 2};
-        if (H <= 4096) return {layer_norm_kernel<T, 1, 32, 4, false>, 4};
-        if (H <= 8192) return {layer_norm_kernel<T, 1, 32, 8, false>, 8};
-        if (H <= 16384) return {layer_norm_kernel<T, 1, 32, 16, false>, 16};
-        return {layer_norm_long_kernel<T, 1, false>, 0};
-    }
-    return {nullptr, 0};
+// Whole 8-element chunks: a thread holds up to four, sixteen warps a row: 16384 elements.
+template <typename T, int BITS>
+static LnChoice ln_forward_vec(int H) {
+    const int smem = 8 * H;          // w and b as fp32
+    if (H <= 256) return {layer_norm_kernel<T, 1, 1, BITS>, 1, smem};
+    if (H <= 1024) return {layer_norm_kernel<T, 4, 1, BITS>, 1, smem};
+    if (H <= 2048) return {layer_norm_kernel<T, 4, 2, BITS>, 2, smem};
+    if (H <= 4096) return {layer_norm_kernel<T, 4, 4, BITS>, 4, smem};
+    if (H <= 8192) return {layer_norm_kernel<T, 4, 8, BITS>, 8, smem};
+    if (H <= 16384) return {layer_norm_kernel<T, 4, 16, BITS>, 16, smem};
+    return {layer_norm_long_kernel<T, 8, BITS>, 0, 0};
+}
+template <typename T>
+static LnChoice ln_forward_odd(int H) {
+    if (H <= 256) return {layer_norm_odd_kernel<T, 8, 1>, 1, 0};
+    if (H <= 512) return {layer_norm_odd_kernel<T, 8, 2>, 2, 0};
+    if (H <= 1024) return {layer_norm_odd_kernel<T, 8, 4>, 4, 0};
+    if (H <= 2048) return {layer_norm_odd_kernel<T, 8, 8>, 8, 0};
+    if (H <= 4096) return {layer_norm_odd_kernel<T, 8, 16>, 16, 0};
+    if (H <= 8192) return {layer_norm_odd_kernel<T, 16, 16>, 16, 0};
+    if (H <= 16384) return {layer_norm_odd_kernel<T, 32, 16>, 16, 0};
+    return {layer_norm_long_kernel<T, 1, 0>, 0, 0};
+}
+// bits: element width of an MX result, 0 for one in x's type
+template <typename T>
+static LnChoice ln_forward_kernel(bool vec, int bits, int H) {
+    if (!vec) return ln_forward_odd<T>(H);
+    return bits == 0 ? ln_forward_vec<T, 0>(H) : bits == 4 ? ln_forward_vec<T, 4>(H) : bits == 6 ? ln_forward_vec<T, 6>(H) : ln_forward_vec<T, 8>(H);
 }
 
 // Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row.
 constexpr int kLnBackwardMax = 8192;
 static int ln_backward_warps(int H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
 template <typename T>
-static LnKernel ln_backward_kernel(bool vec, int H) {
+static LnChoice ln_backward_kernel(bool vec, int H) {
+    const int warps = ln_backward_warps(H);
     if (vec) {
-        if (H <= 256) return layer_norm_backward_kernel<T, 8, 1, 1>;
-        switch (ln_backward_warps(H)) {
-            case 1: return layer_norm_backward_kernel<T, 8, 2, 1>;
-            case 2: return layer_norm_backward_kernel<T, 8, 2, 2>;
-            case 4: return layer_norm_backward_kernel<T, 8, 2, 4>;
-            case 8: return layer_norm_backward_kernel<T, 8, 2, 8>;
-            default: return layer_norm_backward_kernel<T, 8, 2, 16>;
+        // w as fp32; one warp per row: room for the eight warps' column sums
+        if (H <= 256) return {layer_norm_backward_kernel<T, 1, 1>, 1, 8 * 256 * 4};
+        switch (warps) {
+            case 1: return {layer_norm_backward_kernel<T, 2, 1>, 1, 8 * 512 * 4};
+            case 2: return {layer_norm_backward_kernel<T, 2, 2>, 2, 4 * H};
+            case 4: return {layer_norm_backward_kernel<T, 2, 4>, 4, 4 * H};
+            case 8: return {layer_norm_backward_kernel<T, 2, 8>, 8, 4 * H};
+            default: return {layer_norm_backward_kernel<T, 2, 16>, 16, 4 * H};
         }
     }
-    if (H <= 256) return layer_norm_backward_kernel<T, 1, 8, 1>;
-    switch (ln_backward_warps(H)) {
-        case 1: return layer_norm_backward_kernel<T, 1, 16, 1>;
-        case 2: return layer_norm_backward_kernel<T, 1, 16, 2>;
-        case 4: return layer_norm_backward_kernel<T, 1, 16, 4>;
-        case 8: return layer_norm_backward_kernel<T, 1, 16, 8>;
-        default: return layer_norm_backward_kernel<T, 1, 16, 16>;
+    if (H <= 256) return {layer_norm_backward_odd_kernel<T, 8, 1>, 1, 0};
+    switch (warps) {
+        case 1: return {layer_norm_backward_odd_kernel<T, 16, 1>, 1, 0};
+        case 2: return {layer_norm_backward_odd_kernel<T, 16, 2>, 2, 0};
+        case 4: return {layer_norm_backward_odd_kernel<T, 16, 4>, 4, 0};
+        case 8: return {layer_norm_backward_odd_kernel<T, 16, 8>, 8, 0};
+        default: return {layer_norm_backward_odd_kernel<T, 16, 16>, 16, 0};
     }
 }
 
@@ -103,18 +111,18 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
         return fail(MXFP6_ERR_BAD_ARG, "%s: x must be 32-byte (fp32) or 16-byte (bf16) aligned, weight, bias and codes 16-byte", what);
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
-    const LnChoice k = x_dtype == 0 ? (mx ? ln_forward_kernel<float, true>(vec, (int)H) : ln_forward_kernel<float, false>(vec, (int)H))
-                                    : (mx ? ln_forward_kernel<__nv_bfloat16, true>(vec, (int)H) : ln_forward_kernel<__nv_bfloat16, false>(vec, (int)H));
+    const int bits = mx ? fmt_block_bytes(fmt) / 4 : 0;
+    const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(vec, bits, (int)H) : ln_forward_kernel<__nv_bfloat16>(vec, bits, (int)H);
     const int threads = k.warps == 0 ? 1024 : k.warps == 1 ? 256 : 32 * k.warps;
     int per_sm = 0;
-    if ((rc = resident_ctas(*d, (const void*)k.kern, threads, &per_sm))) return rc;
+    if ((rc = resident_ctas(*d, (const void*)k.kern, threads, k.smem, &per_sm))) return rc;
     const int64_t want = k.warps == 1 ? (rows + 7) / 8 : rows, cap = (int64_t)d->sm_count * per_sm;
     LnParams P{};
     P.x = x; P.y = y; P.w = w; P.b = b; P.w_bf16 = w_dtype;
     P.mean = mean; P.rstd = rstd;
     P.q_out = (uint8_t*)packed; P.q_scales = (uint8_t*)scales; P.q_fmt = fmt;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H; P.eps = eps;
-    return launch_pdl(k.kern, (unsigned)(want < cap ? want : cap), (unsigned)threads, 0, (cudaStream_t)stream, P);
+    return launch_pdl(k.kern, (unsigned)(want < cap ? want : cap), (unsigned)threads, (size_t)k.smem, (cudaStream_t)stream, P);
 }
 
 static int ln_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd, const void* w, int w_dtype,
@@ -147,9 +155,8 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     P.part = sums ? (float*)ws : nullptr;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H;
     if (H <= kLnBackwardMax) {
-        const LnKernel k = x_dtype == 0 ? ln_backward_kernel<float>(vec, (int)H) : ln_backward_kernel<__nv_bfloat16>(vec, (int)H);
-        const int warps = ln_backward_warps((int)H);
-        if ((rc = launch_pdl(k, (unsigned)parts, (unsigned)(warps == 1 ? 256 : 32 * warps), 0, st, P))) return rc;
+        const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(vec, (int)H) : ln_backward_kernel<__nv_bfloat16>(vec, (int)H);
+        if ((rc = launch_pdl(k.kern, (unsigned)parts, (unsigned)(k.warps == 1 ? 256 : 32 * k.warps), (size_t)k.smem, st, P))) return rc;
     } else {
         if (sums) {
             LnKernel k = x_dtype == 0 ? layer_norm_columns_kernel<float> : layer_norm_columns_kernel<__nv_bfloat16>;

@@ -140,105 +140,220 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
     }
 }
 
-// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes and scale.
-__device__ __forceinline__ void mx_store8(const float (&v)[8], int fmt, uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
-    float amax = fmaxf(amax3(v[0], v[1], v[2]), fmaxf(amax3(v[3], v[4], v[5]), fmaxf(fabsf(v[6]), fabsf(v[7]))));
+// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes of BITS bits and scale.
+template <int BITS>
+__device__ __forceinline__ void mx_store8(const float2 (&v)[4], int fmt, uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
+    float amax = amax3(amax3(v[0].x, v[0].y, v[1].x), amax3(v[1].y, v[2].x, v[2].y), fmaxf(fabsf(v[3].x), fabsf(v[3].y)));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const int sb = quant_scale_byte(amax, fmt);
     const float f = quant_inv_scale(sb);
     float s[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = v[i] * f;
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = __fmul2_rn(v[i], make_float2(f, f));
+        s[2 * i] = t.x; s[2 * i + 1] = t.y;
+    }
     const int j = (col >> 3) & 3;                   // place of these eight in their block
-    if (fmt == kE2M1) {
+    if constexpr (BITS == 4) {
         const uint32_t w = cvt_oct_e2m1(s);
         if (live) *reinterpret_cast<uint32_t*>(codes_row + col / 2) = w;
-    } else if (fmt_fp8(fmt)) {
-        const uint32_t w0 = cvt_quad_rt(s[0], s[1], s[2], s[3], fmt), w1 = cvt_quad_rt(s[4], s[5], s[6], s[7], fmt);
-        if (live) *reinterpret_cast<uint2*>(codes_row + col) = make_uint2(w0, w1);
+    } else if constexpr (BITS == 8) {
+        uint2 w;
+        if (fmt == kE4M3) w = make_uint2(cvt_quad<kE4M3>(s[0], s[1], s[2], s[3]), cvt_quad<kE4M3>(s[4], s[5], s[6], s[7]));
+        else w = make_uint2(cvt_quad<kE5M2>(s[0], s[1], s[2], s[3]), cvt_quad<kE5M2>(s[4], s[5], s[6], s[7]));
+        if (live) *reinterpret_cast<uint2*>(codes_row + col) = w;
     } else {
-        // 48 bits a lane: four lanes hold 24 bytes, which three of them write
-        const uint64_t w = (uint64_t)cvt_quad_rt(s[0], s[1], s[2], s[3], fmt) | ((uint64_t)cvt_quad_rt(s[4], s[5], s[6], s[7], fmt) << 24);
-        const uint64_t nx = (uint64_t)__shfl_down_sync(0xffffffffu, (unsigned long long)w, 1);
-        if (live && j < 3) *reinterpret_cast<uint64_t*>(codes_row + (col / 32) * 24 + 8 * j) = (w >> (16 * j)) | (nx << (48 - 16 * j));
+        uint32_t lo, hi;                            // 24 bits each
+        if (fmt == kE2M3) { lo = cvt_quad<kE2M3>(s[0], s[1], s[2], s[3]); hi = cvt_quad<kE2M3>(s[4], s[5], s[6], s[7]); }
+        else { lo = cvt_quad<kE3M2>(s[0], s[1], s[2], s[3]); hi = cvt_quad<kE3M2>(s[4], s[5], s[6], s[7]); }
+        // 48 bits a lane: four lanes hold 24 bytes, which three of them write, 8 each: lane j the bits from 64 j on, which start at
+        // bit 16 j of its own 48 and run on into its neighbour's
+        const uint32_t w0 = lo | (hi << 24), w1 = hi >> 8;
+        const uint32_t n0 = __shfl_down_sync(0xffffffffu, w0, 1), n1 = __shfl_down_sync(0xffffffffu, w1, 1);
+        const uint32_t a = j == 2 ? w1 : w0, b = j == 2 ? n0 : w1, c = j == 2 ? n1 : n0;
+        const uint32_t o0 = __byte_perm(a, b, j == 0 ? 0x3210 : j == 1 ? 0x5432 : 0x5410);
+        const uint32_t o1 = __byte_perm(b, c, j == 0 ? 0x5410 : j == 1 ? 0x7654 : 0x5432);
+        if (live && j < 3) *reinterpret_cast<uint2*>(codes_row + (col / 32) * 24 + 8 * j) = make_uint2(o0, o1);
     }
     if (live && j == 0) scales_row[col / 32] = (uint8_t)sb;
 }
 
+// Parameter vectors in shared memory, as fp32 whatever their type and filled where they are absent: float4 planes of H / 8
+// (the low halves of the 8-element chunks, then the high halves), so that neighbouring threads read neighbouring 16 bytes.
+__device__ __forceinline__ void stage_param(const void* w, int is_bf16, float fill, int H, float4* plane) {
+    const int n = H >> 3;
+    for (int c = threadIdx.x; c < n; c += blockDim.x) {
+        float v[8];
+        ld_param<8>(w, is_bf16, 8 * c, fill, v);
+        plane[c] = make_float4(v[0], v[1], v[2], v[3]);
+        plane[n + c] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+__device__ __forceinline__ void ld_staged(const float4* plane, int n, int chunk, float2 (&v)[4]) {
+    const float4 lo = plane[chunk], hi = plane[n + chunk];
+    v[0] = make_float2(lo.x, lo.y); v[1] = make_float2(lo.z, lo.w); v[2] = make_float2(hi.x, hi.y); v[3] = make_float2(hi.z, hi.w);
+}
+template <typename T>
+__device__ __forceinline__ void unpack2(const Raw<T, 8>& r, float2 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = make_float2(__uint_as_float(r.u[2 * i]), __uint_as_float(r.u[2 * i + 1]));
+        else v[i] = make_float2(bf16_lo(r.u[i]), bf16_hi(r.u[i]));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void st_row2(T* p, const float2 (&v)[4]) {
+    const float t[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+    st_row<T, 8>(p, t);
+}
+
 // ---------------------------------------------------------------------------------- forward
-// WARPS warps own a row, V * C elements per thread.  WARPS = 1: eight warps per CTA with a row each.  MX: the result leaves as codes and scales.
-template <typename T, int V, int C, int WARPS, bool MX>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+// WARPS warps own a row, C chunks of 8 elements per thread.  WARPS = 1: eight warps per CTA with a row each.  BITS = 0: the result is
+// written in x's type; 4, 6, 8: it leaves as codes and scales.  The next row is on its way in registers while this one is worked
+// on, the arithmetic runs on pairs (fma.f32x2), and the parameters are staged once per CTA: bf16 rows are bound by issue, not by
+// HBM, when each element costs 25 instructions (16384 x 8192 in 124 us).
+template <typename T, int C, int WARPS, int BITS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 16 ? 1 : WARPS == 1 ? 2 : 16 / WARPS)
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     constexpr int ROWS = WARPS == 1 ? 8 : 1;                    // rows a CTA works on at a time
+    __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
+    extern __shared__ float4 prm[];                             // w, then b
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int n8 = P.H >> 3;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
+    const T* x = reinterpret_cast<const T*>(P.x);
+    Raw<T, 8> raw[C];
+    auto load = [&](int64_t r) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            if (r < P.rows && chunk < n8) raw[c] = ld_raw<T, 8>(x + r * P.H + 8 * chunk);
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};           // columns past H stay zero
+    load(row);
+    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
+    stage_param(P.b, P.w_bf16, 0.f, P.H, prm + 2 * n8);
+    __syncthreads();
+    for (int par = 0; row < P.rows; row += step, par ^= 1) {
+        float2 v[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c) unpack2<T>(raw[c], v[c]);
+        load(row + step);
+        float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s2 = __fadd2_rn(s2, v[c][i]);
+        float s[1] = {s2.x + s2.y};
+        row_sum<1, WARPS>(s, red[par]);
+        const float mean0 = s[0] * P.inv_h;
+        float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (tid + c * TPR < n8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[c][i] = __fadd2_rn(v[c][i], make_float2(-mean0, -mean0));
+                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                    d2 = __fadd2_rn(d2, v[c][i]);
+                }
+            }
+        }
+        float q[2] = {q2.x + q2.y, d2.x + d2.y};
+        row_sum<2, WARPS>(q, red2[par]);
+        const float corr = q[1] * P.inv_h;
+        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
+        if (tid == 0) {
+            if (P.mean) P.mean[row] = mean0 + corr;
+            if (P.rstd) P.rstd[row] = rstd;
+        }
+        const float shift = -corr * rstd;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            const bool live = chunk < n8;
+            float2 o[4];
+            if (live) {
+                float2 w[4], b[4];
+                ld_staged(prm, n8, chunk, w);
+                ld_staged(prm + 2 * n8, n8, chunk, b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
+            }
+            if constexpr (BITS) {
+                if (!live)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = make_float2(0.f, 0.f);
+                mx_store8<BITS>(o, P.q_fmt, P.q_out + row * (P.H / 32) * (4 * BITS), P.q_scales + row * (P.H / 32), 8 * chunk, live);
+            } else if (live) {
+                st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, o);
+            }
+        }
+    }
+}
+
+// Rows of any width and alignment (the result in x's type): V = 1 element per access, C per thread.
+template <typename T, int C, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+layer_norm_odd_kernel(const LnParams P) {
+    constexpr int TPR = 32 * WARPS;
+    constexpr int ROWS = WARPS == 1 ? 8 : 1;
     __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
     pdl_launch_dependents();
     pdl_wait();
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * ROWS;
-    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
-    const T* x = reinterpret_cast<const T*>(P.x);
-    Raw<T, V> cur[C];
-    auto load = [&](int64_t r, Raw<T, V> (&dst)[C]) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = (tid + c * TPR) * V;
-            dst[c] = Raw<T, V>{};
-            if (r < P.rows && col < P.H) dst[c] = ld_raw<T, V>(x + r * P.H + col);
-        }
-    };
-    load(row, cur);
-    for (int par = 0; row < P.rows; row += step, par ^= 1) {
-        // the next row is on its way while this one is worked on
-        Raw<T, V> nxt[C];
-        load(row + step, nxt);
-        float v[C][V];
+    int par = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0); row < P.rows; row += step, par ^= 1) {
+        const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
+        float v[C];
         float s[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            unpack<T, V>(cur[c], v[c]);                          // columns past H hold zeros
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[0] += v[c][i];
+            const int col = tid + c * TPR;
+            float t[1] = {0.f};
+            if (col < P.H) unpack<T, 1>(ld_raw<T, 1>(x + col), t);
+            v[c] = t[0];
         }
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[0] += v[c];
         row_sum<1, WARPS>(s, red[par]);
         const float mean0 = s[0] * P.inv_h;
         float q[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if ((tid + c * TPR) * V < P.H) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) { v[c][i] -= mean0; q[0] = fmaf(v[c][i], v[c][i], q[0]); q[1] += v[c][i]; }
-            }
-        }
+        for (int c = 0; c < C; ++c)
+            if (tid + c * TPR < P.H) { v[c] -= mean0; q[0] = fmaf(v[c], v[c], q[0]); q[1] += v[c]; }
         row_sum<2, WARPS>(q, red2[par]);
-        const float corr = q[1] * P.inv_h, mean = mean0 + corr;
+        const float corr = q[1] * P.inv_h;
         const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
-        if (tid == 0 && P.mean) P.mean[row] = mean;
+        if (tid == 0 && P.mean) P.mean[row] = mean0 + corr;
         if (tid == 0 && P.rstd) P.rstd[row] = rstd;
+        const float shift = -corr * rstd;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (tid + c * TPR) * V;
-            const bool live = col < P.H;
-            float w[V], b[V], o[V];
-            if (live) { ld_param<V>(P.w, P.w_bf16, col, 1.f, w); ld_param<V>(P.b, P.w_bf16, col, 0.f, b); }
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = live ? fmaf((v[c][i] - corr) * rstd, w[i], b[i]) : 0.f;
-            if constexpr (MX) {
-                mx_store8(o, P.q_fmt, P.q_out + row * (P.H / 32) * fmt_block_bytes(P.q_fmt), P.q_scales + row * (P.H / 32), col, live);
-            } else if (live) {
-                st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
+            const int col = tid + c * TPR;
+            if (col < P.H) {
+                float w[1], b[1];
+                ld_param<1>(P.w, P.w_bf16, col, 1.f, w);
+                ld_param<1>(P.b, P.w_bf16, col, 0.f, b);
+                const float o[1] = {fmaf(fmaf(v[c], rstd, shift), w[0], b[0])};
+                st_row<T, 1>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
             }
         }
-#pragma unroll
-        for (int c = 0; c < C; ++c) cur[c] = nxt[c];
     }
 }
 
 // Rows longer than the registers of a CTA hold: a CTA of 1024 threads passes over its row three times (the second and third
 // pass find it in L2).
-template <typename T, int V, bool MX>
+template <typename T, int V, int BITS>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P) {
     __shared__ float red[32], red2[64];
     pdl_launch_dependents();
@@ -263,10 +378,11 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
             for (int i = 0; i < V; ++i) { const float d = v[i] - mean0; q[0] = fmaf(d, d, q[0]); q[1] += d; }
         }
         row_sum<2, 32>(q, red2);
-        const float corr = q[1] * P.inv_h, mean = mean0 + corr;
+        const float corr = q[1] * P.inv_h;
         const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
-        if (threadIdx.x == 0 && P.mean) P.mean[row] = mean;
+        if (threadIdx.x == 0 && P.mean) P.mean[row] = mean0 + corr;
         if (threadIdx.x == 0 && P.rstd) P.rstd[row] = rstd;
+        const float shift = -corr * rstd;
         // every thread makes the same number of rounds: the lanes of a block exchange their largest magnitudes
         for (int c0 = 0; c0 < P.H; c0 += 1024 * V) {
             const int col = c0 + threadIdx.x * V;
@@ -279,10 +395,11 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
                 ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
                 ld_param<V>(P.b, P.w_bf16, col, 0.f, b);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = fmaf((v[i] - mean0 - corr) * rstd, w[i], b[i]);
+                for (int i = 0; i < V; ++i) v[i] = fmaf(fmaf(v[i] - mean0, rstd, shift), w[i], b[i]);
             }
-            if constexpr (MX) {
-                mx_store8(v, P.q_fmt, P.q_out + row * (P.H / 32) * fmt_block_bytes(P.q_fmt), P.q_scales + row * (P.H / 32), col, live);
+            if constexpr (BITS) {
+                const float2 o[4] = {make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]), make_float2(v[6], v[7])};
+                mx_store8<BITS>(o, P.q_fmt, P.q_out + row * (P.H / 32) * (4 * BITS), P.q_scales + row * (P.H / 32), col, live);
             } else if (live) {
                 st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, v);
             }
@@ -291,57 +408,177 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
 }
 
 // ---------------------------------------------------------------------------------- backward
-template <typename T, int V, int C, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+// WARPS warps own a row, C chunks of 8 columns per thread; the same columns of every row, whose parameter gradients the thread
+// sums in registers.  As in the forward kernel the next row is on its way while this one is worked on (without that, HBM idles
+// through every row's reduction: 16384 x 8192 bf16 in 273 us) and the arithmetic runs on pairs.
+template <typename T, int C, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 : 16 / WARPS)
 layer_norm_backward_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     constexpr int ROWS = WARPS == 1 ? 8 : 1;
     __shared__ float red[2][2 * WARPS];
-    __shared__ float fold[WARPS == 1 ? 8 * 32 * V * C : 1];     // one warp per row: the warps' column sums meet here
+    extern __shared__ float4 prm[];                             // w; at the end the warps' column sums (one warp per row)
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int n8 = P.H >> 3;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const T* dy = reinterpret_cast<const T*>(P.dy);
+    Raw<T, 8> rx[C], rg[C];
+    float mean_n = 0.f, rstd_n = 0.f;
+    auto load = [&](int64_t r) {
+        if (r < P.rows) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int chunk = tid + c * TPR;
+                if (chunk < n8) {
+                    rx[c] = ld_raw<T, 8>(x + r * P.H + 8 * chunk);
+                    rg[c] = ld_raw<T, 8>(dy + r * P.H + 8 * chunk);
+                }
+            }
+            mean_n = __ldcg(P.mean + r);
+            rstd_n = __ldcg(P.rstd + r);
+        }
+    };
+    float2 dw[C][4], db[C][4];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        rx[c] = Raw<T, 8>{}; rg[c] = Raw<T, 8>{};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = make_float2(0.f, 0.f);
+    }
+    load(row);
+    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
+    __syncthreads();
+    for (int par = 0; row < P.rows; row += step, par ^= 1) {
+        const float mean = mean_n, rstd = rstd_n;
+        float2 xh[C][4], g[C][4];
+#pragma unroll
+        for (int c = 0; c < C; ++c) { unpack2<T>(rx[c], xh[c]); unpack2<T>(rg[c], g[c]); }
+        load(row + step);
+        float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            if (chunk < n8) {
+                float2 w[4];
+                ld_staged(prm, n8, chunk, w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // (the distance from the mean is taken before the scaling: x * rstd - mean * rstd loses digits of rows far from zero)
+                    xh[c][i] = __fmul2_rn(__fadd2_rn(xh[c][i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                    dw[c][i] = __ffma2_rn(g[c][i], xh[c][i], dw[c][i]);
+                    db[c][i] = __fadd2_rn(db[c][i], g[c][i]);
+                    g[c][i] = __fmul2_rn(g[c][i], w[i]);
+                    a2 = __fadd2_rn(a2, g[c][i]);
+                    b2 = __ffma2_rn(g[c][i], xh[c][i], b2);
+                }
+            }
+        }
+        float s[2] = {a2.x + a2.y, b2.x + b2.y};
+        row_sum<2, WARPS>(s, red[par]);
+        const float m1 = -s[0] * P.inv_h, m2 = -s[1] * P.inv_h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            if (chunk < n8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    g[c][i] = __fmul2_rn(__fadd2_rn(g[c][i], __ffma2_rn(xh[c][i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
+                st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g[c]);
+            }
+        }
+    }
+    if (!P.part) return;
+    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
+    if constexpr (WARPS == 1) {
+        // eight warps hold sums of the same columns
+        float* fold = reinterpret_cast<float*>(prm);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    reinterpret_cast<float2*>(fold)[(threadIdx.x >> 5) * (TPR * 4 * C) + (tid + c * TPR) * 4 + i] = k ? db[c][i] : dw[c][i];
+            __syncthreads();
+            for (int col = threadIdx.x; col < P.H; col += 256) {
+                float a = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) a += fold[r * (TPR * 8 * C) + col];
+                out[(int64_t)k * P.H + col] = a;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            if (chunk < n8) {
+                float4* o = reinterpret_cast<float4*>(out + 8 * chunk);
+                o[0] = make_float4(dw[c][0].x, dw[c][0].y, dw[c][1].x, dw[c][1].y);
+                o[1] = make_float4(dw[c][2].x, dw[c][2].y, dw[c][3].x, dw[c][3].y);
+                o = reinterpret_cast<float4*>(out + P.H + 8 * chunk);
+                o[0] = make_float4(db[c][0].x, db[c][0].y, db[c][1].x, db[c][1].y);
+                o[1] = make_float4(db[c][2].x, db[c][2].y, db[c][3].x, db[c][3].y);
+            }
+        }
+    }
+}
+
+// Rows of any width and alignment, one element per access.
+template <typename T, int C, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
+layer_norm_backward_odd_kernel(const LnParams P) {
+    constexpr int TPR = 32 * WARPS;
+    constexpr int ROWS = WARPS == 1 ? 8 : 1;
+    __shared__ float red[2][2 * WARPS];
+    __shared__ float fold[WARPS == 1 ? 8 * 32 * C : 1];         // one warp per row: the warps' column sums meet here
     pdl_launch_dependents();
     pdl_wait();
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const int64_t step = (int64_t)gridDim.x * ROWS;
-    const T* x = reinterpret_cast<const T*>(P.x);
-    const T* dy = reinterpret_cast<const T*>(P.dy);
-    float dw[C][V], db[C][V];
+    float dw[C], db[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < V; ++i) dw[c][i] = db[c][i] = 0.f;
+    for (int c = 0; c < C; ++c) dw[c] = db[c] = 0.f;
     int par = 0;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0); row < P.rows; row += step, par ^= 1) {
-        const float mean = P.mean[row], rstd = P.rstd[row];
-        float xh[C][V], g[C][V];
+        const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
+        const T* dy = reinterpret_cast<const T*>(P.dy) + row * P.H;
+        const float mean = __ldcg(P.mean + row), rstd = __ldcg(P.rstd + row);
+        float xh[C], g[C];
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (tid + c * TPR) * V;
-            if (col < P.H) {
-                float w[V];
-                unpack<T, V>(ld_raw<T, V>(x + row * P.H + col), xh[c]);
-                unpack<T, V>(ld_raw<T, V>(dy + row * P.H + col), g[c]);
-                ld_param<V>(P.w, P.w_bf16, col, 1.f, w);
+            const int col = tid + c * TPR;
+            float t[1] = {0.f}, u[1] = {0.f};
+            if (col < P.H) { unpack<T, 1>(ld_raw<T, 1>(x + col), t); unpack<T, 1>(ld_raw<T, 1>(dy + col), u); }
+            xh[c] = t[0]; g[c] = u[0];
+        }
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    xh[c][i] = (xh[c][i] - mean) * rstd;
-                    dw[c][i] = fmaf(g[c][i], xh[c][i], dw[c][i]);
-                    db[c][i] += g[c][i];
-                    g[c][i] *= w[i];
-                    s[0] += g[c][i];
-                    s[1] = fmaf(g[c][i], xh[c][i], s[1]);
-                }
+        for (int c = 0; c < C; ++c) {
+            const int col = tid + c * TPR;
+            if (col < P.H) {
+                float w[1];
+                ld_param<1>(P.w, P.w_bf16, col, 1.f, w);
+                xh[c] = (xh[c] - mean) * rstd;
+                dw[c] = fmaf(g[c], xh[c], dw[c]);
+                db[c] += g[c];
+                g[c] *= w[0];
+                s[0] += g[c];
+                s[1] = fmaf(g[c], xh[c], s[1]);
             }
         }
         row_sum<2, WARPS>(s, red[par]);
         const float m1 = s[0] * P.inv_h, m2 = s[1] * P.inv_h;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (tid + c * TPR) * V;
+            const int col = tid + c * TPR;
             if (col < P.H) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[c][i] = (g[c][i] - fmaf(xh[c][i], m2, m1)) * rstd;
-                st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, g[c]);
+                const float o[1] = {(g[c] - fmaf(xh[c], m2, m1)) * rstd};
+                st_row<T, 1>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
             }
         }
     }
@@ -352,24 +589,18 @@ layer_norm_backward_kernel(const LnParams P) {
         if constexpr (WARPS == 1) {
             __syncthreads();
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int i = 0; i < V; ++i) fold[(threadIdx.x >> 5) * (32 * V * C) + (tid + c * 32) * V + i] = k ? db[c][i] : dw[c][i];
+            for (int c = 0; c < C; ++c) fold[(threadIdx.x >> 5) * (32 * C) + tid + c * 32] = k ? db[c] : dw[c];
             __syncthreads();
             for (int col = threadIdx.x; col < P.H; col += 256) {
                 float a = 0.f;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) a += fold[r * (32 * V * C) + col];
+                for (int r = 0; r < 8; ++r) a += fold[r * (32 * C) + col];
                 out[(int64_t)k * P.H + col] = a;
             }
         } else {
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int col = (tid + c * TPR) * V;
-                if (col < P.H)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) out[(int64_t)k * P.H + col + i] = k ? db[c][i] : dw[c][i];
-            }
+            for (int c = 0; c < C; ++c)
+                if (tid + c * TPR < P.H) out[(int64_t)k * P.H + tid + c * TPR] = k ? db[c] : dw[c];
         }
     }
 }

@@ -123,7 +123,7 @@ struct DeviceState {
     size_t ws_bytes = 0;
     std::vector<std::pair<void*, size_t>> ws_all;   // every buffer ever handed out: none is freed, launches and graphs may hold them
     std::map<const void*, bool> smem_attr_set;
-    std::map<const void*, int> ctas_per_sm;
+    std::map<std::pair<const void*, int>, int> ctas_per_sm;
 };
 static std::mutex g_mu;
 static DeviceState g_dev[64];
@@ -274,11 +274,14 @@ static uint32_t fmt_mma_code(int f) {      // operand format field of kind::mxf8
     return f == MXFP6_E2M3 ? kFmtE2M3 : f == MXFP6_E3M2 ? kFmtE3M2 : f == MXFP8_E4M3 ? kFmtE4M3 : f == MXFP8_E5M2 ? kFmtE5M2 : kFmtE2M1;
 }
 
-// CTAs of a kernel (no dynamic shared memory) that one SM holds, asked once per device
-static int resident_ctas(DeviceState& d, const void* kern, int threads, int* out) {
+// CTAs of a kernel that one SM holds, asked once per device and amount of dynamic shared memory; the kernel is then allowed that amount
+static int resident_ctas(DeviceState& d, const void* kern, int threads, int smem, int* out) {
     std::lock_guard<std::mutex> lk(g_mu);
-    int& n = d.ctas_per_sm[kern];
-    if (n == 0) CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0));
+    int& n = d.ctas_per_sm[{kern, smem}];
+    if (n == 0) {
+        if (smem > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+        CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, (size_t)smem));
+    }
     if (n < 1) return fail(MXFP6_ERR_CUDA, "a kernel of %d threads does not fit an SM", threads);
     *out = n;
     return MXFP6_OK;

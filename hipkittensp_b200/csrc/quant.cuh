@@ -62,15 +62,13 @@ __device__ __forceinline__ uint32_t cvt_quad(float x0, float x1, float x2, float
     return mad_u32(hi12, 4096u, lo12);
 }
 
-// E8M0 byte of a block whose largest magnitude is amax
+// E8M0 byte of a block whose largest magnitude is amax: the exponent field of amax less the format's own exponent range.
+// A zero or subnormal amax lies below every format's smallest scale (field 0: byte 0); an infinite one gets the largest byte.
 __device__ __forceinline__ int quant_scale_byte(float amax, int fmt) {
-    const uint32_t u = __float_as_uint(amax);
-    int fl = (int)((u >> 23) & 0xff) - 127;
-    if (((u >> 23) & 0xff) == 0) fl = 31 - __clz(u & 0x7fffff) - 149;     // fp32 subnormal
-    int sb = fl - quant_emax(fmt) + 127;
-    sb = sb < 0 ? 0 : sb > 254 ? 254 : sb;
-    if (!(amax > 0.f)) sb = 0;
-    if (isinf(amax)) sb = 254;
+    const int field = (int)(__float_as_uint(amax) >> 23);
+    int sb = field - quant_emax(fmt);
+    sb = sb < 0 ? 0 : sb;
+    if (field >= 255) sb = isinf(amax) ? 254 : 0;
     return sb;
 }
 
