@@ -12,16 +12,16 @@ struct LnChoice {
 };
 
 // Whole 8-element chunks: a thread holds up to four, sixteen warps a row: 16384 elements.
-template <typename T, int BITS>
+template <typename T, int FMT>
 static LnChoice ln_forward_vec(int H) {
     const int smem = 8 * H;          // w and b as fp32
-    if (H <= 256) return {layer_norm_kernel<T, 1, 1, BITS>, 1, smem};
-    if (H <= 1024) return {layer_norm_kernel<T, 4, 1, BITS>, 1, smem};
-    if (H <= 2048) return {layer_norm_kernel<T, 4, 2, BITS>, 2, smem};
-    if (H <= 4096) return {layer_norm_kernel<T, 4, 4, BITS>, 4, smem};
-    if (H <= 8192) return {layer_norm_kernel<T, 4, 8, BITS>, 8, smem};
-    if (H <= 16384) return {layer_norm_kernel<T, 4, 16, BITS>, 16, smem};
-    return {layer_norm_long_kernel<T, 8, BITS>, 0, 0};
+    if (H <= 256) return {layer_norm_kernel<T, 1, 1, FMT>, 1, smem};
+    if (H <= 1024) return {layer_norm_kernel<T, 4, 1, FMT>, 1, smem};
+    if (H <= 2048) return {layer_norm_kernel<T, 4, 2, FMT>, 2, smem};
+    if (H <= 4096) return {layer_norm_kernel<T, 4, 4, FMT>, 4, smem};
+    if (H <= 8192) return {layer_norm_kernel<T, 4, 8, FMT>, 8, smem};
+    if (H <= 16384) return {layer_norm_kernel<T, 4, 16, FMT>, 16, smem};
+    return {layer_norm_long_kernel<T, 8, FMT>, 0, 0};
 }
 template <typename T>
 static LnChoice ln_forward_odd(int H) {
@@ -32,13 +32,20 @@ static LnChoice ln_forward_odd(int H) {
     if (H <= 4096) return {layer_norm_odd_kernel<T, 8, 16>, 16, 0};
     if (H <= 8192) return {layer_norm_odd_kernel<T, 16, 16>, 16, 0};
     if (H <= 16384) return {layer_norm_odd_kernel<T, 32, 16>, 16, 0};
-    return {layer_norm_long_kernel<T, 1, 0>, 0, 0};
+    return {layer_norm_long_kernel<T, 1, -1>, 0, 0};
 }
-// bits: element width of an MX result, 0 for one in x's type
+// fmt: format of an MX result, negative for one in x's type
 template <typename T>
-static LnChoice ln_forward_kernel(bool vec, int bits, int H) {
+static LnChoice ln_forward_kernel(bool vec, int fmt, int H) {
     if (!vec) return ln_forward_odd<T>(H);
-    return bits == 0 ? ln_forward_vec<T, 0>(H) : bits == 4 ? ln_forward_vec<T, 4>(H) : bits == 6 ? ln_forward_vec<T, 6>(H) : ln_forward_vec<T, 8>(H);
+    switch (fmt) {
+        case MXFP6_E2M3: return ln_forward_vec<T, MXFP6_E2M3>(H);
+        case MXFP6_E3M2: return ln_forward_vec<T, MXFP6_E3M2>(H);
+        case MXFP8_E4M3: return ln_forward_vec<T, MXFP8_E4M3>(H);
+        case MXFP8_E5M2: return ln_forward_vec<T, MXFP8_E5M2>(H);
+        case MXFP4_E2M1: return ln_forward_vec<T, MXFP4_E2M1>(H);
+        default: return ln_forward_vec<T, -1>(H);
+    }
 }
 
 // Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row.
@@ -111,8 +118,7 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
         return fail(MXFP6_ERR_BAD_ARG, "%s: x must be 32-byte (fp32) or 16-byte (bf16) aligned, weight, bias and codes 16-byte", what);
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
-    const int bits = mx ? fmt_block_bytes(fmt) / 4 : 0;
-    const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(vec, bits, (int)H) : ln_forward_kernel<__nv_bfloat16>(vec, bits, (int)H);
+    const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(vec, fmt, (int)H) : ln_forward_kernel<__nv_bfloat16>(vec, fmt, (int)H);
     const int threads = k.warps == 0 ? 1024 : k.warps == 1 ? 256 : 32 * k.warps;
     int per_sm = 0;
     if ((rc = resident_ctas(*d, (const void*)k.kern, threads, k.smem, &per_sm))) return rc;
@@ -120,7 +126,7 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
     LnParams P{};
     P.x = x; P.y = y; P.w = w; P.b = b; P.w_bf16 = w_dtype;
     P.mean = mean; P.rstd = rstd;
-    P.q_out = (uint8_t*)packed; P.q_scales = (uint8_t*)scales; P.q_fmt = fmt;
+    P.q_out = (uint8_t*)packed; P.q_scales = (uint8_t*)scales;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H; P.eps = eps;
     return launch_pdl(k.kern, (unsigned)(want < cap ? want : cap), (unsigned)threads, (size_t)k.smem, (cudaStream_t)stream, P);
 }

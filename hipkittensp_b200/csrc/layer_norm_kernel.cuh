@@ -32,7 +32,6 @@ struct LnParams {
     float* part;             // backward: [grid][2][H] partial sums of dw and db, or null when they are not wanted
     uint8_t* q_out;          // forward to an MX operand: codes [rows, H * bits / 8] ...
     uint8_t* q_scales;       // ... and scales [rows, H / 32]
-    int q_fmt;
     int64_t rows;
     int H;
     float inv_h, eps;
@@ -140,13 +139,13 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
     }
 }
 
-// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes of BITS bits and scale.
-template <int BITS>
-__device__ __forceinline__ void mx_store8(const float2 (&v)[4], int fmt, uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
+// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes and scale.
+template <int FMT>
+__device__ __forceinline__ void mx_store8(const float2 (&v)[4], uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
     float amax = amax3(amax3(v[0].x, v[0].y, v[1].x), amax3(v[1].y, v[2].x, v[2].y), fmaxf(fabsf(v[3].x), fabsf(v[3].y)));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int sb = quant_scale_byte(amax, fmt);
+    const int sb = quant_scale_byte(amax, FMT);
     const float f = quant_inv_scale(sb);
     float s[8];
 #pragma unroll
@@ -155,18 +154,14 @@ __device__ __forceinline__ void mx_store8(const float2 (&v)[4], int fmt, uint8_t
         s[2 * i] = t.x; s[2 * i + 1] = t.y;
     }
     const int j = (col >> 3) & 3;                   // place of these eight in their block
-    if constexpr (BITS == 4) {
+    if constexpr (FMT == kE2M1) {
         const uint32_t w = cvt_oct_e2m1(s);
         if (live) *reinterpret_cast<uint32_t*>(codes_row + col / 2) = w;
-    } else if constexpr (BITS == 8) {
-        uint2 w;
-        if (fmt == kE4M3) w = make_uint2(cvt_quad<kE4M3>(s[0], s[1], s[2], s[3]), cvt_quad<kE4M3>(s[4], s[5], s[6], s[7]));
-        else w = make_uint2(cvt_quad<kE5M2>(s[0], s[1], s[2], s[3]), cvt_quad<kE5M2>(s[4], s[5], s[6], s[7]));
+    } else if constexpr (fmt_fp8(FMT)) {
+        const uint2 w = make_uint2(cvt_quad<FMT>(s[0], s[1], s[2], s[3]), cvt_quad<FMT>(s[4], s[5], s[6], s[7]));
         if (live) *reinterpret_cast<uint2*>(codes_row + col) = w;
     } else {
-        uint32_t lo, hi;                            // 24 bits each
-        if (fmt == kE2M3) { lo = cvt_quad<kE2M3>(s[0], s[1], s[2], s[3]); hi = cvt_quad<kE2M3>(s[4], s[5], s[6], s[7]); }
-        else { lo = cvt_quad<kE3M2>(s[0], s[1], s[2], s[3]); hi = cvt_quad<kE3M2>(s[4], s[5], s[6], s[7]); }
+        const uint32_t lo = cvt_quad<FMT>(s[0], s[1], s[2], s[3]), hi = cvt_quad<FMT>(s[4], s[5], s[6], s[7]);      // 24 bits each
         // 48 bits a lane: four lanes hold 24 bytes, which three of them write, 8 each: lane j the bits from 64 j on, which start at
         // bit 16 j of its own 48 and run on into its neighbour's
         const uint32_t w0 = lo | (hi << 24), w1 = hi >> 8;
@@ -209,12 +204,13 @@ __device__ __forceinline__ void st_row2(T* p, const float2 (&v)[4]) {
 }
 
 // ---------------------------------------------------------------------------------- forward
-// WARPS warps own a row, C chunks of 8 elements per thread.  WARPS = 1: eight warps per CTA with a row each.  BITS = 0: the result is
-// written in x's type; 4, 6, 8: it leaves as codes and scales.  The next row is on its way in registers while this one is worked
+// WARPS warps own a row, C chunks of 8 elements per thread.  WARPS = 1: eight warps per CTA with a row each.  FMT < 0: the result is
+// written in x's type; otherwise it leaves as codes and scales.  The next row is on its way in registers while this one is worked
 // on, the arithmetic runs on pairs (fma.f32x2), and the parameters are staged once per CTA: bf16 rows are bound by issue, not by
-// HBM, when each element costs 25 instructions (16384 x 8192 in 124 us).
-template <typename T, int C, int WARPS, int BITS>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 16 ? 1 : WARPS == 1 ? 2 : 16 / WARPS)
+// HBM, when each element costs 25 instructions (16384 x 8192 in 124 us).  Threads whose columns lie past H take part in everything
+// but the stores, on zeros: a branch per chunk would keep the chunks' instructions from being interleaved.
+template <typename T, int C, int WARPS, int FMT>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 16 ? 1 : (sizeof(T) == 2 ? 24 : 16) / (WARPS == 1 ? 8 : WARPS))
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     constexpr int ROWS = WARPS == 1 ? 8 : 1;                    // rows a CTA works on at a time
@@ -257,13 +253,12 @@ layer_norm_kernel(const LnParams P) {
         float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            if (tid + c * TPR < n8) {
+            const float m = tid + c * TPR < n8 ? -mean0 : 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[c][i] = __fadd2_rn(v[c][i], make_float2(-mean0, -mean0));
-                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
-                    d2 = __fadd2_rn(d2, v[c][i]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                v[c][i] = __fadd2_rn(v[c][i], make_float2(m, m));
+                q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                d2 = __fadd2_rn(d2, v[c][i]);
             }
         }
         float q[2] = {q2.x + q2.y, d2.x + d2.y};
@@ -279,23 +274,16 @@ layer_norm_kernel(const LnParams P) {
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
             const bool live = chunk < n8;
-            float2 o[4];
-            if (live) {
-                float2 w[4], b[4];
-                ld_staged(prm, n8, chunk, w);
-                ld_staged(prm + 2 * n8, n8, chunk, b);
+            float2 o[4], w[4], b[4];
+            ld_staged(prm, n8, live ? chunk : 0, w);
+            ld_staged(prm + 2 * n8, n8, live ? chunk : 0, b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    o[i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
-            }
-            if constexpr (BITS) {
-                if (!live)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = make_float2(0.f, 0.f);
-                mx_store8<BITS>(o, P.q_fmt, P.q_out + row * (P.H / 32) * (4 * BITS), P.q_scales + row * (P.H / 32), 8 * chunk, live);
-            } else if (live) {
+            for (int i = 0; i < 4; ++i)
+                o[i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
+            if constexpr (FMT >= 0)
+                mx_store8<FMT>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, live);
+            else if (live)
                 st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, o);
-            }
         }
     }
 }
@@ -353,7 +341,7 @@ layer_norm_odd_kernel(const LnParams P) {
 
 // Rows longer than the registers of a CTA hold: a CTA of 1024 threads passes over its row three times (the second and third
 // pass find it in L2).
-template <typename T, int V, int BITS>
+template <typename T, int V, int FMT>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P) {
     __shared__ float red[32], red2[64];
     pdl_launch_dependents();
@@ -397,9 +385,9 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[i] = fmaf(fmaf(v[i] - mean0, rstd, shift), w[i], b[i]);
             }
-            if constexpr (BITS) {
+            if constexpr (FMT >= 0) {
                 const float2 o[4] = {make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]), make_float2(v[6], v[7])};
-                mx_store8<BITS>(o, P.q_fmt, P.q_out + row * (P.H / 32) * (4 * BITS), P.q_scales + row * (P.H / 32), col, live);
+                mx_store8<FMT>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), col, live);
             } else if (live) {
                 st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, v);
             }
@@ -461,20 +449,19 @@ layer_norm_backward_kernel(const LnParams P) {
         float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            // (threads past H: dy is zero there, and so is all that is summed)
             const int chunk = tid + c * TPR;
-            if (chunk < n8) {
-                float2 w[4];
-                ld_staged(prm, n8, chunk, w);
+            float2 w[4];
+            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // (the distance from the mean is taken before the scaling: x * rstd - mean * rstd loses digits of rows far from zero)
-                    xh[c][i] = __fmul2_rn(__fadd2_rn(xh[c][i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
-                    dw[c][i] = __ffma2_rn(g[c][i], xh[c][i], dw[c][i]);
-                    db[c][i] = __fadd2_rn(db[c][i], g[c][i]);
-                    g[c][i] = __fmul2_rn(g[c][i], w[i]);
-                    a2 = __fadd2_rn(a2, g[c][i]);
-                    b2 = __ffma2_rn(g[c][i], xh[c][i], b2);
-                }
+            for (int i = 0; i < 4; ++i) {
+                // (the distance from the mean is taken before the scaling: x * rstd - mean * rstd loses digits of rows far from zero)
+                xh[c][i] = __fmul2_rn(__fadd2_rn(xh[c][i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                dw[c][i] = __ffma2_rn(g[c][i], xh[c][i], dw[c][i]);
+                db[c][i] = __fadd2_rn(db[c][i], g[c][i]);
+                g[c][i] = __fmul2_rn(g[c][i], w[i]);
+                a2 = __fadd2_rn(a2, g[c][i]);
+                b2 = __ffma2_rn(g[c][i], xh[c][i], b2);
             }
         }
         float s[2] = {a2.x + a2.y, b2.x + b2.y};
@@ -483,12 +470,10 @@ layer_norm_backward_kernel(const LnParams P) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
-            if (chunk < n8) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    g[c][i] = __fmul2_rn(__fadd2_rn(g[c][i], __ffma2_rn(xh[c][i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
-                st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g[c]);
-            }
+            for (int i = 0; i < 4; ++i)
+                g[c][i] = __fmul2_rn(__fadd2_rn(g[c][i], __ffma2_rn(xh[c][i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
+            if (chunk < n8) st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g[c]);
         }
     }
     if (!P.part) return;
