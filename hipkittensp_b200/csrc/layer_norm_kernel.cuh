@@ -210,7 +210,7 @@ __device__ __forceinline__ void st_row2(T* p, const float2 (&v)[4]) {
 // HBM, when each element costs 25 instructions (16384 x 8192 in 124 us).  Threads whose columns lie past H take part in everything
 // but the stores, on zeros: a branch per chunk would keep the chunks' instructions from being interleaved.
 template <typename T, int C, int WARPS, int FMT>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 16 ? 1 : (sizeof(T) == 2 ? 24 : 16) / (WARPS == 1 ? 8 : WARPS))
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 : 16 / WARPS)
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     constexpr int ROWS = WARPS == 1 ? 8 : 1;                    // rows a CTA works on at a time

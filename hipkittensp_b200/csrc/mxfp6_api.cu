@@ -51,7 +51,7 @@ struct Options {
     int no_sf_tma = 0;       // MXFP6_NO_SF_TMA: scale arrays read with plain loads
     int pdl = 1;             // MXFP6_PDL: programmatic dependent launch
     int group_p = 16;        // MXFP6_GROUP_P: pair tiles per rasterisation group
-    int quant_quad = 0;      // MXFP6_QUANT_PATH=quad: the plain-load quantiser
+    int quant_quad = 0;      // MXFP6_QUANT_PATH=quad: the plain-load quantiser and dequantiser
     int wait_ms = 2000;      // MXFP6_WAIT_MS: budget of one bounded wait (read when a device is first used)
     // MXFP6_L2 = "load,store": L2 eviction policy of the pair kernel's TMA traffic (0 normal, 1 evict_first, 2 evict_last).
     // Operand tiles are asked for again by other pairs and C is written once: keeping the former and letting the latter
@@ -1191,7 +1191,20 @@ extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int6
 }
 
 template <int F, typename T>
-static int launch_dequantize(const DeviceState& d, const uint8_t* packed, const uint8_t* scales, int64_t n_oct, T* out, cudaStream_t st) {
+static int launch_dequantize(DeviceState& d, const uint8_t* packed, const uint8_t* scales, int64_t n_oct, T* out, cudaStream_t st) {
+    const int64_t n_blocks = n_oct / 4;
+    // bulk copies of whole 16-byte pieces, block numbers that fit a tensor map's coordinate
+    if (!((uintptr_t)packed & 15) && !((uintptr_t)scales & 15) && n_blocks < 0x7fffff00LL && !options().quant_quad) {
+        using Cfg = DequantCfg<F, T>;
+        auto kern = dequantize_tma_kernel<F, T>;
+        CUtensorMap tm;
+        int rc = make_map(out, n_blocks, 32, Cfg::TILE, sizeof(T) == 4 ? 4 : 5, &tm);
+        if (!rc) rc = ensure_smem_attr(d, (const void*)kern, Cfg::SMEM_ALLOC);
+        if (rc) return rc;
+        const int64_t want = (n_blocks + Cfg::TILE * Cfg::WARPS - 1) / (Cfg::TILE * Cfg::WARPS), cap = (int64_t)d.sm_count * Cfg::CTAS_PER_SM;
+        return launch_pdl(kern, (unsigned)(want < cap ? want : cap), 32 * Cfg::WARPS, Cfg::SMEM_ALLOC, st, tm, packed, scales, (long long)n_blocks,
+                          d.status, d.wait_cycles);
+    }
     // four octets per thread; the grid covers the device eight times over at most
     int64_t blocks = (n_oct + 4 * 256 - 1) / (4 * 256);
     if (blocks > (int64_t)d.sm_count * 8) blocks = (int64_t)d.sm_count * 8;

@@ -49,6 +49,11 @@ __device__ __forceinline__ void bulk_store_1d(void* dst_global, uint32_t src_sme
                  ::"l"(dst_global), "r"(src_smem), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void bulk_load_1d(uint32_t dst_smem, const void* src_global, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst_smem), "l"(src_global), "r"(bytes), "r"(bar) : "memory");
+}
+
 __device__ __forceinline__ bool quant_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
                                            unsigned long long wait_cycles, int code) {
     if (mbar_try_wait(bar, parity)) return true;

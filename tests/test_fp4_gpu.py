@@ -61,16 +61,16 @@ def test_quantize_edge_values(path):
 
 
 @pytest.mark.parametrize("fmt", [R.E2M3, R.E3M2, R.E4M3, R.E5M2, R.E2M1])
-@pytest.mark.parametrize("shift", [0, 1])
-def test_dequantize_all_codes_and_scales(fmt, shift):
-    """Every code under scales over the whole range, to fp32 and bf16, from operands that start on an odd byte too."""
+@pytest.mark.parametrize("rows,K,shift", [(40, 544, 0), (40, 544, 1), (1, 32, 0), (3, 32, 0), (1, 1056, 0), (700, 2048, 0), (700, 2048, 16)])
+def test_dequantize_all_codes_and_scales(fmt, rows, K, shift):
+    """Every code under scales over the whole range, to fp32 and bf16; block counts around a warp's tile of 32 and past a ring's
+    length; operands that start on an odd byte too."""
     rng = np.random.default_rng(fmt)
-    rows, K = 40, 544
     packed = rng.integers(0, 256, size=(rows, R._FMT[fmt]["bits"] * K // 8), dtype=np.uint8)
     scales = rng.integers(1, 255, size=(rows, K // 32), dtype=np.uint8)
-    scales[0, :3] = [0, 254, 127]
+    scales.reshape(-1)[:min(3, scales.size)] = [0, 254, 127][:min(3, scales.size)]
     want = torch.from_numpy(R.dequantize(packed, scales, fmt))
-    buf = torch.zeros(packed.size + 1, dtype=torch.uint8, device="cuda")
+    buf = torch.zeros(packed.size + 16, dtype=torch.uint8, device="cuda")
     dev = buf[shift:shift + packed.size].view(rows, -1)
     dev.copy_(torch.from_numpy(packed))
     for dtype in (torch.float32, torch.bfloat16):
