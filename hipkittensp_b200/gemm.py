@@ -19,7 +19,7 @@ def _accept(t, name: str, dtype) -> None:
         raise RuntimeError("Expected a torch.Tensor")
     if not t.is_contiguous():
         raise RuntimeError("Tensor must be contiguous")
-    if t.device.type == "cpu":
+    if not t.is_cuda:
         raise RuntimeError("Tensor must be on CUDA device")
     if t.dim() > 4:
         raise RuntimeError("Expected Tensor.ndim <= 4")
@@ -46,31 +46,26 @@ def row_bytes(K: int, fmt: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream_ptr() -> int:
     """Handle of torch's current stream on the current device."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def _on_device_of(t):
-    """Context that makes t's device current; free when it already is (the common case)."""
-    if t.device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(t.device)
+def _launch(t, entry, *args) -> None:
+    """entry(*args, stream) on torch's current stream of t's device, with that device current; raises on an error code."""
+    device = t.get_device()
+    if device == _current_device():
+        rc = entry(*args, _stream_ptr())
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, _stream_ptr())
+    if rc:
+        check(rc)
 
 
 def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None = None, b_static: bool = False) -> None:
@@ -97,11 +92,11 @@ def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None
         raise RuntimeError("B must be [N, 3K/4] (fp6), [N, K] (fp8) or [N, K/2] (fp4) with the K of A")
     if tuple(scale_A.shape) != (M, K // 32) or tuple(scale_B.shape) != (N, K // 32):
         raise RuntimeError("scales must be [rows, K/32]")
-    if len({t.device for t in (A, B, C, scale_A, scale_B)}) != 1:
+    device = A.get_device()
+    if B.get_device() != device or C.get_device() != device or scale_A.get_device() != device or scale_B.get_device() != device:
         raise RuntimeError("all tensors must be on the same device")
-    with _on_device_of(A):
-        check(lib.mxfp6_gemm_ex(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), C.data_ptr(),
-                                M, N, K, fmt, fb, _lib.FLAG_B_STATIC if b_static else 0, _stream_ptr()))
+    _launch(A, lib.mxfp6_gemm_ex, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), C.data_ptr(),
+            M, N, K, fmt, fb, _lib.FLAG_B_STATIC if b_static else 0)
 
 
 def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2M3) -> None:
@@ -117,6 +112,9 @@ def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2
     _accept(scale_B, "scale_B", torch.uint8)
     M, N = A.shape[0], B.shape[0]
     K = _k_of(A, fmt, "A")
+    if _k_of(B, fmt, "B") != K:
+        raise RuntimeError("A and B disagree on K")
+    _check_scales(A, B, scale_A, scale_B, K)
     if not 1 <= len(dests) <= 8:
         raise RuntimeError("1 to 8 destinations")
     ldc = dests[0].stride(0)
@@ -126,9 +124,16 @@ def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2
         if col_offset < 0 or col_offset + N > d.shape[1]:
             raise RuntimeError("column window outside the destination")
     ptrs = (ctypes.c_void_p * len(dests))(*[d.data_ptr() + 2 * col_offset for d in dests])
-    with _on_device_of(A):
-        check(lib.mxfp6_gemm_multi(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
-                                   ldc, M, N, K, fmt, fmt, _stream_ptr()))
+    _launch(A, lib.mxfp6_gemm_multi, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
+            ldc, M, N, K, fmt, fmt)
+
+
+def _check_scales(A, B, scale_A, scale_B, K: int) -> None:
+    if K % 32 or tuple(scale_A.shape) != (A.shape[0], K // 32) or tuple(scale_B.shape) != (B.shape[0], K // 32):
+        raise RuntimeError("scales must be [rows, K/32]")
+    device = A.get_device()
+    if B.get_device() != device or scale_A.get_device() != device or scale_B.get_device() != device:
+        raise RuntimeError("all tensors must be on the same device")
 
 
 def copy_gather_scratch_bytes(M: int, N: int, strip_tiles: int) -> int:
@@ -149,6 +154,9 @@ def dispatch_copy_gather(A, B, dests, col_offset: int, scale_A, scale_B, scratch
     _accept(scale_B, "scale_B", torch.uint8)
     M, N = A.shape[0], B.shape[0]
     K = _k_of(A, fmt, "A")
+    if _k_of(B, fmt, "B") != K:
+        raise RuntimeError("A and B disagree on K")
+    _check_scales(A, B, scale_A, scale_B, K)
     if not 1 <= len(dests) <= 8:
         raise RuntimeError("1 to 8 destinations")
     ldc = dests[0].stride(0)
@@ -161,10 +169,9 @@ def dispatch_copy_gather(A, B, dests, col_offset: int, scale_A, scale_B, scratch
         raise RuntimeError("scratch must be a contiguous tensor on the operands' device")
     ptrs = (ctypes.c_void_p * len(dests))(*[d.data_ptr() + 2 * col_offset for d in dests])
     streams = (ctypes.c_void_p * max(len(copy_streams), 1))(*[s.cuda_stream for s in copy_streams])
-    with _on_device_of(A):
-        check(lib.mxfp6_gemm_copy_gather(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
-                                         ldc, M, N, K, fmt, fmt, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
-                                         strip_tiles, streams, len(copy_streams), _stream_ptr()))
+    _launch(A, lib.mxfp6_gemm_copy_gather, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
+            ldc, M, N, K, fmt, fmt, scratch.data_ptr(), scratch.numel() * scratch.element_size(),
+            strip_tiles, streams, len(copy_streams))
 
 
 def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out_fmt: int = E2M3):
@@ -178,13 +185,13 @@ def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = No
     M, N, K = A.shape[0], B.shape[0], _k_of(A, fmt, "A")
     if _k_of(B, fb, "B") != K:
         raise RuntimeError("A and B disagree on K")
+    _check_scales(A, B, scale_A, scale_B, K)
     if N % 64:
         raise RuntimeError("N must be a multiple of 64")
-    out = torch.empty((M, row_bytes(N, out_fmt)), dtype=torch.uint8, device=A.device)
-    scales = torch.empty((M, N // 32), dtype=torch.uint8, device=A.device)
-    with _on_device_of(A):
-        check(lib.mxfp6_gemm_requant(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
-                                     scales.data_ptr(), M, N, K, fmt, fb, out_fmt, _stream_ptr()))
+    out = A.new_empty((M, row_bytes(N, out_fmt)))
+    scales = A.new_empty((M, N // 32))
+    _launch(A, lib.mxfp6_gemm_requant, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
+            scales.data_ptr(), M, N, K, fmt, fb, out_fmt)
     return out, scales
 
 
@@ -201,6 +208,7 @@ def gemm_scaled(A, scale_A, B, scale_B, row_scale=None, col_scale=None, bias=Non
     M, N, K = A.shape[0], B.shape[0], _k_of(A, fmt, "A")
     if _k_of(B, fb, "B") != K:
         raise RuntimeError("A and B disagree on K")
+    _check_scales(A, B, scale_A, scale_B, K)
     for name, v, n in (("row_scale", row_scale, M), ("col_scale", col_scale, N), ("bias", bias, N)):
         if v is not None:
             if not isinstance(v, torch.Tensor) or v.dtype != torch.float32 or not v.is_contiguous():
@@ -210,14 +218,15 @@ def gemm_scaled(A, scale_A, B, scale_B, row_scale=None, col_scale=None, bias=Non
             if v.numel() != n:
                 raise RuntimeError(f"{name} must have {n} elements, has {v.numel()}")
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+        out = A.new_empty((M, N), dtype=torch.bfloat16)
     _accept(out, "C", torch.bfloat16)
     if tuple(out.shape) != (M, N):
         raise RuntimeError(f"C must be [{M}, {N}]")
+    if out.get_device() != A.get_device():
+        raise RuntimeError("all tensors must be on the same device")
     ptr = lambda v: 0 if v is None else v.data_ptr()
-    with _on_device_of(A):
-        check(lib.mxfp6_gemm_scaled(A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
-                                    ptr(row_scale), ptr(col_scale), ptr(bias), M, N, K, fmt, fb, _stream_ptr()))
+    _launch(A, lib.mxfp6_gemm_scaled, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
+            ptr(row_scale), ptr(col_scale), ptr(bias), M, N, K, fmt, fb)
     return out
 
 
@@ -225,7 +234,7 @@ def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=
     """Allocating convenience wrapper around dispatch_micro; returns C."""
     M, N = A.shape[0], B.shape[0]
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=A.device)
+        out = A.new_empty((M, N), dtype=torch.bfloat16)
     dispatch_micro(A, B, out, scale_A, scale_B, fmt, fmt_b)
     return out
 
@@ -233,18 +242,17 @@ def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=
 def quantize(x: torch.Tensor, fmt: int = E2M3):
     """fp32 or bf16 [rows,K] on the GPU -> (operand bytes u8 [rows,3K/4] for fp6 / [rows,K] for fp8 / [rows,K/2] for fp4,
     scales u8 [rows,K/32])."""
-    if x.device.type == "cpu":
+    if not x.is_cuda:
         raise RuntimeError("Tensor must be on CUDA device")
     if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() != 2 or not x.is_contiguous():
         raise RuntimeError("quantize expects a contiguous 2-D fp32 or bf16 tensor")
     rows, K = x.shape
     if K % 32:
         raise RuntimeError("K must be a multiple of 32")
-    packed = torch.empty((rows, row_bytes(K, fmt)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, K // 32), dtype=torch.uint8, device=x.device)
-    with _on_device_of(x):
-        check(lib.mxfp6_quantize(x.data_ptr(), 0 if x.dtype == torch.float32 else 1, rows, K, fmt,
-                                 packed.data_ptr(), scales.data_ptr(), _stream_ptr()))
+    packed = x.new_empty((rows, row_bytes(K, fmt)), dtype=torch.uint8)
+    scales = x.new_empty((rows, K // 32), dtype=torch.uint8)
+    _launch(x, lib.mxfp6_quantize, x.data_ptr(), 0 if x.dtype == torch.float32 else 1, rows, K, fmt,
+            packed.data_ptr(), scales.data_ptr())
     return packed, scales
 
 
@@ -257,12 +265,11 @@ def dequantize(packed: torch.Tensor, scales: torch.Tensor, fmt: int = E2M3, dtyp
         raise RuntimeError("dtype must be torch.float32 or torch.bfloat16")
     if K % 32 or tuple(scales.shape) != (rows, K // 32):
         raise RuntimeError("scales must be [rows, K/32]")
-    if scales.device != packed.device:
+    if scales.get_device() != packed.get_device():
         raise RuntimeError("all tensors must be on the same device")
-    out = torch.empty((rows, K), dtype=dtype, device=packed.device)
-    with _on_device_of(packed):
-        check(lib.mxfp6_dequantize_ex(packed.data_ptr(), scales.data_ptr(), rows, K, fmt, out.data_ptr(),
-                                      0 if dtype == torch.float32 else 1, _stream_ptr()))
+    out = packed.new_empty((rows, K), dtype=dtype)
+    _launch(packed, lib.mxfp6_dequantize_ex, packed.data_ptr(), scales.data_ptr(), rows, K, fmt, out.data_ptr(),
+            0 if dtype == torch.float32 else 1)
     return out
 
 
@@ -279,6 +286,5 @@ def tma_dump(packed: torch.Tensor, row0: int = 0, k0: int = 0) -> torch.Tensor:
     """Diagnostic: the 16 KiB shared-memory image of one 128x128 operand box as the GEMM loads it."""
     rows, K = packed.shape[0], packed.shape[1] // 3 * 4
     out = torch.empty(16384, dtype=torch.uint8, device=packed.device)
-    with _on_device_of(packed):
-        check(lib.mxfp6_debug_tma_dump(packed.data_ptr(), rows, K, row0, k0, out.data_ptr(), _stream_ptr()))
+    _launch(packed, lib.mxfp6_debug_tma_dump, packed.data_ptr(), rows, K, row0, k0, out.data_ptr())
     return out

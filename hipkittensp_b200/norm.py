@@ -6,8 +6,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import E2M3, check, lib
-from .gemm import _on_device_of, _stream_ptr, row_bytes
+from ._lib import E2M3, lib
+from .gemm import _launch, row_bytes
 
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -33,7 +33,7 @@ def _vector(t, name: str, n: int, like, dtype=None) -> int:
         raise RuntimeError("Expected a torch.Tensor")
     if not t.is_contiguous():
         raise RuntimeError("Tensor must be contiguous")
-    if t.device != like.device:
+    if not t.is_cuda or t.get_device() != like.get_device():
         raise RuntimeError("all tensors must be on the same device")
     if t.dtype not in (_DTYPE if dtype is None else (dtype,)):
         raise RuntimeError(f"{name} must be {'fp32 or bf16' if dtype is None else dtype}")
@@ -63,13 +63,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
         out = torch.empty_like(x)
     else:
         _rows_matrix(out, "out")
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != x.get_device():
             raise RuntimeError("out must have the shape, dtype and device of x")
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    with _on_device_of(x):
-        check(lib.mxfp6_layer_norm(x.data_ptr(), _DTYPE[x.dtype], w, b, wd, out.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-                                   rows, H, eps, _stream_ptr()))
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _launch(x, lib.mxfp6_layer_norm, x.data_ptr(), _DTYPE[x.dtype], w, b, wd, out.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+            rows, H, eps)
     return out, mean, rstd
 
 
@@ -81,14 +80,21 @@ def layer_norm_quantize(x, weight=None, bias=None, eps: float = 1e-5, fmt: int =
     if H % 32:
         raise RuntimeError("H must be a multiple of 32")
     w, b, wd = _parameters(x, weight, bias)
-    packed = torch.empty((rows, row_bytes(H, fmt)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, H // 32), dtype=torch.uint8, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    with _on_device_of(x):
-        check(lib.mxfp6_layer_norm_quantize(x.data_ptr(), _DTYPE[x.dtype], w, b, wd, fmt, packed.data_ptr(), scales.data_ptr(),
-                                            mean.data_ptr(), rstd.data_ptr(), rows, H, eps, _stream_ptr()))
+    packed = x.new_empty((rows, row_bytes(H, fmt)), dtype=torch.uint8)
+    scales = x.new_empty((rows, H // 32), dtype=torch.uint8)
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _launch(x, lib.mxfp6_layer_norm_quantize, x.data_ptr(), _DTYPE[x.dtype], w, b, wd, fmt, packed.data_ptr(), scales.data_ptr(),
+            mean.data_ptr(), rstd.data_ptr(), rows, H, eps)
     return packed, scales, mean, rstd
+
+
+def _backward(dy, x, m, r, w, wd, dx, dweight, dbias, stream) -> int:
+    rows, H = x.shape
+    nbytes = lib.mxfp6_layer_norm_backward_workspace_bytes(rows, H)
+    work = x.new_empty(nbytes, dtype=torch.uint8)
+    return lib.mxfp6_layer_norm_backward(dy.data_ptr(), x.data_ptr(), _DTYPE[x.dtype], m, r, w, wd, dx.data_ptr(), dweight.data_ptr(),
+                                         dbias.data_ptr(), rows, H, work.data_ptr(), nbytes, stream)
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None):
@@ -97,7 +103,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     Returns (dx, dweight, dbias): dx in x's type, the sums over the rows in fp32 [H] whatever weight's type."""
     _rows_matrix(x, "x")
     _rows_matrix(dy, "dy")
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.get_device() != x.get_device():
         raise RuntimeError("dy must have the shape, dtype and device of x")
     rows, H = x.shape
     if mean is None or rstd is None:
@@ -105,11 +111,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     m, r = _vector(mean, "mean", rows, x, torch.float32), _vector(rstd, "rstd", rows, x, torch.float32)
     w, _, wd = _parameters(x, weight, None)
     dx = torch.empty_like(x)
-    grads = torch.empty((2, H), dtype=torch.float32, device=x.device)
-    dweight, dbias = grads.unbind(0)
-    with _on_device_of(x):
-        nbytes = lib.mxfp6_layer_norm_backward_workspace_bytes(rows, H)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib.mxfp6_layer_norm_backward(dy.data_ptr(), x.data_ptr(), _DTYPE[x.dtype], m, r, w, wd, dx.data_ptr(),
-                                            dweight.data_ptr(), dbias.data_ptr(), rows, H, work.data_ptr(), nbytes, _stream_ptr()))
+    dweight = x.new_empty(H, dtype=torch.float32)
+    dbias = torch.empty_like(dweight)
+    _launch(x, _backward, dy, x, m, r, w, wd, dx, dweight, dbias)
     return dx, dweight, dbias
