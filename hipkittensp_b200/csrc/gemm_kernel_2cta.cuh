@@ -537,22 +537,33 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                             }
                         }
                     } else {
-                    const int col = q0 + piece * OC + 2 * lane;
-#pragma unroll 4
-                    for (int r = quad * 32; r < quad * 32 + 32; ++r) {
-                        const int row = my_p0 + r;
-                        if (row >= P.c_rows) break;
-                        const uint32_t x = *reinterpret_cast<const uint32_t*>(stage + r * (OC * 2) + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+                        // 32 rows of 64 columns per warp, two columns per lane.  Rows go in batches whose reads are independent (a row at
+                        // a time cost 150 ns a row: 1111 x 2050 x 1920 in 27.6 us against 9.0 us for N = 2048).
+                        const int col = q0 + piece * OC + 2 * lane;
+                        const bool two = col + 1 < P.c_cols, one = col < P.c_cols;
                         for (int d = 0; d < P.ndst; ++d) {
-                            __nv_bfloat16* dst = (d == 0 ? P.c : P.c_more[d - 1]) + (size_t)row * P.ldc + col;
-                            if (col + 1 < P.c_cols && (reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
-                                *reinterpret_cast<uint32_t*>(dst) = x;
-                            } else {
-                                if (col < P.c_cols) dst[0] = __ushort_as_bfloat16((unsigned short)(x & 0xffffu));
-                                if (col + 1 < P.c_cols) dst[1] = __ushort_as_bfloat16((unsigned short)(x >> 16));
+                            __nv_bfloat16* cbase = d == 0 ? P.c : P.c_more[d - 1];
+                            const bool words = (P.ldc & 1) == 0 && (reinterpret_cast<uintptr_t>(cbase) & 3) == 0;      // every column pair on 4 bytes
+#pragma unroll 1
+                            for (int r0 = quad * 32; r0 < quad * 32 + 32; r0 += 8) {
+                                uint32_t x[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    x[i] = *reinterpret_cast<const uint32_t*>(stage + (r0 + i) * (OC * 2) + ((((lane >> 2) ^ ((r0 + i) & 7)) << 4) | ((lane & 3) << 2)));
+                                __nv_bfloat16* dst = cbase + (size_t)(my_p0 + r0) * P.ldc + col;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i, dst += P.ldc) {
+                                    const bool row_in = my_p0 + r0 + i < P.c_rows;
+                                    if (words) {
+                                        if (row_in && two) *reinterpret_cast<uint32_t*>(dst) = x[i];
+                                        if (row_in && one && !two) dst[0] = __ushort_as_bfloat16((unsigned short)(x[i] & 0xffffu));
+                                    } else {
+                                        if (row_in && one) dst[0] = __ushort_as_bfloat16((unsigned short)(x[i] & 0xffffu));
+                                        if (row_in && two) dst[1] = __ushort_as_bfloat16((unsigned short)(x[i] >> 16));
+                                    }
+                                }
                             }
                         }
-                    }
                     }
                     // (the next use of this buffer is two pieces away, behind the barrier that opens every piece)
                     ++n_out;
