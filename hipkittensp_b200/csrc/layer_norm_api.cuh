@@ -48,8 +48,9 @@ static LnChoice ln_forward_kernel(bool vec, int fmt, int H) {
     }
 }
 
-// Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row.
-constexpr int kLnBackwardMax = 8192;
+// Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row; bf16 rows of whole chunks up to 16384 keep x and dy
+// in shared memory.
+constexpr int kLnBackwardMax = 8192, kLnBackwardWide = 16384;
 static int ln_backward_warps(int H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
 template <typename T>
 static LnChoice ln_backward_kernel(bool vec, int H) {
@@ -75,9 +76,8 @@ static LnChoice ln_backward_kernel(bool vec, int H) {
     }
 }
 
-// Number of partial sums per column of the parameter gradients, which is the grid of the kernel that writes them.
-static int ln_backward_parts(int64_t rows, int64_t H, int sm_count) {
-    if (rows <= 0) return 0;
+// Number of partial sums per column of the parameter gradients: the grid of the kernel that writes them.
+static int ln_parts(int64_t rows, int64_t H, int sm_count) {
     if (H <= kLnBackwardMax) {
         const int warps = ln_backward_warps((int)H);
         const int64_t want = warps == 1 ? (rows + 7) / 8 : rows;
@@ -87,6 +87,13 @@ static int ln_backward_parts(int64_t rows, int64_t H, int sm_count) {
     int64_t y = 8 * (int64_t)sm_count / ((H + 255) / 256);
     if (y > (rows + 15) / 16) y = (rows + 15) / 16;
     return (int)(y < 1 ? 1 : y);
+}
+static int ln_parts_wide(int64_t rows, int sm_count) { return (int)(rows < sm_count ? rows : sm_count); }
+// ... the most that any kernel which may serve such rows writes (their type and alignment are not known here)
+static int ln_parts_most(int64_t rows, int64_t H, int sm_count) {
+    if (rows <= 0) return 0;
+    const int n = ln_parts(rows, H, sm_count), w = H > kLnBackwardMax && H <= kLnBackwardWide ? ln_parts_wide(rows, sm_count) : 0;
+    return n > w ? n : w;
 }
 
 static int ln_check(const char* what, int64_t rows, int64_t H, int x_dtype, int w_dtype) {
@@ -150,8 +157,8 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
     const bool sums = dw || db;
-    const int parts = ln_backward_parts(rows, H, d->sm_count);
-    const size_t need = sums ? (size_t)parts * 2 * (size_t)H * 4 : 0;
+    // one size for every type and alignment of such rows
+    const size_t need = sums ? (size_t)ln_parts_most(rows, H, d->sm_count) * 2 * (size_t)H * 4 : 0;
     if (sums && (!ws || ws_bytes < need)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace too small: need %zu bytes, got %zu", what, need, ws ? ws_bytes : 0);
     if (sums && ((uintptr_t)ws & 15)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace must be 16-byte aligned", what);
     const bool vec = H % 8 == 0 && ln_rows_vec(x, x_dtype) && ln_rows_vec(dy, x_dtype) && ln_rows_vec(dx, x_dtype) && !((uintptr_t)w & 15);
@@ -160,9 +167,15 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd);
     P.part = sums ? (float*)ws : nullptr;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H;
+    int parts = ln_parts(rows, H, d->sm_count);
     if (H <= kLnBackwardMax) {
         const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(vec, (int)H) : ln_backward_kernel<__nv_bfloat16>(vec, (int)H);
         if ((rc = launch_pdl(k.kern, (unsigned)parts, (unsigned)(k.warps == 1 ? 256 : 32 * k.warps), (size_t)k.smem, st, P))) return rc;
+    } else if (vec && x_dtype == 1 && H <= kLnBackwardWide) {
+        const int smem = 4 * (int)H + 2 * 2 * 4 * 512 * 16;
+        parts = ln_parts_wide(rows, d->sm_count);
+        if ((rc = ensure_smem_attr(*d, (const void*)layer_norm_backward_wide_kernel, 4 * kLnBackwardWide + 2 * 2 * 4 * 512 * 16))) return rc;
+        if ((rc = launch_pdl(layer_norm_backward_wide_kernel, (unsigned)parts, 512, (size_t)smem, st, P))) return rc;
     } else {
         if (sums) {
             LnKernel k = x_dtype == 0 ? layer_norm_columns_kernel<float> : layer_norm_columns_kernel<__nv_bfloat16>;

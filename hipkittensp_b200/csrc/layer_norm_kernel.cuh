@@ -513,6 +513,114 @@ layer_norm_backward_kernel(const LnParams P) {
     }
 }
 
+// bf16 rows of 8192 to 16384 elements: four chunks per thread, whose column sums alone take 64 of its 128 registers.  x and dy of
+// the next two rows are copied by cp.async into slots of shared memory that only this thread reads (no barrier), and both passes
+// over a row read them there (4096 x 16384 in 83 us; passing over global memory again and summing the columns in a kernel of
+// their own took 311 us).
+__global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const LnParams P) {
+    typedef __nv_bfloat16 T;
+    constexpr int C = 4, D = 2, TPR = 512, SLOT = TPR * 16;
+    __shared__ float red[2][2 * 16];
+    extern __shared__ float4 prm[];                             // w, then the slots: [x, dy][row][chunk][thread]
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, n8 = P.H >> 3;
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const T* dy = reinterpret_cast<const T*>(P.dy);
+    const uint32_t sx = smem_u32(prm + 2 * n8) + tid * 16, sg = sx + D * C * SLOT;
+    // columns past H are never copied and stay zero
+#pragma unroll
+    for (int i = 0; i < 2 * D * C; ++i) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sx + i * SLOT), "r"(0) : "memory");
+    auto load = [&](int d, int64_t r) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            if (r < P.rows && chunk < n8) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sx + (d * C + c) * SLOT), "l"(x + r * P.H + 8 * chunk) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sg + (d * C + c) * SLOT), "l"(dy + r * P.H + 8 * chunk) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto take = [&](uint32_t slot, float2 (&v)[4]) {
+        Raw<T, 8> r;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"(slot) : "memory");
+        unpack2<T>(r, v);
+    };
+    float2 dw[C][4], db[C][4];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = make_float2(0.f, 0.f);
+    int64_t row = blockIdx.x;
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(d, row + (int64_t)d * gridDim.x);
+    float mean_n = 0.f, rstd_n = 0.f;
+    if (row < P.rows) { mean_n = __ldcg(P.mean + row); rstd_n = __ldcg(P.rstd + row); }
+    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
+    __syncthreads();
+    for (int par = 0; row < P.rows; row += gridDim.x, par ^= 1) {
+        static_assert(D == 2, "the slot alternates with the parity of the reduction");
+        const float mean = mean_n, rstd = rstd_n;
+        const int64_t next = row + gridDim.x;
+        if (next < P.rows) { mean_n = __ldcg(P.mean + next); rstd_n = __ldcg(P.rstd + next); }
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+        float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            // (threads past H: dy is zero there, and so is all that is summed)
+            const int chunk = tid + c * TPR;
+            float2 xh[4], g[4], w[4];
+            take(sx + (par * C + c) * SLOT, xh);
+            take(sg + (par * C + c) * SLOT, g);
+            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xh[i] = __fmul2_rn(__fadd2_rn(xh[i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                dw[c][i] = __ffma2_rn(g[i], xh[i], dw[c][i]);
+                db[c][i] = __fadd2_rn(db[c][i], g[i]);
+                g[i] = __fmul2_rn(g[i], w[i]);
+                a2 = __fadd2_rn(a2, g[i]);
+                b2 = __ffma2_rn(g[i], xh[i], b2);
+            }
+        }
+        float s[2] = {a2.x + a2.y, b2.x + b2.y};
+        row_sum<2, 16>(s, red[par]);
+        const float m1 = -s[0] * P.inv_h, m2 = -s[1] * P.inv_h;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int chunk = tid + c * TPR;
+            float2 xh[4], g[4], w[4];
+            take(sx + (par * C + c) * SLOT, xh);
+            take(sg + (par * C + c) * SLOT, g);
+            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xh[i] = __fmul2_rn(__fadd2_rn(xh[i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                g[i] = __fmul2_rn(g[i], w[i]);
+                g[i] = __fmul2_rn(__fadd2_rn(g[i], __ffma2_rn(xh[i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
+            }
+            if (chunk < n8) st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g);
+        }
+        load(par, row + (int64_t)D * gridDim.x);                // the slots of this row have been read
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!P.part) return;
+    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int chunk = tid + c * TPR;
+        if (chunk < n8) {
+            float4* o = reinterpret_cast<float4*>(out + 8 * chunk);
+            o[0] = make_float4(dw[c][0].x, dw[c][0].y, dw[c][1].x, dw[c][1].y);
+            o[1] = make_float4(dw[c][2].x, dw[c][2].y, dw[c][3].x, dw[c][3].y);
+            o = reinterpret_cast<float4*>(out + P.H + 8 * chunk);
+            o[0] = make_float4(db[c][0].x, db[c][0].y, db[c][1].x, db[c][1].y);
+            o[1] = make_float4(db[c][2].x, db[c][2].y, db[c][3].x, db[c][3].y);
+        }
+    }
+}
+
 // Rows of any width and alignment, one element per access.
 template <typename T, int C, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
