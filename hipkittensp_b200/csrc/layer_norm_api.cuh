@@ -11,89 +11,104 @@ struct LnChoice {
     int smem;        // dynamic shared memory
 };
 
-// Whole 8-element chunks: a thread holds up to four, sixteen warps a row: 16384 elements.
-template <typename T, int FMT>
-static LnChoice ln_forward_vec(int H) {
-    const int smem = 8 * H;          // w and b as fp32
-    if (H <= 256) return {layer_norm_kernel<T, 1, 1, FMT>, 1, smem};
-    if (H <= 1024) return {layer_norm_kernel<T, 4, 1, FMT>, 1, smem};
-    if (H <= 2048) return {layer_norm_kernel<T, 4, 2, FMT>, 2, smem};
-    if (H <= 4096) return {layer_norm_kernel<T, 4, 4, FMT>, 4, smem};
-    if (H <= 8192) return {layer_norm_kernel<T, 4, 8, FMT>, 8, smem};
-    if (H <= 16384) return {layer_norm_kernel<T, 4, 16, FMT>, 16, smem};
-    return {layer_norm_long_kernel<T, 8, FMT>, 0, 0};
+// How the rows of the matrices lie: whole aligned chunks of 8 elements; any width and start, but the same place in the 16- or
+// 32-byte units of memory in each matrix; or anything else.
+enum LnRows : int { kLnWhole, kLnOdd, kLnApart };
+static LnRows ln_rows(int64_t H, int dtype, const void* w, const void* b, const void* p, const void* q, const void* r) {
+    const uintptr_t unit = dtype == 0 ? 31 : 15, at = (uintptr_t)p & unit;
+    if (((uintptr_t)q & unit) != at || ((uintptr_t)r & unit) != at) return kLnApart;
+    return at == 0 && H % 8 == 0 && !((uintptr_t)w & 15) && !((uintptr_t)b & 15) ? kLnWhole : kLnOdd;
 }
-template <typename T>
-static LnChoice ln_forward_odd(int H) {
-    if (H <= 256) return {layer_norm_odd_kernel<T, 8, 1>, 1, 0};
-    if (H <= 512) return {layer_norm_odd_kernel<T, 8, 2>, 2, 0};
-    if (H <= 1024) return {layer_norm_odd_kernel<T, 8, 4>, 4, 0};
-    if (H <= 2048) return {layer_norm_odd_kernel<T, 8, 8>, 8, 0};
-    if (H <= 4096) return {layer_norm_odd_kernel<T, 8, 16>, 16, 0};
-    if (H <= 8192) return {layer_norm_odd_kernel<T, 16, 16>, 16, 0};
-    if (H <= 16384) return {layer_norm_odd_kernel<T, 32, 16>, 16, 0};
-    return {layer_norm_long_kernel<T, 1, -1>, 0, 0};
+
+// A thread holds up to four chunks, sixteen warps a row: 16384 elements, and 7 fewer where the row may start anywhere in its chunk.
+template <typename T, int FMT, bool ODD>
+static LnChoice ln_forward_choice(int H) {
+    const int smem = 8 * H + (ODD ? 128 : 0);          // w and b as fp32
+    const int span = H + (ODD ? 7 : 0);
+    if (span <= 256) return {layer_norm_kernel<T, 1, 1, FMT, ODD>, 1, smem};
+    if (span <= 1024) return {layer_norm_kernel<T, 4, 1, FMT, ODD>, 1, smem};
+    if (span <= 2048) return {layer_norm_kernel<T, 4, 2, FMT, ODD>, 2, smem};
+    if (span <= 4096) return {layer_norm_kernel<T, 4, 4, FMT, ODD>, 4, smem};
+    if (span <= 8192) return {layer_norm_kernel<T, 4, 8, FMT, ODD>, 8, smem};
+    if (span <= 16384) return {layer_norm_kernel<T, 4, 16, FMT, ODD>, 16, smem};
+    return {layer_norm_long_kernel<T, ODD ? 1 : 8, FMT>, 0, 0};
 }
 // fmt: format of an MX result, negative for one in x's type
 template <typename T>
-static LnChoice ln_forward_kernel(bool vec, int fmt, int H) {
-    if (!vec) return ln_forward_odd<T>(H);
+static LnChoice ln_forward_kernel(LnRows rows, int fmt, int H) {
+    if (rows == kLnApart) return {layer_norm_long_kernel<T, 1, -1>, 0, 0};
+    if (rows == kLnOdd) return ln_forward_choice<T, -1, true>(H);
     switch (fmt) {
-        case MXFP6_E2M3: return ln_forward_vec<T, MXFP6_E2M3>(H);
-        case MXFP6_E3M2: return ln_forward_vec<T, MXFP6_E3M2>(H);
-        case MXFP8_E4M3: return ln_forward_vec<T, MXFP8_E4M3>(H);
-        case MXFP8_E5M2: return ln_forward_vec<T, MXFP8_E5M2>(H);
-        case MXFP4_E2M1: return ln_forward_vec<T, MXFP4_E2M1>(H);
-        default: return ln_forward_vec<T, -1>(H);
+        case MXFP6_E2M3: return ln_forward_choice<T, MXFP6_E2M3, false>(H);
+        case MXFP6_E3M2: return ln_forward_choice<T, MXFP6_E3M2, false>(H);
+        case MXFP8_E4M3: return ln_forward_choice<T, MXFP8_E4M3, false>(H);
+        case MXFP8_E5M2: return ln_forward_choice<T, MXFP8_E5M2, false>(H);
+        case MXFP4_E2M1: return ln_forward_choice<T, MXFP4_E2M1, false>(H);
+        default: return ln_forward_choice<T, -1, false>(H);
     }
 }
 
 // Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row; bf16 rows of whole chunks up to 16384 keep x and dy
-// in shared memory.
+// in shared memory; the rest (kern = null) goes over its rows again.
 constexpr int kLnBackwardMax = 8192, kLnBackwardWide = 16384;
-static int ln_backward_warps(int H) { return H <= 512 ? 1 : H <= 1024 ? 2 : H <= 2048 ? 4 : H <= 4096 ? 8 : 16; }
+static int ln_backward_warps(int span) { return span <= 512 ? 1 : span <= 1024 ? 2 : span <= 2048 ? 4 : span <= 4096 ? 8 : 16; }
+template <typename T, bool ODD>
+static LnChoice ln_backward_choice(int H) {
+    const int span = H + (ODD ? 7 : 0);
+    if (span > kLnBackwardMax) return {nullptr, 0, 0};
+    const int smem = 4 * H + (ODD ? 64 : 0);           // w as fp32; one warp per row: room for the eight warps' column sums
+    if (span <= 256) return {layer_norm_backward_kernel<T, 1, 1, ODD>, 1, 8 * 256 * 4};
+    switch (ln_backward_warps(span)) {
+        case 1: return {layer_norm_backward_kernel<T, 2, 1, ODD>, 1, 8 * 512 * 4};
+        case 2: return {layer_norm_backward_kernel<T, 2, 2, ODD>, 2, smem};
+        case 4: return {layer_norm_backward_kernel<T, 2, 4, ODD>, 4, smem};
+        case 8: return {layer_norm_backward_kernel<T, 2, 8, ODD>, 8, smem};
+        default: return {layer_norm_backward_kernel<T, 2, 16, ODD>, 16, smem};
+    }
+}
 template <typename T>
-static LnChoice ln_backward_kernel(bool vec, int H) {
-    const int warps = ln_backward_warps(H);
-    if (vec) {
-        // w as fp32; one warp per row: room for the eight warps' column sums
-        if (H <= 256) return {layer_norm_backward_kernel<T, 1, 1>, 1, 8 * 256 * 4};
-        switch (warps) {
-            case 1: return {layer_norm_backward_kernel<T, 2, 1>, 1, 8 * 512 * 4};
-            case 2: return {layer_norm_backward_kernel<T, 2, 2>, 2, 4 * H};
-            case 4: return {layer_norm_backward_kernel<T, 2, 4>, 4, 4 * H};
-            case 8: return {layer_norm_backward_kernel<T, 2, 8>, 8, 4 * H};
-            default: return {layer_norm_backward_kernel<T, 2, 16>, 16, 4 * H};
-        }
+static LnChoice ln_backward_kernel(LnRows rows, int H) {
+    return rows == kLnApart ? LnChoice{nullptr, 0, 0} : rows == kLnOdd ? ln_backward_choice<T, true>(H) : ln_backward_choice<T, false>(H);
+}
+
+// CTAs for `rows` rows at a time (eight rows per CTA when a warp owns one), at most cap, and the step from one of a CTA's rows to
+// its next.  Rows that start anywhere are dealt so that a CTA's rows lie a multiple of eight apart.
+static int ln_grid(int64_t rows, int warps, bool odd, int64_t cap, int64_t* step) {
+    int64_t grid;
+    if (odd) {
+        const int64_t want = warps == 1 ? 8 * ((rows + 63) / 64) : rows;
+        cap = cap / 8 * 8;
+        grid = want <= cap ? want : cap;
+        *step = want <= cap ? (warps == 1 ? 8 * grid : rows) : (warps == 1 ? 8 * grid : grid);
+    } else {
+        const int64_t want = warps == 1 ? (rows + 7) / 8 : rows;
+        grid = want < cap ? want : cap;
+        *step = warps == 1 ? 8 * grid : grid;
     }
-    if (H <= 256) return {layer_norm_backward_odd_kernel<T, 8, 1>, 1, 0};
-    switch (warps) {
-        case 1: return {layer_norm_backward_odd_kernel<T, 16, 1>, 1, 0};
-        case 2: return {layer_norm_backward_odd_kernel<T, 16, 2>, 2, 0};
-        case 4: return {layer_norm_backward_odd_kernel<T, 16, 4>, 4, 0};
-        case 8: return {layer_norm_backward_odd_kernel<T, 16, 8>, 8, 0};
-        default: return {layer_norm_backward_odd_kernel<T, 16, 16>, 16, 0};
-    }
+    return (int)grid;
 }
 
 // Number of partial sums per column of the parameter gradients: the grid of the kernel that writes them.
-static int ln_parts(int64_t rows, int64_t H, int sm_count) {
-    if (H <= kLnBackwardMax) {
-        const int warps = ln_backward_warps((int)H);
-        const int64_t want = warps == 1 ? (rows + 7) / 8 : rows;
-        const int64_t cap = (int64_t)sm_count * (warps == 1 ? 2 : 16 / warps);      // 512 threads of 128 registers per SM
-        return (int)(want < cap ? want : cap);
-    }
+static int64_t ln_backward_cap(int warps, int sm_count) { return (int64_t)sm_count * (warps == 1 ? 2 : 16 / warps); }      // 512 threads of 128 registers per SM
+static int ln_parts_wide(int64_t rows, int sm_count) { return (int)(rows < sm_count ? rows : sm_count); }
+static int ln_parts_columns(int64_t rows, int64_t H, int sm_count) {
     int64_t y = 8 * (int64_t)sm_count / ((H + 255) / 256);
     if (y > (rows + 15) / 16) y = (rows + 15) / 16;
     return (int)(y < 1 ? 1 : y);
 }
-static int ln_parts_wide(int64_t rows, int sm_count) { return (int)(rows < sm_count ? rows : sm_count); }
-// ... the most that any kernel which may serve such rows writes (their type and alignment are not known here)
-static int ln_parts_most(int64_t rows, int64_t H, int sm_count) {
+// ... the most that any kernel which may serve such rows writes (their type and place are not known here)
+static int64_t ln_parts_most(int64_t rows, int64_t H, int sm_count) {
     if (rows <= 0) return 0;
-    const int n = ln_parts(rows, H, sm_count), w = H > kLnBackwardMax && H <= kLnBackwardWide ? ln_parts_wide(rows, sm_count) : 0;
-    return n > w ? n : w;
+    int64_t most = ln_parts_columns(rows, H, sm_count), step;
+    auto take = [&](int64_t n) { if (n > most) most = n; };
+    for (int odd = 0; odd < 2; ++odd) {
+        const int64_t span = H + 7 * odd;
+        if (span > kLnBackwardMax) continue;
+        const int warps = ln_backward_warps((int)span);
+        take(ln_grid(rows, warps, odd != 0, ln_backward_cap(warps, sm_count), &step));
+    }
+    if (H > kLnBackwardMax && H <= kLnBackwardWide) take(ln_parts_wide(rows, sm_count));
+    return most;
 }
 
 static int ln_check(const char* what, int64_t rows, int64_t H, int x_dtype, int w_dtype) {
@@ -104,8 +119,9 @@ static int ln_check(const char* what, int64_t rows, int64_t H, int x_dtype, int 
     return MXFP6_OK;
 }
 static bool ln_natural(const void* p, int dtype) { return !((uintptr_t)p & (dtype == 0 ? 3 : 1)); }
-// whole 8-element loads of the row matrices (32 or 16 bytes) and of the parameter vectors (16 bytes at a time)
-static bool ln_rows_vec(const void* p, int dtype) { return !((uintptr_t)p & (dtype == 0 ? 31 : 15)); }
+
+// elements from the 16- or 32-byte boundary in front of p to p
+static int ln_offset(const void* p, int dtype) { return (int)((uintptr_t)p & (dtype == 0 ? 31 : 15)) / (dtype == 0 ? 4 : 2); }
 
 static int ln_forward(const char* what, const void* x, int x_dtype, const void* w, const void* b, int w_dtype, void* y, int fmt,
                       void* packed, void* scales, float* mean, float* rstd, int64_t rows, int64_t H, float eps, void* stream) {
@@ -120,22 +136,23 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
     if (!ln_natural(x, x_dtype) || !ln_natural(y, x_dtype) || !ln_natural(w, w_dtype) || !ln_natural(b, w_dtype) ||
         !ln_natural(mean, 0) || !ln_natural(rstd, 0))
         return fail(MXFP6_ERR_BAD_ARG, "%s: misaligned pointer", what);
-    const bool vec = H % 8 == 0 && ln_rows_vec(x, x_dtype) && ln_rows_vec(y, x_dtype) && !((uintptr_t)w & 15) && !((uintptr_t)b & 15);
-    if (mx && (!vec || ((uintptr_t)packed & 15)))
+    const LnRows place = ln_rows(H, x_dtype, w, b, x, mx ? x : y, x);
+    if (mx && (place != kLnWhole || ((uintptr_t)packed & 15)))
         return fail(MXFP6_ERR_BAD_ARG, "%s: x must be 32-byte (fp32) or 16-byte (bf16) aligned, weight, bias and codes 16-byte", what);
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
-    const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(vec, fmt, (int)H) : ln_forward_kernel<__nv_bfloat16>(vec, fmt, (int)H);
+    const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(place, fmt, (int)H) : ln_forward_kernel<__nv_bfloat16>(place, fmt, (int)H);
     const int threads = k.warps == 0 ? 1024 : k.warps == 1 ? 256 : 32 * k.warps;
     int per_sm = 0;
     if ((rc = resident_ctas(*d, (const void*)k.kern, threads, k.smem, &per_sm))) return rc;
-    const int64_t want = k.warps == 1 ? (rows + 7) / 8 : rows, cap = (int64_t)d->sm_count * per_sm;
     LnParams P{};
     P.x = x; P.y = y; P.w = w; P.b = b; P.w_bf16 = w_dtype;
     P.mean = mean; P.rstd = rstd;
     P.q_out = (uint8_t*)packed; P.q_scales = (uint8_t*)scales;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H; P.eps = eps;
-    return launch_pdl(k.kern, (unsigned)(want < cap ? want : cap), (unsigned)threads, (size_t)k.smem, (cudaStream_t)stream, P);
+    P.offset = ln_offset(x, x_dtype);
+    const int grid = ln_grid(rows, k.warps, place == kLnOdd && k.warps > 0, (int64_t)d->sm_count * per_sm, &P.step);
+    return launch_pdl(k.kern, (unsigned)grid, (unsigned)threads, (size_t)k.smem, (cudaStream_t)stream, P);
 }
 
 static int ln_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd, const void* w, int w_dtype,
@@ -161,31 +178,35 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     const size_t need = sums ? (size_t)ln_parts_most(rows, H, d->sm_count) * 2 * (size_t)H * 4 : 0;
     if (sums && (!ws || ws_bytes < need)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace too small: need %zu bytes, got %zu", what, need, ws ? ws_bytes : 0);
     if (sums && ((uintptr_t)ws & 15)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace must be 16-byte aligned", what);
-    const bool vec = H % 8 == 0 && ln_rows_vec(x, x_dtype) && ln_rows_vec(dy, x_dtype) && ln_rows_vec(dx, x_dtype) && !((uintptr_t)w & 15);
+    const LnRows place = ln_rows(H, x_dtype, w, nullptr, x, dy, dx);
     LnParams P{};
     P.x = x; P.dy = dy; P.y = dx; P.w = w; P.w_bf16 = w_dtype;
     P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd);
     P.part = sums ? (float*)ws : nullptr;
     P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H;
-    int parts = ln_parts(rows, H, d->sm_count);
-    if (H <= kLnBackwardMax) {
-        const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(vec, (int)H) : ln_backward_kernel<__nv_bfloat16>(vec, (int)H);
+    P.offset = ln_offset(x, x_dtype);
+    const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(place, (int)H) : ln_backward_kernel<__nv_bfloat16>(place, (int)H);
+    int parts;
+    if (k.kern) {
+        parts = ln_grid(rows, k.warps, place == kLnOdd, ln_backward_cap(k.warps, d->sm_count), &P.step);
         if ((rc = launch_pdl(k.kern, (unsigned)parts, (unsigned)(k.warps == 1 ? 256 : 32 * k.warps), (size_t)k.smem, st, P))) return rc;
-    } else if (vec && x_dtype == 1 && H <= kLnBackwardWide) {
+    } else if (place == kLnWhole && x_dtype == 1 && H <= kLnBackwardWide) {
         const int smem = 4 * (int)H + 2 * 2 * 4 * 512 * 16;
         parts = ln_parts_wide(rows, d->sm_count);
         if ((rc = ensure_smem_attr(*d, (const void*)layer_norm_backward_wide_kernel, 4 * kLnBackwardWide + 2 * 2 * 4 * 512 * 16))) return rc;
         if ((rc = launch_pdl(layer_norm_backward_wide_kernel, (unsigned)parts, 512, (size_t)smem, st, P))) return rc;
     } else {
+        parts = ln_parts_columns(rows, H, d->sm_count);
         if (sums) {
-            LnKernel k = x_dtype == 0 ? layer_norm_columns_kernel<float> : layer_norm_columns_kernel<__nv_bfloat16>;
-            k<<<dim3((unsigned)((H + 255) / 256), (unsigned)parts), 256, 0, st>>>(P);
+            const LnKernel columns = x_dtype == 0 ? layer_norm_columns_kernel<float> : layer_norm_columns_kernel<__nv_bfloat16>;
+            columns<<<dim3((unsigned)((H + 255) / 256), (unsigned)parts), 256, 0, st>>>(P);
             CUDA_TRY(cudaGetLastError());
         }
-        const LnKernel k = x_dtype == 0 ? (vec ? layer_norm_backward_long_kernel<float, 8> : layer_norm_backward_long_kernel<float, 1>)
+        const bool vec = place == kLnWhole;
+        const LnKernel over = x_dtype == 0 ? (vec ? layer_norm_backward_long_kernel<float, 8> : layer_norm_backward_long_kernel<float, 1>)
                                         : (vec ? layer_norm_backward_long_kernel<__nv_bfloat16, 8> : layer_norm_backward_long_kernel<__nv_bfloat16, 1>);
         const int64_t cap = 2 * (int64_t)d->sm_count;
-        if ((rc = launch_pdl(k, (unsigned)(rows < cap ? rows : cap), 1024, 0, st, P))) return rc;
+        if ((rc = launch_pdl(over, (unsigned)(rows < cap ? rows : cap), 1024, 0, st, P))) return rc;
     }
     if (!sums) return MXFP6_OK;
     return launch_pdl(layer_norm_fold_kernel, (unsigned)((2 * H + 31) / 32), 1024, 0, st, (const float*)ws, parts, (int)H, dw, db);

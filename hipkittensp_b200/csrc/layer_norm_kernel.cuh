@@ -33,7 +33,9 @@ struct LnParams {
     uint8_t* q_out;          // forward to an MX operand: codes [rows, H * bits / 8] ...
     uint8_t* q_scales;       // ... and scales [rows, H / 32]
     int64_t rows;
+    int64_t step;            // rows from one of a thread's rows to its next
     int H;
+    int offset;              // elements from a chunk boundary (16 or 32 bytes) back to the first row's start
     float inv_h, eps;
 };
 
@@ -174,15 +176,68 @@ __device__ __forceinline__ void mx_store8(const float2 (&v)[4], uint8_t* codes_r
     if (live && j == 0) scales_row[col / 32] = (uint8_t)sb;
 }
 
-// Parameter vectors in shared memory, as fp32 whatever their type and filled where they are absent: float4 planes of H / 8
-// (the low halves of the 8-element chunks, then the high halves), so that neighbouring threads read neighbouring 16 bytes.
-__device__ __forceinline__ void stage_param(const void* w, int is_bf16, float fill, int H, float4* plane) {
-    const int n = H >> 3;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) {
+// ---- rows as chunks of 8 elements
+// Rows of whole, aligned chunks (ODD = false) are n = H / 8 chunks.  Other rows are cut at the same 16- or 32-byte boundaries of
+// memory: the row starts `a` elements behind a boundary, its first and last chunk may hold neighbours' elements (which are
+// neither read nor written: those two chunks go element by element), and column `col` is element col + a of the chunks.  `a` is
+// the same for rows that lie a multiple of 8 rows apart, so a CTA takes only such rows, its threads own the same columns in each
+// of them, and the parameters are staged once, shifted by a.
+template <bool ODD>
+struct Chunks {
+    int a, n, H;
+    __device__ __forceinline__ int lo(int chunk) const { return ODD ? min(max(a - 8 * chunk, 0), 8) : 0; }                // first element of the row in this chunk
+    __device__ __forceinline__ int hi(int chunk) const { return ODD ? min(max(a + H - 8 * chunk, 0), 8) : (chunk < n ? 8 : 0); }      // one past its last
+    __device__ __forceinline__ bool whole(int chunk) const { return ODD ? 8 * chunk >= a && 8 * chunk + 8 <= a + H : chunk < n; }
+};
+template <bool ODD>
+__device__ __forceinline__ Chunks<ODD> chunks_of(const LnParams& P, int64_t row) {
+    Chunks<ODD> k;
+    k.H = P.H;
+    k.a = ODD ? (int)((P.offset + row * P.H) & 7) : 0;
+    k.n = ODD ? (k.a + P.H + 7) >> 3 : P.H >> 3;
+    return k;
+}
+// first row of a group of WARPS warps (warp w of eight when one warp owns a row)
+template <bool ODD, int WARPS>
+__device__ __forceinline__ int64_t first_row(int w) {
+    if constexpr (ODD) return (blockIdx.x & 7) + 8 * ((int64_t)w + (WARPS == 1 ? 8 : 1) * (int64_t)(blockIdx.x >> 3));
+    return WARPS == 1 ? (int64_t)blockIdx.x * 8 + w : blockIdx.x;
+}
+// rowp: the row's first chunk (its start less a elements)
+template <typename T, bool ODD>
+__device__ __forceinline__ void ld_chunk(const T* rowp, int chunk, const Chunks<ODD>& k, Raw<T, 8>& r) {
+    if (k.whole(chunk)) {
+        r = ld_raw<T, 8>(rowp + 8 * chunk);
+    } else if constexpr (ODD) {
+        const int lo = k.lo(chunk), hi = k.hi(chunk);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            uint32_t u = 0;
+            if (i >= lo && i < hi) u = ld_raw<T, 1>(rowp + 8 * chunk + i).u[0];
+            if constexpr (sizeof(T) == 4) r.u[i] = u;
+            else r.u[i >> 1] = (i & 1) ? r.u[i >> 1] | (u << 16) : u;
+        }
+    }
+}
+// Parameter vectors in shared memory, as fp32 whatever their type and filled where they are absent: float4 planes of n chunks
+// (the low halves, then the high halves), so that neighbouring threads read neighbouring 16 bytes.
+template <bool ODD>
+__device__ __forceinline__ void stage_param(const void* w, int is_bf16, float fill, const Chunks<ODD>& k, float4* plane) {
+    for (int c = threadIdx.x; c < k.n; c += blockDim.x) {
         float v[8];
-        ld_param<8>(w, is_bf16, 8 * c, fill, v);
+        if constexpr (ODD) {
+            const int lo = k.lo(c), hi = k.hi(c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float t[1] = {0.f};
+                if (i >= lo && i < hi) ld_param<1>(w, is_bf16, 8 * c - k.a + i, fill, t);
+                v[i] = t[0];
+            }
+        } else {
+            ld_param<8>(w, is_bf16, 8 * c, fill, v);
+        }
         plane[c] = make_float4(v[0], v[1], v[2], v[3]);
-        plane[n + c] = make_float4(v[4], v[5], v[6], v[7]);
+        plane[k.n + c] = make_float4(v[4], v[5], v[6], v[7]);
     }
 }
 __device__ __forceinline__ void ld_staged(const float4* plane, int n, int chunk, float2 (&v)[4]) {
@@ -203,45 +258,62 @@ __device__ __forceinline__ void st_row2(T* p, const float2 (&v)[4]) {
     st_row<T, 8>(p, t);
 }
 
+template <typename T, bool ODD>
+__device__ __forceinline__ void st_chunk(T* rowp, int chunk, const Chunks<ODD>& k, const float2 (&v)[4]) {
+    if (k.whole(chunk)) {
+        st_row2<T>(rowp + 8 * chunk, v);
+    } else if constexpr (ODD) {
+        const float t[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+        const int lo = k.lo(chunk), hi = k.hi(chunk);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float o[1] = {t[i]};
+            if (i >= lo && i < hi) st_row<T, 1>(rowp + 8 * chunk + i, o);
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------- forward
 // WARPS warps own a row, C chunks of 8 elements per thread.  WARPS = 1: eight warps per CTA with a row each.  FMT < 0: the result is
 // written in x's type; otherwise it leaves as codes and scales.  The next row is on its way in registers while this one is worked
 // on, the arithmetic runs on pairs (fma.f32x2), and the parameters are staged once per CTA: bf16 rows are bound by issue, not by
 // HBM, when each element costs 25 instructions (16384 x 8192 in 124 us).  Threads whose columns lie past H take part in everything
 // but the stores, on zeros: a branch per chunk would keep the chunks' instructions from being interleaved.
-template <typename T, int C, int WARPS, int FMT>
+template <typename T, int C, int WARPS, int FMT, bool ODD>
 __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 : 16 / WARPS)
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
-    constexpr int ROWS = WARPS == 1 ? 8 : 1;                    // rows a CTA works on at a time
+    static_assert(!ODD || FMT < 0, "an MX result has whole blocks");
     __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
     extern __shared__ float4 prm[];                             // w, then b
     pdl_launch_dependents();
     pdl_wait();
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const int n8 = P.H >> 3;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
-    const T* x = reinterpret_cast<const T*>(P.x);
+    int64_t row = first_row<ODD, WARPS>(WARPS == 1 ? threadIdx.x >> 5 : 0);
+    const Chunks<ODD> K = chunks_of<ODD>(P, row);
+    const T* x = reinterpret_cast<const T*>(P.x) - K.a;
     Raw<T, 8> raw[C];
     auto load = [&](int64_t r) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int chunk = tid + c * TPR;
-            if (r < P.rows && chunk < n8) raw[c] = ld_raw<T, 8>(x + r * P.H + 8 * chunk);
-        }
+        for (int c = 0; c < C; ++c)
+            if (r < P.rows) ld_chunk<T, ODD>(x + r * P.H, tid + c * TPR, K, raw[c]);
     };
 #pragma unroll
-    for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};           // columns past H stay zero
+    for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};           // elements outside the row stay zero
     load(row);
-    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
-    stage_param(P.b, P.w_bf16, 0.f, P.H, prm + 2 * n8);
+    stage_param(P.w, P.w_bf16, 1.f, K, prm);
+    stage_param(P.b, P.w_bf16, 0.f, K, prm + 2 * K.n);
+    // does this warp hold elements outside the row?  (one decision per row; the same for all of this thread's rows)
+    bool inside = true;
+#pragma unroll
+    for (int c = 0; c < C; ++c) inside = inside && K.whole(tid + c * TPR);
+    const bool edge = !__all_sync(0xffffffffu, inside);
     __syncthreads();
-    for (int par = 0; row < P.rows; row += step, par ^= 1) {
+    for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
         float2 v[C][4];
 #pragma unroll
         for (int c = 0; c < C; ++c) unpack2<T>(raw[c], v[c]);
-        load(row + step);
+        load(row + P.step);
         float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -251,14 +323,28 @@ layer_norm_kernel(const LnParams P) {
         row_sum<1, WARPS>(s, red[par]);
         const float mean0 = s[0] * P.inv_h;
         float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
+        if (ODD && edge) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const float m = tid + c * TPR < n8 ? -mean0 : 0.f;
+            for (int c = 0; c < C; ++c) {
+                const int lo = K.lo(tid + c * TPR), hi = K.hi(tid + c * TPR);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[c][i] = __fadd2_rn(v[c][i], make_float2(m, m));
-                q2 = __ffma2_rn(v[c][i], v[c][i], q2);
-                d2 = __fadd2_rn(d2, v[c][i]);
+                for (int i = 0; i < 4; ++i) {
+                    const float2 m = make_float2(2 * i >= lo && 2 * i < hi ? -mean0 : 0.f, 2 * i + 1 >= lo && 2 * i + 1 < hi ? -mean0 : 0.f);
+                    v[c][i] = __fadd2_rn(v[c][i], m);
+                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                    d2 = __fadd2_rn(d2, v[c][i]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float m = ODD || tid + c * TPR < K.n ? -mean0 : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[c][i] = __fadd2_rn(v[c][i], make_float2(m, m));
+                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                    d2 = __fadd2_rn(d2, v[c][i]);
+                }
             }
         }
         float q[2] = {q2.x + q2.y, d2.x + d2.y};
@@ -273,74 +359,23 @@ layer_norm_kernel(const LnParams P) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
-            const bool live = chunk < n8;
+            const bool live = chunk < K.n;
             float2 o[4], w[4], b[4];
-            ld_staged(prm, n8, live ? chunk : 0, w);
-            ld_staged(prm + 2 * n8, n8, live ? chunk : 0, b);
+            ld_staged(prm, K.n, live ? chunk : 0, w);
+            ld_staged(prm + 2 * K.n, K.n, live ? chunk : 0, b);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 o[i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
             if constexpr (FMT >= 0)
                 mx_store8<FMT>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, live);
-            else if (live)
-                st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, o);
+            else
+                st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, o);
         }
     }
 }
 
-// Rows of any width and alignment (the result in x's type): V = 1 element per access, C per thread.
-template <typename T, int C, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
-layer_norm_odd_kernel(const LnParams P) {
-    constexpr int TPR = 32 * WARPS;
-    constexpr int ROWS = WARPS == 1 ? 8 : 1;
-    __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
-    pdl_launch_dependents();
-    pdl_wait();
-    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    int par = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0); row < P.rows; row += step, par ^= 1) {
-        const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
-        float v[C];
-        float s[1] = {0.f};
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = tid + c * TPR;
-            float t[1] = {0.f};
-            if (col < P.H) unpack<T, 1>(ld_raw<T, 1>(x + col), t);
-            v[c] = t[0];
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[0] += v[c];
-        row_sum<1, WARPS>(s, red[par]);
-        const float mean0 = s[0] * P.inv_h;
-        float q[2] = {0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (tid + c * TPR < P.H) { v[c] -= mean0; q[0] = fmaf(v[c], v[c], q[0]); q[1] += v[c]; }
-        row_sum<2, WARPS>(q, red2[par]);
-        const float corr = q[1] * P.inv_h;
-        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
-        if (tid == 0 && P.mean) P.mean[row] = mean0 + corr;
-        if (tid == 0 && P.rstd) P.rstd[row] = rstd;
-        const float shift = -corr * rstd;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = tid + c * TPR;
-            if (col < P.H) {
-                float w[1], b[1];
-                ld_param<1>(P.w, P.w_bf16, col, 1.f, w);
-                ld_param<1>(P.b, P.w_bf16, col, 0.f, b);
-                const float o[1] = {fmaf(fmaf(v[c], rstd, shift), w[0], b[0])};
-                st_row<T, 1>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
-            }
-        }
-    }
-}
-
-// Rows longer than the registers of a CTA hold: a CTA of 1024 threads passes over its row three times (the second and third
-// pass find it in L2).
+// Rows longer than the registers of a CTA hold, and rows of x and y that lie differently in their 16- or 32-byte units (V = 1): a CTA
+// of 1024 threads passes over its row three times (the second and third pass find it in L2).
 template <typename T, int V, int FMT>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P) {
     __shared__ float red[32], red2[64];
@@ -399,32 +434,27 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
 // WARPS warps own a row, C chunks of 8 columns per thread; the same columns of every row, whose parameter gradients the thread
 // sums in registers.  As in the forward kernel the next row is on its way while this one is worked on (without that, HBM idles
 // through every row's reduction: 16384 x 8192 bf16 in 273 us) and the arithmetic runs on pairs.
-template <typename T, int C, int WARPS>
+template <typename T, int C, int WARPS, bool ODD>
 __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 : 16 / WARPS)
 layer_norm_backward_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
-    constexpr int ROWS = WARPS == 1 ? 8 : 1;
     __shared__ float red[2][2 * WARPS];
     extern __shared__ float4 prm[];                             // w; at the end the warps' column sums (one warp per row)
     pdl_launch_dependents();
     pdl_wait();
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const int n8 = P.H >> 3;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0);
-    const T* x = reinterpret_cast<const T*>(P.x);
-    const T* dy = reinterpret_cast<const T*>(P.dy);
+    int64_t row = first_row<ODD, WARPS>(WARPS == 1 ? threadIdx.x >> 5 : 0);
+    const Chunks<ODD> K = chunks_of<ODD>(P, row);
+    const T* x = reinterpret_cast<const T*>(P.x) - K.a;
+    const T* dy = reinterpret_cast<const T*>(P.dy) - K.a;
     Raw<T, 8> rx[C], rg[C];
     float mean_n = 0.f, rstd_n = 0.f;
     auto load = [&](int64_t r) {
         if (r < P.rows) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int chunk = tid + c * TPR;
-                if (chunk < n8) {
-                    rx[c] = ld_raw<T, 8>(x + r * P.H + 8 * chunk);
-                    rg[c] = ld_raw<T, 8>(dy + r * P.H + 8 * chunk);
-                }
+                ld_chunk<T, ODD>(x + r * P.H, tid + c * TPR, K, rx[c]);
+                ld_chunk<T, ODD>(dy + r * P.H, tid + c * TPR, K, rg[c]);
             }
             mean_n = __ldcg(P.mean + r);
             rstd_n = __ldcg(P.rstd + r);
@@ -438,21 +468,21 @@ layer_norm_backward_kernel(const LnParams P) {
         for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = make_float2(0.f, 0.f);
     }
     load(row);
-    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
+    stage_param(P.w, P.w_bf16, 1.f, K, prm);
     __syncthreads();
-    for (int par = 0; row < P.rows; row += step, par ^= 1) {
+    for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
         const float mean = mean_n, rstd = rstd_n;
         float2 xh[C][4], g[C][4];
 #pragma unroll
         for (int c = 0; c < C; ++c) { unpack2<T>(rx[c], xh[c]); unpack2<T>(rg[c], g[c]); }
-        load(row + step);
+        load(row + P.step);
         float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            // (threads past H: dy is zero there, and so is all that is summed)
+            // (outside the row dy is zero, and so is all that is summed)
             const int chunk = tid + c * TPR;
             float2 w[4];
-            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
+            ld_staged(prm, K.n, chunk < K.n ? chunk : 0, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 // (the distance from the mean is taken before the scaling: x * rstd - mean * rstd loses digits of rows far from zero)
@@ -469,11 +499,10 @@ layer_norm_backward_kernel(const LnParams P) {
         const float m1 = -s[0] * P.inv_h, m2 = -s[1] * P.inv_h;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int chunk = tid + c * TPR;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 g[c][i] = __fmul2_rn(__fadd2_rn(g[c][i], __ffma2_rn(xh[c][i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
-            if (chunk < n8) st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g[c]);
+            st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, tid + c * TPR, K, g[c]);
         }
     }
     if (!P.part) return;
@@ -493,23 +522,29 @@ layer_norm_backward_kernel(const LnParams P) {
             for (int col = threadIdx.x; col < P.H; col += 256) {
                 float a = 0.f;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) a += fold[r * (TPR * 8 * C) + col];
+                for (int r = 0; r < 8; ++r) a += fold[r * (TPR * 8 * C) + K.a + col];
                 out[(int64_t)k * P.H + col] = a;
             }
         }
     } else {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int chunk = tid + c * TPR;
-            if (chunk < n8) {
-                float4* o = reinterpret_cast<float4*>(out + 8 * chunk);
-                o[0] = make_float4(dw[c][0].x, dw[c][0].y, dw[c][1].x, dw[c][1].y);
-                o[1] = make_float4(dw[c][2].x, dw[c][2].y, dw[c][3].x, dw[c][3].y);
-                o = reinterpret_cast<float4*>(out + P.H + 8 * chunk);
-                o[0] = make_float4(db[c][0].x, db[c][0].y, db[c][1].x, db[c][1].y);
-                o[1] = make_float4(db[c][2].x, db[c][2].y, db[c][3].x, db[c][3].y);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int chunk = tid + c * TPR;
+                float* o = out + (int64_t)k * P.H + 8 * chunk - K.a;
+                const float2 (&v)[4] = k ? db[c] : dw[c];
+                if constexpr (ODD) {
+                    const float t[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+                    const int lo = K.lo(chunk), hi = K.hi(chunk);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i >= lo && i < hi) o[i] = t[i];
+                } else if (chunk < K.n) {
+                    reinterpret_cast<float4*>(o)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+                    reinterpret_cast<float4*>(o)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+                }
             }
-        }
     }
 }
 
@@ -557,7 +592,7 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
     for (int d = 0; d < D; ++d) load(d, row + (int64_t)d * gridDim.x);
     float mean_n = 0.f, rstd_n = 0.f;
     if (row < P.rows) { mean_n = __ldcg(P.mean + row); rstd_n = __ldcg(P.rstd + row); }
-    stage_param(P.w, P.w_bf16, 1.f, P.H, prm);
+    stage_param(P.w, P.w_bf16, 1.f, Chunks<false>{0, n8, P.H}, prm);
     __syncthreads();
     for (int par = 0; row < P.rows; row += gridDim.x, par ^= 1) {
         static_assert(D == 2, "the slot alternates with the parity of the reduction");
@@ -617,83 +652,6 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
             o = reinterpret_cast<float4*>(out + P.H + 8 * chunk);
             o[0] = make_float4(db[c][0].x, db[c][0].y, db[c][1].x, db[c][1].y);
             o[1] = make_float4(db[c][2].x, db[c][2].y, db[c][3].x, db[c][3].y);
-        }
-    }
-}
-
-// Rows of any width and alignment, one element per access.
-template <typename T, int C, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS)
-layer_norm_backward_odd_kernel(const LnParams P) {
-    constexpr int TPR = 32 * WARPS;
-    constexpr int ROWS = WARPS == 1 ? 8 : 1;
-    __shared__ float red[2][2 * WARPS];
-    __shared__ float fold[WARPS == 1 ? 8 * 32 * C : 1];         // one warp per row: the warps' column sums meet here
-    pdl_launch_dependents();
-    pdl_wait();
-    const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const int64_t step = (int64_t)gridDim.x * ROWS;
-    float dw[C], db[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) dw[c] = db[c] = 0.f;
-    int par = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WARPS == 1 ? threadIdx.x >> 5 : 0); row < P.rows; row += step, par ^= 1) {
-        const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
-        const T* dy = reinterpret_cast<const T*>(P.dy) + row * P.H;
-        const float mean = __ldcg(P.mean + row), rstd = __ldcg(P.rstd + row);
-        float xh[C], g[C];
-        float s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = tid + c * TPR;
-            float t[1] = {0.f}, u[1] = {0.f};
-            if (col < P.H) { unpack<T, 1>(ld_raw<T, 1>(x + col), t); unpack<T, 1>(ld_raw<T, 1>(dy + col), u); }
-            xh[c] = t[0]; g[c] = u[0];
-        }
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = tid + c * TPR;
-            if (col < P.H) {
-                float w[1];
-                ld_param<1>(P.w, P.w_bf16, col, 1.f, w);
-                xh[c] = (xh[c] - mean) * rstd;
-                dw[c] = fmaf(g[c], xh[c], dw[c]);
-                db[c] += g[c];
-                g[c] *= w[0];
-                s[0] += g[c];
-                s[1] = fmaf(g[c], xh[c], s[1]);
-            }
-        }
-        row_sum<2, WARPS>(s, red[par]);
-        const float m1 = s[0] * P.inv_h, m2 = s[1] * P.inv_h;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = tid + c * TPR;
-            if (col < P.H) {
-                const float o[1] = {(g[c] - fmaf(xh[c], m2, m1)) * rstd};
-                st_row<T, 1>(reinterpret_cast<T*>(P.y) + row * P.H + col, o);
-            }
-        }
-    }
-    if (!P.part) return;
-    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if constexpr (WARPS == 1) {
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < C; ++c) fold[(threadIdx.x >> 5) * (32 * C) + tid + c * 32] = k ? db[c] : dw[c];
-            __syncthreads();
-            for (int col = threadIdx.x; col < P.H; col += 256) {
-                float a = 0.f;
-#pragma unroll
-                for (int r = 0; r < 8; ++r) a += fold[r * (32 * C) + col];
-                out[(int64_t)k * P.H + col] = a;
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (tid + c * TPR < P.H) out[(int64_t)k * P.H + tid + c * TPR] = k ? db[c] : dw[c];
         }
     }
 }

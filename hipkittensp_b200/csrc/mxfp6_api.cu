@@ -279,7 +279,7 @@ static int resident_ctas(DeviceState& d, const void* kern, int threads, int smem
     std::lock_guard<std::mutex> lk(g_mu);
     int& n = d.ctas_per_sm[{kern, smem}];
     if (n == 0) {
-        if (smem > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+        if (smem > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 132 * 1024));
         CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, (size_t)smem));
     }
     if (n < 1) return fail(MXFP6_ERR_CUDA, "a kernel of %d threads does not fit an SM", threads);

@@ -67,7 +67,8 @@ def _check_forward(x, w, b, eps, y, mean, rstd):
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} elements, worst {((y.double() - ry).abs() / tol).max().item():.2f} of the bound"
 
 
-WIDTHS = [1, 2, 7, 8, 31, 32, 96, 255, 256, 264, 512, 520, 1001, 1024, 1032, 2048, 2056, 4095, 4096, 5000, 8192, 8200, 16384, 16392, 16385, 40000]
+WIDTHS = [1, 2, 3, 7, 8, 9, 31, 32, 96, 249, 250, 255, 256, 264, 505, 506, 512, 520, 1001, 1017, 1018, 1024, 1032, 2041, 2042, 2048, 2056, 4090, 4095, 4096, 5000, 8185, 8186,
+          8192, 8200, 16377, 16378, 16384, 16392, 16385, 40000]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -105,6 +106,34 @@ def test_forward_without_parameters_in_place_and_unaligned():
     y, mean, rstd = hk.layer_norm(xs, w, b, out=ys)
     _check_forward(x, w, b, 1e-5, y, mean, rstd)
     assert buf[0] == 7 and buf[-1] == 7
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,H", [(1, 5), (40, 9), (500, 33), (777, 1003), (300, 3001), (5000, 67), (200, 16370)])
+@pytest.mark.parametrize("start", [0, 1, 5])
+def test_rows_that_start_anywhere(rows, H, dtype, start):
+    """Rows of odd widths from a buffer that starts off every vector boundary: nothing beside the rows is written, and what lies
+    there (NaN) is not read; both passes, many rows per CTA and few."""
+    x, w, b, dy = _inputs(rows, H, dtype)
+    n = rows * H
+    make = lambda t: torch.full((n + 16,), float("nan"), dtype=dtype, device=DEV)
+    bufs = [make(t) for t in range(4)]
+    xs, ys, gs, ds = (t[start:start + n].view(rows, H) for t in bufs)
+    xs.copy_(x)
+    gs.copy_(dy)
+    y, mean, rstd = hk.layer_norm(xs, w, b, out=ys)
+    _check_forward(x, w, b, 1e-5, y, mean, rstd)
+    dw, db = torch.empty(H, device=DEV), torch.empty(H, device=DEV)
+    nbytes = hk.lib.mxfp6_layer_norm_backward_workspace_bytes(rows, H)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+    for dx in (ds, torch.empty(n + 16, dtype=dtype, device=DEV)[(start + 1) % 8:][:n].view(rows, H)):      # the second lies apart from x and dy
+        rc = hk.lib.mxfp6_layer_norm_backward(gs.data_ptr(), xs.data_ptr(), 0 if dtype == torch.float32 else 1, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+                                              0 if dtype == torch.float32 else 1, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), rows, H, work.data_ptr(), nbytes,
+                                              torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, hk.lib.mxfp6_last_error()
+        _check_backward(dy, x, mean, rstd, w, dx, dw, db)
+    for t in bufs:
+        assert torch.isnan(t[:start]).all() and torch.isnan(t[start + n:]).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
