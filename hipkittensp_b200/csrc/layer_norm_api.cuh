@@ -26,6 +26,16 @@ static LnChoice ln_forward_choice(int H) {
     const int smem = 8 * H + (ODD ? 128 : 0);          // w and b as fp32
     const int span = H + (ODD ? 7 : 0);
     if (span <= 256) return {layer_norm_kernel<T, 1, 1, FMT, ODD>, 1, smem};
+    if (span <= 512) return {layer_norm_kernel<T, 2, 1, FMT, ODD>, 1, smem};
+    // three chunks per thread where they are enough: with four, up to half of the threads would work on nothing
+    // (8192 x 5000 bf16 41 -> 39 us, 30000 x 700 27 -> 22 us)
+    if constexpr (FMT < 0) {
+        if (span <= 768) return {layer_norm_kernel<T, 3, 1, FMT, ODD>, 1, smem};
+        if (span > 1024 && span <= 1536) return {layer_norm_kernel<T, 3, 2, FMT, ODD>, 2, smem};
+        if (span > 2048 && span <= 3 * 1024) return {layer_norm_kernel<T, 3, 4, FMT, ODD>, 4, smem};
+        if (span > 4096 && span <= 6144) return {layer_norm_kernel<T, 3, 8, FMT, ODD>, 8, smem};
+        if (span > 8192 && span <= 12288) return {layer_norm_kernel<T, 3, 16, FMT, ODD>, 16, smem};
+    }
     if (span <= 1024) return {layer_norm_kernel<T, 4, 1, FMT, ODD>, 1, smem};
     if (span <= 2048) return {layer_norm_kernel<T, 4, 2, FMT, ODD>, 2, smem};
     if (span <= 4096) return {layer_norm_kernel<T, 4, 4, FMT, ODD>, 4, smem};

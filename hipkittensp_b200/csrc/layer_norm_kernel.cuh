@@ -179,7 +179,7 @@ __device__ __forceinline__ void mx_store8(const float2 (&v)[4], uint8_t* codes_r
 // ---- rows as chunks of 8 elements
 // Rows of whole, aligned chunks (ODD = false) are n = H / 8 chunks.  Other rows are cut at the same 16- or 32-byte boundaries of
 // memory: the row starts `a` elements behind a boundary, its first and last chunk may hold neighbours' elements (which are
-// neither read nor written: those two chunks go element by element), and column `col` is element col + a of the chunks.  `a` is
+// masked when read and never written), and column `col` is element col + a of the chunks.  `a` is
 // the same for rows that lie a multiple of 8 rows apart, so a CTA takes only such rows, its threads own the same columns in each
 // of them, and the parameters are staged once, shifted by a.
 template <bool ODD>
@@ -203,20 +203,42 @@ __device__ __forceinline__ int64_t first_row(int w) {
     if constexpr (ODD) return (blockIdx.x & 7) + 8 * ((int64_t)w + (WARPS == 1 ? 8 : 1) * (int64_t)(blockIdx.x >> 3));
     return WARPS == 1 ? (int64_t)blockIdx.x * 8 + w : blockIdx.x;
 }
-// rowp: the row's first chunk (its start less a elements)
+// Chunk `chunk` of the row whose first chunk starts at element `at` of the matrix m (which may be before its first element).  A chunk
+// at an end of the row is loaded whole, with what it holds of the neighbouring rows, and masked when it is used (loading it
+// element by element would wait for the elements to put them together, a row ahead of their use: 8192 x 4097 bf16 in 95 us);
+// only a row whose chunks reach past the matrix (inner = false) is loaded element by element.
 template <typename T, bool ODD>
-__device__ __forceinline__ void ld_chunk(const T* rowp, int chunk, const Chunks<ODD>& k, Raw<T, 8>& r) {
-    if (k.whole(chunk)) {
-        r = ld_raw<T, 8>(rowp + 8 * chunk);
-    } else if constexpr (ODD) {
-        const int lo = k.lo(chunk), hi = k.hi(chunk);
+__device__ __forceinline__ void ld_chunk(const T* m, int64_t at, bool inner, int chunk, const Chunks<ODD>& k, Raw<T, 8>& r) {
+    if constexpr (!ODD) {
+        if (chunk < k.n) r = ld_raw<T, 8>(m + at + 8 * chunk);
+    } else if (chunk < k.n) {
+        const int64_t e = at + 8 * chunk;
+        if (inner) {
+            r = ld_raw<T, 8>(m + e);
+        } else {
+            const int lo = k.lo(chunk), hi = k.hi(chunk);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            uint32_t u = 0;
-            if (i >= lo && i < hi) u = ld_raw<T, 1>(rowp + 8 * chunk + i).u[0];
-            if constexpr (sizeof(T) == 4) r.u[i] = u;
-            else r.u[i >> 1] = (i & 1) ? r.u[i >> 1] | (u << 16) : u;
+            for (int i = 0; i < 8; ++i) {
+                uint32_t u = 0;
+                if (i >= lo && i < hi) u = ld_raw<T, 1>(m + e + i).u[0];
+                if constexpr (sizeof(T) == 4) r.u[i] = u;
+                else r.u[i >> 1] = (i & 1) ? r.u[i >> 1] | (u << 16) : u;
+            }
         }
+    }
+}
+// zeros for the elements of a chunk that belong to other rows
+template <typename T>
+__device__ __forceinline__ void mask_chunk(const Chunks<true>& k, int chunk, Raw<T, 8>& r) {
+    const int lo = k.lo(chunk), hi = k.hi(chunk);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < lo || i >= hi) r.u[i] = 0;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r.u[i] &= (2 * i >= lo && 2 * i < hi ? 0xffffu : 0u) | (2 * i + 1 >= lo && 2 * i + 1 < hi ? 0xffff0000u : 0u);
     }
 }
 // Parameter vectors in shared memory, as fp32 whatever their type and filled where they are absent: float4 planes of n chunks
@@ -291,12 +313,16 @@ layer_norm_kernel(const LnParams P) {
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
     int64_t row = first_row<ODD, WARPS>(WARPS == 1 ? threadIdx.x >> 5 : 0);
     const Chunks<ODD> K = chunks_of<ODD>(P, row);
-    const T* x = reinterpret_cast<const T*>(P.x) - K.a;
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const int64_t elements = P.rows * P.H;
     Raw<T, 8> raw[C];
     auto load = [&](int64_t r) {
+        if (r < P.rows) {
+            const int64_t at = r * P.H - K.a;
+            const bool inner = at >= 0 && at + 8 * K.n <= elements;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (r < P.rows) ld_chunk<T, ODD>(x + r * P.H, tid + c * TPR, K, raw[c]);
+            for (int c = 0; c < C; ++c) ld_chunk<T, ODD>(x, at, inner, tid + c * TPR, K, raw[c]);
+        }
     };
 #pragma unroll
     for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};           // elements outside the row stay zero
@@ -311,6 +337,11 @@ layer_norm_kernel(const LnParams P) {
     __syncthreads();
     for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
         float2 v[C][4];
+        if constexpr (ODD) {
+            if (edge)
+#pragma unroll
+                for (int c = 0; c < C; ++c) mask_chunk<T>(K, tid + c * TPR, raw[c]);
+        }
 #pragma unroll
         for (int c = 0; c < C; ++c) unpack2<T>(raw[c], v[c]);
         load(row + P.step);
@@ -445,16 +476,19 @@ layer_norm_backward_kernel(const LnParams P) {
     const int tid = WARPS == 1 ? (threadIdx.x & 31) : threadIdx.x;
     int64_t row = first_row<ODD, WARPS>(WARPS == 1 ? threadIdx.x >> 5 : 0);
     const Chunks<ODD> K = chunks_of<ODD>(P, row);
-    const T* x = reinterpret_cast<const T*>(P.x) - K.a;
-    const T* dy = reinterpret_cast<const T*>(P.dy) - K.a;
+    const T* x = reinterpret_cast<const T*>(P.x);
+    const T* dy = reinterpret_cast<const T*>(P.dy);
+    const int64_t elements = P.rows * P.H;
     Raw<T, 8> rx[C], rg[C];
     float mean_n = 0.f, rstd_n = 0.f;
     auto load = [&](int64_t r) {
         if (r < P.rows) {
+            const int64_t at = r * P.H - K.a;
+            const bool inner = at >= 0 && at + 8 * K.n <= elements;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                ld_chunk<T, ODD>(x + r * P.H, tid + c * TPR, K, rx[c]);
-                ld_chunk<T, ODD>(dy + r * P.H, tid + c * TPR, K, rg[c]);
+                ld_chunk<T, ODD>(x, at, inner, tid + c * TPR, K, rx[c]);
+                ld_chunk<T, ODD>(dy, at, inner, tid + c * TPR, K, rg[c]);
             }
             mean_n = __ldcg(P.mean + r);
             rstd_n = __ldcg(P.rstd + r);
@@ -469,10 +503,19 @@ layer_norm_backward_kernel(const LnParams P) {
     }
     load(row);
     stage_param(P.w, P.w_bf16, 1.f, K, prm);
+    bool inside = true;
+#pragma unroll
+    for (int c = 0; c < C; ++c) inside = inside && K.whole(tid + c * TPR);
+    const bool edge = !__all_sync(0xffffffffu, inside);         // (one decision per row, as in the forward kernel)
     __syncthreads();
     for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
         const float mean = mean_n, rstd = rstd_n;
         float2 xh[C][4], g[C][4];
+        if constexpr (ODD) {
+            if (edge)
+#pragma unroll
+                for (int c = 0; c < C; ++c) { mask_chunk<T>(K, tid + c * TPR, rx[c]); mask_chunk<T>(K, tid + c * TPR, rg[c]); }
+        }
 #pragma unroll
         for (int c = 0; c < C; ++c) { unpack2<T>(rx[c], xh[c]); unpack2<T>(rg[c], g[c]); }
         load(row + P.step);
