@@ -305,9 +305,10 @@ static int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Most output tiles a problem may have and still split tiles along K (bounds the counter region).
 constexpr int64_t kMaxSplitTiles = 65536;
 
-// kelems: elements of K per K-block of the kernels (128; 256 on the 4-bit path)
+// kelems: elements of K per K-block of the kernels (128; 256 on the 4-bit path); min_rows: weight rows per CTA from which the
+// even-rows skinny form is taken
 static Plan make_plan(int64_t M, int64_t N, int64_t K, int sm_count, bool allow_pair = true, bool plain = false,
-                      bool even_rows_ok = true, int kelems = 128) {
+                      bool even_rows_ok = true, int kelems = 128, int min_rows = 80) {
     Plan p{};
     p.ctas = 1;
     const Options& o = options();
@@ -361,7 +362,7 @@ static Plan make_plan(int64_t M, int64_t N, int64_t K, int sm_count, bool allow_
             const int64_t rows = ceil_div(N, slots * waves);
             // (measured at K = 8192: 97 rows per CTA, N = 28672, 34.9 against 38.5 us for the K-split form; 49 rows per
             // CTA, N = 14336, 27.7 against 24.5 us: with few rows per CTA the K-split form's parallelism along K wins)
-            if (rows >= 80) { p.streamk = false; p.ctas = 2; p.p_tile = (int)rows; }
+            if (rows >= min_rows) { p.streamk = false; p.ctas = 2; p.p_tile = (int)rows; }
         } else if (!p.swap && wide_rows && p.bn == 256) {
             const int64_t waves = ceil_div(N, (int64_t)sm_count * 256);
             const int64_t rows = (ceil_div(N, (int64_t)sm_count * waves) + 7) / 8 * 8;
@@ -444,11 +445,11 @@ static bool dest_by_tma(const Dest& dst) {
     return ok;
 }
 static Plan plan_for(const void* sfa, const void* sfb, const Dest& dst, int64_t M, int64_t N, int64_t K, int sm_count,
-                     bool requant = false, int kelems = 128) {
+                     bool requant = false, int kelems = 128, int min_rows = 80) {
     // several destinations are written untransposed from whole tiles; a re-quantised result needs tiles that start on
     // multiples of 32 rows and columns
     (void)sfa; (void)sfb; (void)dst;
-    return make_plan(M, N, K, sm_count, true, dst.n > 1, !requant, kelems);
+    return make_plan(M, N, K, sm_count, true, dst.n > 1, !requant, kelems, min_rows);
 }
 
 // Everything a call passes in.  Two calls with equal keys launch the same kernel with the same arguments, so the
@@ -606,7 +607,12 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     const bool sf_tma = scales_by_tma(sfa, sfb, K);
     const bool f4 = fmt_a == MXFP4_E2M1 && fmt_b == MXFP4_E2M1 && o.f4;      // the 4-bit MMA takes two E2M1 operands
     const int kelems = f4 ? 256 : 128;
-    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d.sm_count, q_fmt >= 0, kelems);
+    // 4-bit weights or activations: the even-rows form pays from fewer rows per CTA than for the wider formats (whose rule is left as
+    // it was).  Its time goes with K alone, the K-split form's with N * K; M = 16, even-rows / K-split: 70 rows (N = 20480), K = 8192
+    // 18.2 / 21.0 us for E2M1 x E2M1 and 27.2 / 29.6 us for E4M3 x E2M1; 49 rows, K = 4096 11.5 / 13.5 and 16.2 / 16.3 us;
+    // 49 rows, K = 8192 17.7 / 17.3 and 27.2 / 23.5 us.
+    const int min_rows = fmt_a == MXFP4_E2M1 || fmt_b == MXFP4_E2M1 ? (K <= 4096 ? 48 : 64) : 80;
+    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d.sm_count, q_fmt >= 0, kelems, min_rows);
 
     Recipe r;
     r.key = key;

@@ -97,6 +97,8 @@ PAIRS = [(FP4, FP4), (R.E4M3, FP4), (R.E2M3, FP4), (FP4, R.E5M2), (FP4, R.E3M2)]
 SHAPES = [(1, 28672, 256), (16, 24320, 384), (16, 520, 1024), (17, 384, 640), (33, 200, 128), (64, 24000, 256), (100, 30000, 128), (128, 130, 2048),
           (130, 200, 384), (300, 520, 1152), (384, 768, 512), (1536, 1792, 640), (1111, 2050, 1024), (2048, 2304, 256),
           # rows of C that are not 16-byte multiples, odd and even, in the unswapped single-CTA tiles
+          # even-rows tiles of few rows per CTA, ragged in rows and columns
+          (3, 14400, 512), (16, 19500, 4224), (32, 15001, 1024),
           (300, 1001, 512), (300, 1002, 384), (70, 30001, 128), (520, 1003, 256)]
 
 
