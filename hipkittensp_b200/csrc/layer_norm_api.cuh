@@ -58,8 +58,8 @@ static LnChoice ln_forward_kernel(LnRows rows, int fmt, int H) {
     }
 }
 
-// Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row; bf16 rows of whole chunks up to 16384 keep x and dy
-// in shared memory; the rest (kern = null) goes over its rows again.
+// Backward holds x, dy and both column sums: 16 elements a thread, 8192 a row; bf16 rows up to 16384 keep x and dy in shared
+// memory; the rest (kern = null) goes over its rows again.
 constexpr int kLnBackwardMax = 8192, kLnBackwardWide = 16384;
 static int ln_backward_warps(int span) { return span <= 512 ? 1 : span <= 1024 ? 2 : span <= 2048 ? 4 : span <= 4096 ? 8 : 16; }
 template <typename T, bool ODD>
@@ -78,7 +78,12 @@ static LnChoice ln_backward_choice(int H) {
 }
 template <typename T>
 static LnChoice ln_backward_kernel(LnRows rows, int H) {
-    return rows == kLnApart ? LnChoice{nullptr, 0, 0} : rows == kLnOdd ? ln_backward_choice<T, true>(H) : ln_backward_choice<T, false>(H);
+    if (rows == kLnApart) return {nullptr, 0, 0};
+    const int span = H + (rows == kLnOdd ? 7 : 0);
+    if constexpr (sizeof(T) == 2)
+        if (span > kLnBackwardMax && span <= kLnBackwardWide)
+            return {rows == kLnOdd ? layer_norm_backward_wide_kernel<true> : layer_norm_backward_wide_kernel<false>, 16, 4 * H + 64 + 2 * 2 * 4 * 512 * 16};
+    return rows == kLnOdd ? ln_backward_choice<T, true>(H) : ln_backward_choice<T, false>(H);
 }
 
 // CTAs for `rows` rows at a time (eight rows per CTA when a warp owns one), at most cap, and the step from one of a CTA's rows to
@@ -99,8 +104,14 @@ static int ln_grid(int64_t rows, int warps, bool odd, int64_t cap, int64_t* step
 }
 
 // Number of partial sums per column of the parameter gradients: the grid of the kernel that writes them.
-static int64_t ln_backward_cap(int warps, int sm_count) { return (int64_t)sm_count * (warps == 1 ? 2 : 16 / warps); }      // 512 threads of 128 registers per SM
-static int ln_parts_wide(int64_t rows, int sm_count) { return (int)(rows < sm_count ? rows : sm_count); }
+// At most what is resident (512 threads of 128 registers per SM), and no more than keeps the partials' 8 bytes per column and part
+// at a third of the 6 or 12 bytes per element that the rows move, as long as every SM has a CTA (1500 x 1001 fp32: 562 instead of
+// 1184 parts).
+static int64_t ln_backward_cap(int warps, int sm_count, int64_t rows, int elem_bytes) {
+    const int64_t resident = (int64_t)sm_count * (warps == 1 ? 2 : 16 / warps);
+    const int64_t few = rows * elem_bytes * 3 / 32, least = few > sm_count ? few : sm_count;
+    return least < resident ? least : resident;
+}
 static int ln_parts_columns(int64_t rows, int64_t H, int sm_count) {
     int64_t y = 8 * (int64_t)sm_count / ((H + 255) / 256);
     if (y > (rows + 15) / 16) y = (rows + 15) / 16;
@@ -115,9 +126,9 @@ static int64_t ln_parts_most(int64_t rows, int64_t H, int sm_count) {
         const int64_t span = H + 7 * odd;
         if (span > kLnBackwardMax) continue;
         const int warps = ln_backward_warps((int)span);
-        take(ln_grid(rows, warps, odd != 0, ln_backward_cap(warps, sm_count), &step));
+        take(ln_grid(rows, warps, odd != 0, ln_backward_cap(warps, sm_count, rows, 4), &step));
     }
-    if (H > kLnBackwardMax && H <= kLnBackwardWide) take(ln_parts_wide(rows, sm_count));
+    if (H + 7 > kLnBackwardMax && H <= kLnBackwardWide) take(rows < sm_count ? rows : sm_count);
     return most;
 }
 
@@ -198,13 +209,9 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(place, (int)H) : ln_backward_kernel<__nv_bfloat16>(place, (int)H);
     int parts;
     if (k.kern) {
-        parts = ln_grid(rows, k.warps, place == kLnOdd, ln_backward_cap(k.warps, d->sm_count), &P.step);
+        parts = ln_grid(rows, k.warps, place == kLnOdd, ln_backward_cap(k.warps, d->sm_count, rows, x_dtype == 0 ? 4 : 2), &P.step);
+        if (k.smem > 48 * 1024 && (rc = ensure_smem_attr(*d, (const void*)k.kern, 4 * kLnBackwardWide + 64 + 2 * 2 * 4 * 512 * 16))) return rc;
         if ((rc = launch_pdl(k.kern, (unsigned)parts, (unsigned)(k.warps == 1 ? 256 : 32 * k.warps), (size_t)k.smem, st, P))) return rc;
-    } else if (place == kLnWhole && x_dtype == 1 && H <= kLnBackwardWide) {
-        const int smem = 4 * (int)H + 2 * 2 * 4 * 512 * 16;
-        parts = ln_parts_wide(rows, d->sm_count);
-        if ((rc = ensure_smem_attr(*d, (const void*)layer_norm_backward_wide_kernel, 4 * kLnBackwardWide + 2 * 2 * 4 * 512 * 16))) return rc;
-        if ((rc = launch_pdl(layer_norm_backward_wide_kernel, (unsigned)parts, 512, (size_t)smem, st, P))) return rc;
     } else {
         parts = ln_parts_columns(rows, H, d->sm_count);
         if (sums) {

@@ -461,6 +461,26 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
     }
 }
 
+// a thread's column sums to their places in a vector of H
+template <int C, int TPR, bool ODD>
+__device__ __forceinline__ void st_sums(float* out, int tid, const Chunks<ODD>& k, const float2 (&v)[C][4]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int chunk = tid + c * TPR;
+        float* o = out + 8 * chunk - k.a;
+        if constexpr (ODD) {
+            const float t[8] = {v[c][0].x, v[c][0].y, v[c][1].x, v[c][1].y, v[c][2].x, v[c][2].y, v[c][3].x, v[c][3].y};
+            const int lo = k.lo(chunk), hi = k.hi(chunk);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i >= lo && i < hi) o[i] = t[i];
+        } else if (chunk < k.n) {
+            reinterpret_cast<float4*>(o)[0] = make_float4(v[c][0].x, v[c][0].y, v[c][1].x, v[c][1].y);
+            reinterpret_cast<float4*>(o)[1] = make_float4(v[c][2].x, v[c][2].y, v[c][3].x, v[c][3].y);
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------- backward
 // WARPS warps own a row, C chunks of 8 columns per thread; the same columns of every row, whose parameter gradients the thread
 // sums in registers.  As in the forward kernel the next row is on its way while this one is worked on (without that, HBM idles
@@ -523,9 +543,11 @@ layer_norm_backward_kernel(const LnParams P) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             // (outside the row dy is zero, and so is all that is summed)
+            // (the branch costs nothing here and keeps the registers of fp32 rows down: 16384 x 8192 in 256 us, 279 without it)
             const int chunk = tid + c * TPR;
+            if (chunk >= K.n) continue;
             float2 w[4];
-            ld_staged(prm, K.n, chunk < K.n ? chunk : 0, w);
+            ld_staged(prm, K.n, chunk, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 // (the distance from the mean is taken before the scaling: x * rstd - mean * rstd loses digits of rows far from zero)
@@ -570,31 +592,16 @@ layer_norm_backward_kernel(const LnParams P) {
             }
         }
     } else {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int chunk = tid + c * TPR;
-                float* o = out + (int64_t)k * P.H + 8 * chunk - K.a;
-                const float2 (&v)[4] = k ? db[c] : dw[c];
-                if constexpr (ODD) {
-                    const float t[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-                    const int lo = K.lo(chunk), hi = K.hi(chunk);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i >= lo && i < hi) o[i] = t[i];
-                } else if (chunk < K.n) {
-                    reinterpret_cast<float4*>(o)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-                    reinterpret_cast<float4*>(o)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
-                }
-            }
+st_sums<C, TPR, ODD>(out, tid, K, dw);
+        st_sums<C, TPR, ODD>(out + P.H, tid, K, db);
     }
 }
 
 // bf16 rows of 8192 to 16384 elements: four chunks per thread, whose column sums alone take 64 of its 128 registers.  x and dy of
 // the next two rows are copied by cp.async into slots of shared memory that only this thread reads (no barrier), and both passes
-// over a row read them there (4096 x 16384 in 83 us; passing over global memory again and summing the columns in a kernel of
+// over a row read them there (4096 x 16384 in 81 us; passing over global memory again and summing the columns in a kernel of
 // their own took 311 us).
+template <bool ODD>
 __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const LnParams P) {
     typedef __nv_bfloat16 T;
     constexpr int C = 4, D = 2, TPR = 512, SLOT = TPR * 16;
@@ -602,27 +609,52 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
     extern __shared__ float4 prm[];                             // w, then the slots: [x, dy][row][chunk][thread]
     pdl_launch_dependents();
     pdl_wait();
-    const int tid = threadIdx.x, n8 = P.H >> 3;
+    const int tid = threadIdx.x;
+    int64_t row = blockIdx.x;
+    const Chunks<ODD> K = chunks_of<ODD>(P, row);
     const T* x = reinterpret_cast<const T*>(P.x);
     const T* dy = reinterpret_cast<const T*>(P.dy);
-    const uint32_t sx = smem_u32(prm + 2 * n8) + tid * 16, sg = sx + D * C * SLOT;
+    const int64_t elements = P.rows * P.H;
+    const uint32_t sx = smem_u32(prm + 2 * K.n) + tid * 16, sg = sx + D * C * SLOT;
+    auto put = [&](uint32_t slot, const Raw<T, 8>& r) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(slot), "r"(r.u[0]), "r"(r.u[1]), "r"(r.u[2]), "r"(r.u[3]) : "memory");
+    };
+    auto get = [&](uint32_t slot) {
+        Raw<T, 8> r;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"(slot) : "memory");
+        return r;
+    };
     // columns past H are never copied and stay zero
 #pragma unroll
-    for (int i = 0; i < 2 * D * C; ++i) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sx + i * SLOT), "r"(0) : "memory");
+    for (int i = 0; i < 2 * D * C; ++i) put(sx + i * SLOT, Raw<T, 8>{});
     auto load = [&](int d, int64_t r) {
+        if (r < P.rows) {
+            const int64_t at = r * P.H - K.a;
+            const bool inner = at >= 0 && at + 8 * K.n <= elements;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int chunk = tid + c * TPR;
-            if (r < P.rows && chunk < n8) {
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sx + (d * C + c) * SLOT), "l"(x + r * P.H + 8 * chunk) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sg + (d * C + c) * SLOT), "l"(dy + r * P.H + 8 * chunk) : "memory");
+            for (int c = 0; c < C; ++c) {
+                const int chunk = tid + c * TPR;
+                const uint32_t px = sx + (d * C + c) * SLOT, pg = sg + (d * C + c) * SLOT;
+                if (chunk >= K.n) continue;
+                if (!ODD || inner) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(px), "l"(x + at + 8 * chunk) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(pg), "l"(dy + at + 8 * chunk) : "memory");
+                } else {
+                    Raw<T, 8> t{};
+                    ld_chunk<T, ODD>(x, at, false, chunk, K, t);
+                    put(px, t);
+                    ld_chunk<T, ODD>(dy, at, false, chunk, K, t);
+                    put(pg, t);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto take = [&](uint32_t slot, float2 (&v)[4]) {
-        Raw<T, 8> r;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"(slot) : "memory");
+    auto take = [&](uint32_t slot, int chunk, float2 (&v)[4]) {
+        Raw<T, 8> r = get(slot);
+        if constexpr (ODD) {
+            if (!K.whole(chunk)) mask_chunk<T>(K, chunk, r);
+        }
         unpack2<T>(r, v);
     };
     float2 dw[C][4], db[C][4];
@@ -630,28 +662,27 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) dw[c][i] = db[c][i] = make_float2(0.f, 0.f);
-    int64_t row = blockIdx.x;
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(d, row + (int64_t)d * gridDim.x);
+    for (int d = 0; d < D; ++d) load(d, row + d * P.step);
     float mean_n = 0.f, rstd_n = 0.f;
     if (row < P.rows) { mean_n = __ldcg(P.mean + row); rstd_n = __ldcg(P.rstd + row); }
-    stage_param(P.w, P.w_bf16, 1.f, Chunks<false>{0, n8, P.H}, prm);
+    stage_param(P.w, P.w_bf16, 1.f, K, prm);
     __syncthreads();
-    for (int par = 0; row < P.rows; row += gridDim.x, par ^= 1) {
+    for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
         static_assert(D == 2, "the slot alternates with the parity of the reduction");
         const float mean = mean_n, rstd = rstd_n;
-        const int64_t next = row + gridDim.x;
+        const int64_t next = row + P.step;
         if (next < P.rows) { mean_n = __ldcg(P.mean + next); rstd_n = __ldcg(P.rstd + next); }
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
         float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            // (threads past H: dy is zero there, and so is all that is summed)
             const int chunk = tid + c * TPR;
+            if (chunk >= K.n) continue;
             float2 xh[4], g[4], w[4];
-            take(sx + (par * C + c) * SLOT, xh);
-            take(sg + (par * C + c) * SLOT, g);
-            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
+            take(sx + (par * C + c) * SLOT, chunk, xh);
+            take(sg + (par * C + c) * SLOT, chunk, g);
+            ld_staged(prm, K.n, chunk, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 xh[i] = __fmul2_rn(__fadd2_rn(xh[i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
@@ -668,35 +699,26 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
+            if (chunk >= K.n) continue;
             float2 xh[4], g[4], w[4];
-            take(sx + (par * C + c) * SLOT, xh);
-            take(sg + (par * C + c) * SLOT, g);
-            ld_staged(prm, n8, chunk < n8 ? chunk : 0, w);
+            take(sx + (par * C + c) * SLOT, chunk, xh);
+            take(sg + (par * C + c) * SLOT, chunk, g);
+            ld_staged(prm, K.n, chunk, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 xh[i] = __fmul2_rn(__fadd2_rn(xh[i], make_float2(-mean, -mean)), make_float2(rstd, rstd));
                 g[i] = __fmul2_rn(g[i], w[i]);
                 g[i] = __fmul2_rn(__fadd2_rn(g[i], __ffma2_rn(xh[i], make_float2(m2, m2), make_float2(m1, m1))), make_float2(rstd, rstd));
             }
-            if (chunk < n8) st_row2<T>(reinterpret_cast<T*>(P.y) + row * P.H + 8 * chunk, g);
+            st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, g);
         }
-        load(par, row + (int64_t)D * gridDim.x);                // the slots of this row have been read
+        load(par, row + D * P.step);                            // the slots of this row have been read
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!P.part) return;
     float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int chunk = tid + c * TPR;
-        if (chunk < n8) {
-            float4* o = reinterpret_cast<float4*>(out + 8 * chunk);
-            o[0] = make_float4(dw[c][0].x, dw[c][0].y, dw[c][1].x, dw[c][1].y);
-            o[1] = make_float4(dw[c][2].x, dw[c][2].y, dw[c][3].x, dw[c][3].y);
-            o = reinterpret_cast<float4*>(out + P.H + 8 * chunk);
-            o[0] = make_float4(db[c][0].x, db[c][0].y, db[c][1].x, db[c][1].y);
-            o[1] = make_float4(db[c][2].x, db[c][2].y, db[c][3].x, db[c][3].y);
-        }
-    }
+    st_sums<C, TPR, ODD>(out, tid, K, dw);
+    st_sums<C, TPR, ODD>(out + P.H, tid, K, db);
 }
 
 // Rows longer than a CTA's registers hold: dx with a second pass over the row, and the parameter gradients by a kernel whose
