@@ -98,23 +98,22 @@ __device__ __forceinline__ int quant_block32_amax(const float* v, float amax, ui
     // 2^-e, -127 <= -e <= 127, is an fp32 value (2^-127 a subnormal one) and the product with an element of the
     // block is exact: |x| * 2^-e < 2^(emax+1)
     const float f = e == 127 ? __uint_as_float(0x00400000u) : __uint_as_float((uint32_t)(127 - e) << 23);
+    float s[32];                                   // products two at a time
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const float2 t = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(f, f));
+        s[i] = t.x; s[i + 1] = t.y;
+    }
     if constexpr (FMT == kE4M3 || FMT == kE5M2) {
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-            out[g] = cvt_quad<FMT>(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+        for (int g = 0; g < 8; ++g) out[g] = cvt_quad<FMT>(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
     } else if constexpr (FMT == kE2M1) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float s[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] = v[8 * g + i] * f;
-            out[g] = cvt_oct_e2m1(s);
-        }
+        for (int g = 0; g < 4; ++g) out[g] = cvt_oct_e2m1(s + 8 * g);
     } else {
         uint32_t w24[8];
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-            w24[g] = cvt_quad<FMT>(v[4 * g] * f, v[4 * g + 1] * f, v[4 * g + 2] * f, v[4 * g + 3] * f);
+        for (int g = 0; g < 8; ++g) w24[g] = cvt_quad<FMT>(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
 #pragma unroll
         for (int h4 = 0; h4 < 2; ++h4) {      // 4 x 24 bits -> 3 words, twice
             const uint32_t* q = w24 + 4 * h4;
