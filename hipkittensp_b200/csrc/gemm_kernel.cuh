@@ -97,9 +97,9 @@ struct GemmParams {
 template <bool SWAP>
 __device__ __forceinline__ float affine_one(const GemmParams& P, float x, int p, int q) {
     const int m = SWAP ? q : p, n = SWAP ? p : q;
-    const float sn = (P.scale_n && n < P.c_cols) ? __ldg(P.scale_n + n) : 1.f;
-    const float sm = (P.scale_m && m < P.c_rows) ? __ldg(P.scale_m + m) : 1.f;
-    const float bn = (P.bias_n && n < P.c_cols) ? __ldg(P.bias_n + n) : 0.f;
+    const float sn = (P.scale_n && n < P.c_cols) ? __ldcg(P.scale_n + n) : 1.f;
+    const float sm = (P.scale_m && m < P.c_rows) ? __ldcg(P.scale_m + m) : 1.f;
+    const float bn = (P.bias_n && n < P.c_cols) ? __ldcg(P.bias_n + n) : 0.f;
     return __fadd_rn(__fmul_rn(__fmul_rn(x, sn), sm), bn);
 }
 
@@ -113,30 +113,30 @@ __device__ __forceinline__ void affine_chunk(const GemmParams& P, uint32_t (&v)[
     if (SWAP) {
         // p is the column of C: one scale and one bias for the whole chunk; the row scale varies along it
         const bool in = p < P.c_cols;
-        const float sn = (P.scale_n && in) ? __ldg(P.scale_n + p) : 1.f;
-        const float bn = (P.bias_n && in) ? __ldg(P.bias_n + p) : 0.f;
+        const float sn = (P.scale_n && in) ? __ldcg(P.scale_n + p) : 1.f;
+        const float bn = (P.bias_n && in) ? __ldcg(P.bias_n + p) : 0.f;
 #pragma unroll
         for (int i = 0; i < CW; ++i) {
-            const float sm = (P.scale_m && q0 + i < P.c_rows) ? __ldg(P.scale_m + q0 + i) : 1.f;
+            const float sm = (P.scale_m && q0 + i < P.c_rows) ? __ldcg(P.scale_m + q0 + i) : 1.f;
             v[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(__uint_as_float(v[i]), sn), sm), bn));
         }
     } else {
-        const float sm = (P.scale_m && p < P.c_rows) ? __ldg(P.scale_m + p) : 1.f;
+        const float sm = (P.scale_m && p < P.c_rows) ? __ldcg(P.scale_m + p) : 1.f;
         const bool whole = q0 + CW <= P.c_cols;     // q0 is a multiple of 16 and the vectors are 16-byte aligned
 #pragma unroll
         for (int i = 0; i < CW; i += 4) {
             float4 sn = make_float4(1.f, 1.f, 1.f, 1.f), bn = make_float4(0.f, 0.f, 0.f, 0.f);
             if (whole) {
-                if (P.scale_n) sn = __ldg(reinterpret_cast<const float4*>(P.scale_n + q0 + i));
-                if (P.bias_n) bn = __ldg(reinterpret_cast<const float4*>(P.bias_n + q0 + i));
+                if (P.scale_n) sn = __ldcg(reinterpret_cast<const float4*>(P.scale_n + q0 + i));
+                if (P.bias_n) bn = __ldcg(reinterpret_cast<const float4*>(P.bias_n + q0 + i));
             } else {
                 float* s4 = reinterpret_cast<float*>(&sn);
                 float* b4 = reinterpret_cast<float*>(&bn);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (q0 + i + e < P.c_cols) {
-                        if (P.scale_n) s4[e] = __ldg(P.scale_n + q0 + i + e);
-                        if (P.bias_n) b4[e] = __ldg(P.bias_n + q0 + i + e);
+                        if (P.scale_n) s4[e] = __ldcg(P.scale_n + q0 + i + e);
+                        if (P.bias_n) b4[e] = __ldcg(P.bias_n + q0 + i + e);
                     }
                 }
             }
@@ -656,7 +656,7 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                             const bool is_p = i < 16;
                             const int row = is_p ? sg.p0 + ridx : sg.q0 + ridx - 128;
                             const bool live = row < (is_p ? P.p_rows : P.q_rows) && kb4 + w < P.sf_words;
-                            v[i] = live ? __ldg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + (kb4 + w) * 4)) : 0u;
+                            v[i] = live ? __ldcg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + (kb4 + w) * 4)) : 0u;
                         }
                         const int g = n_grp % Cfg::ATOM_GROUPS;
                         ok = wait_bar_warp(bar_atom_empty(g), ((n_grp / Cfg::ATOM_GROUPS) & 1) ^ 1, abort_flag, P, kStatusTimeoutScale);
@@ -715,13 +715,13 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
             // fetched while the accumulator is still being computed, then shared through shared memory
             float row_scale = 1.f, cs[2] = {1.f, 1.f}, cb[2] = {0.f, 0.f};
             if (!Cfg::SWAP && affine) {
-                if (P.scale_m && sg.p0 + prow < P.c_rows) row_scale = __ldg(P.scale_m + sg.p0 + prow);
+                if (P.scale_m && sg.p0 + prow < P.c_rows) row_scale = __ldcg(P.scale_m + sg.p0 + prow);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int c = sg.q0 + etid + 128 * h;
                     if (etid + 128 * h < BN && c < P.c_cols) {
-                        if (P.scale_n) cs[h] = __ldg(P.scale_n + c);
-                        if (P.bias_n) cb[h] = __ldg(P.bias_n + c);
+                        if (P.scale_n) cs[h] = __ldcg(P.scale_n + c);
+                        if (P.bias_n) cb[h] = __ldcg(P.bias_n + c);
                     }
                 }
             }

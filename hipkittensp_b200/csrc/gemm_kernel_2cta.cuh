@@ -349,7 +349,7 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                         const bool is_p = i < 16;
                         const int row = is_p ? p0 + 128 * (int)rank + ridx : q0 + ridx - 128;
                         const bool live = row < (is_p ? P.p_rows : P.q_rows) && w < P.sf_words;
-                        v[i] = live ? __ldg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + w * 4)) : 0u;
+                        v[i] = live ? __ldcg(reinterpret_cast<const uint32_t*>((is_p ? P.sfp : P.sfq) + (size_t)row * P.sf_ld + w * 4)) : 0u;
                     }
                     const int g = n_grp % Cfg::ATOM_GROUPS;
                     ok = wait_bar_warp(bar_atom_empty(g), ((n_grp / Cfg::ATOM_GROUPS) & 1) ^ 1, abort_flag, P, kStatusTimeoutScale);
@@ -405,9 +405,9 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
             float2 col_scale = make_float2(1.f, 1.f), col_bias = make_float2(0.f, 0.f);
             if (affine) {
                 const int c = q0 + 2 * etid;
-                if (P.scale_m && my_p0 + prow < P.c_rows) row_scale = __ldg(P.scale_m + my_p0 + prow);
-                if (P.scale_n) { if (c < P.c_cols) col_scale.x = __ldg(P.scale_n + c); if (c + 1 < P.c_cols) col_scale.y = __ldg(P.scale_n + c + 1); }
-                if (P.bias_n) { if (c < P.c_cols) col_bias.x = __ldg(P.bias_n + c); if (c + 1 < P.c_cols) col_bias.y = __ldg(P.bias_n + c + 1); }
+                if (P.scale_m && my_p0 + prow < P.c_rows) row_scale = __ldcg(P.scale_m + my_p0 + prow);
+                if (P.scale_n) { if (c < P.c_cols) col_scale.x = __ldcg(P.scale_n + c); if (c + 1 < P.c_cols) col_scale.y = __ldcg(P.scale_n + c + 1); }
+                if (P.bias_n) { if (c < P.c_cols) col_bias.x = __ldcg(P.bias_n + c); if (c + 1 < P.c_cols) col_bias.y = __ldcg(P.bias_n + c + 1); }
             }
             ok = epilogue_all(wait_bar_warp(bar_acc_full(b), (n_seg >> 1) & 1, abort_flag, P, kStatusTimeoutEpilogue));
             if (!ok) break;

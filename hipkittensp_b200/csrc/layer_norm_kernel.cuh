@@ -42,8 +42,7 @@ struct LnParams {
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// V consecutive elements as they lie in memory (V = 8: one 16- or 32-byte load; V = 1: any alignment).  Data of the row
-// matrices goes past L1, which keeps the weights.
+// V consecutive elements as they lie in memory (V = 8: one 16- or 32-byte load; V = 1: any alignment), not kept in L1.
 template <typename T, int V> struct Raw { uint32_t u[V == 8 ? (sizeof(T) == 4 ? 8 : 4) : 1]; };
 
 template <typename T, int V>
@@ -89,7 +88,8 @@ __device__ __forceinline__ void st_row(T* p, const float (&v)[V]) {
         *p = __float2bfloat16_rn(v[0]);
     }
 }
-// V elements of a parameter vector (fill where there is none)
+// V elements of a parameter vector (fill where there is none), from L2: under programmatic dependent launch an L1 line may be older
+// than the preceding kernel's writes
 template <int V>
 __device__ __forceinline__ void ld_param(const void* w, int is_bf16, int col, float fill, float (&v)[V]) {
     if (!w) {
@@ -98,20 +98,20 @@ __device__ __forceinline__ void ld_param(const void* w, int is_bf16, int col, fl
     } else if (is_bf16) {
         const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(w) + col;
         if constexpr (V == 8) {
-            const uint4 q = *reinterpret_cast<const uint4*>(p);
+            const uint4 q = __ldcg(reinterpret_cast<const uint4*>(p));
             const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(u[i]); v[2 * i + 1] = bf16_hi(u[i]); }
         } else {
-            v[0] = __bfloat162float(*p);
+            v[0] = bf16_lo(__ldcg(reinterpret_cast<const unsigned short*>(p)));
         }
     } else {
         const float* p = reinterpret_cast<const float*>(w) + col;
         if constexpr (V == 8) {
-            const float4 a = *reinterpret_cast<const float4*>(p), c = *reinterpret_cast<const float4*>(p + 4);
+            const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), c = __ldcg(reinterpret_cast<const float4*>(p + 4));
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
         } else {
-            v[0] = *p;
+            v[0] = __ldcg(p);
         }
     }
 }
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const Ln
     for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x, par ^= 1) {
         const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
         const T* dy = reinterpret_cast<const T*>(P.dy) + row * P.H;
-        const float mean = P.mean[row], rstd = P.rstd[row];
+        const float mean = __ldcg(P.mean + row), rstd = __ldcg(P.rstd + row);
         float s[2] = {0.f, 0.f};
         for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
             float v[V], g[V], w[V];
@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const LnParams 
         float v[1], g[1];
         unpack<T, 1>(ld_raw<T, 1>(x + r * P.H + col), v);
         unpack<T, 1>(ld_raw<T, 1>(dy + r * P.H + col), g);
-        dw = fmaf(g[0], (v[0] - P.mean[r]) * P.rstd[r], dw);
+        dw = fmaf(g[0], (v[0] - __ldcg(P.mean + r)) * __ldcg(P.rstd + r), dw);
         db += g[0];
     }
     float* out = P.part + (int64_t)blockIdx.y * 2 * P.H;

@@ -37,6 +37,16 @@ static int fail(int code, const char* fmt, ...) {
     g_err = buf;
     return code;
 }
+// No C++ exception leaves a C entry point (the tables of kernels and tensor maps allocate).
+template <typename F>
+static int guarded(F body) noexcept {
+    try {
+        return body();
+    } catch (...) {
+        try { g_err = "out of host memory"; } catch (...) {}
+        return MXFP6_ERR_CUDA;
+    }
+}
 #define CUDA_TRY(expr)                                                                              \
     do {                                                                                            \
         cudaError_t e_ = (expr);                                                                    \
@@ -1220,8 +1230,8 @@ static int launch_dequantize(DeviceState& d, const uint8_t* packed, const uint8_
     return launch_pdl(vec ? dequantize_kernel<F, T, true> : dequantize_kernel<F, T, false>, (unsigned)blocks, 256, 0, st, packed, scales, n_oct, out);
 }
 
-extern "C" int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out,
-                                   int out_dtype, void* stream) {
+static int dequantize_impl(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out,
+                           int out_dtype, void* stream) {
     if (rows < 0 || K < 0 || K % 32) return fail(MXFP6_ERR_BAD_ARG, "dequantize: rows=%lld K=%lld (K must be a multiple of 32)", (long long)rows, (long long)K);
     if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "dequantize: bad format %d", fmt);
     if (out_dtype != 0 && out_dtype != 1) return fail(MXFP6_ERR_BAD_ARG, "dequantize: out_dtype must be 0 (fp32) or 1 (bf16)");
@@ -1245,20 +1255,27 @@ extern "C" int mxfp6_dequantize_ex(const void* packed, const void* scales, int64
 #undef DQ
 }
 
+extern "C" int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out, int out_dtype,
+                                   void* stream) {
+    return guarded([&] { return dequantize_impl(packed, scales, rows, K, fmt, out, out_dtype, stream); });
+}
+
 extern "C" int mxfp6_dequantize(const void* packed, const void* scales, int64_t rows, int64_t K, int fmt, void* out_f32, void* stream) {
     return mxfp6_dequantize_ex(packed, scales, rows, K, fmt, out_f32, 0, stream);
 }
 
 extern "C" int mxfp6_layer_norm(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, void* y,
                                 float* mean, float* rstd, int64_t rows, int64_t H, float eps, void* stream) {
-    return ln_forward("layer_norm", x, x_dtype, weight, bias, w_dtype, y, -1, nullptr, nullptr, mean, rstd, rows, H, eps, stream);
+    return guarded([&] { return ln_forward("layer_norm", x, x_dtype, weight, bias, w_dtype, y, -1, nullptr, nullptr, mean, rstd, rows, H, eps, stream); });
 }
 
 extern "C" int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, int fmt,
                                          void* packed, void* scales, float* mean, float* rstd, int64_t rows, int64_t H, float eps,
                                          void* stream) {
-    if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "layer_norm_quantize: bad format %d", fmt);
-    return ln_forward("layer_norm_quantize", x, x_dtype, weight, bias, w_dtype, nullptr, fmt, packed, scales, mean, rstd, rows, H, eps, stream);
+    return guarded([&] {
+        if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "layer_norm_quantize: bad format %d", fmt);
+        return ln_forward("layer_norm_quantize", x, x_dtype, weight, bias, w_dtype, nullptr, fmt, packed, scales, mean, rstd, rows, H, eps, stream);
+    });
 }
 
 extern "C" size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H) {
@@ -1271,7 +1288,7 @@ extern "C" size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_
 extern "C" int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,
                                          const void* weight, int w_dtype, void* dx, float* dweight, float* dbias, int64_t rows,
                                          int64_t H, void* workspace, size_t workspace_bytes, void* stream) {
-    return ln_backward(dy, x, x_dtype, mean, rstd, weight, w_dtype, dx, dweight, dbias, rows, H, workspace, workspace_bytes, stream);
+    return guarded([&] { return ln_backward(dy, x, x_dtype, mean, rstd, weight, w_dtype, dx, dweight, dbias, rows, H, workspace, workspace_bytes, stream); });
 }
 
 extern "C" int mxfp6_device_status(int* status_out) {

@@ -44,7 +44,8 @@ extern "C" {
 #define MXFP8_E5M2 3
 /* MX-FP4 operands (E2M1: +-0, 0.5, 1, 1.5, 2, 3, 4, 6): two codes per byte, the lower element in the low nibble, row-major
  * [rows, K/2], 32-byte aligned, same E8M0 scale per 32 elements.  Every entry point that takes a format takes this one.
- * The nibbles are spread to 8-bit slots on the way into shared memory and multiplied by kind::mxf8f6f4.
+ * A and B both E2M1: the products run on the 4-bit tensor-core path (kind::mxf4, K = 64 per instruction); mixed with a wider
+ * format the nibbles are spread to 8-bit slots on the way into shared memory and multiplied by kind::mxf8f6f4.
  * (No counterpart in the reference.) */
 #define MXFP4_E2M1 4
 
@@ -192,7 +193,8 @@ int mxfp6_gemm_noalloc(const void* a, const void* sfa, const void* b, const void
 /*
  * Block quantiser: src [rows, K] (src_dtype 0 = fp32, 1 = bf16), K % 32 == 0  ->
  * packed [rows, 3K/4] (fp6), [rows, K] (fp8) or [rows, K/2] (fp4) + scales [rows, K/32].  Scale exponent = floor(log2(amax)) - 2
- * (E2M3, E2M1), - 4 (E3M2), - 8 (E4M3) or - 15 (E5M2); elements rounded to nearest even and saturated.  The step in front of the GEMM; the
+ * (E2M3, E2M1), - 4 (E3M2), - 8 (E4M3) or - 15 (E5M2); elements rounded to nearest even and saturated (a NaN does not count
+ * towards amax and is stored as the largest magnitude).  The step in front of the GEMM; the
  * reference's fp8 harness does it on the host (kernels/gemm/fp8fp32/FP8_8wave/8_wave.cu:258-268).
  */
 int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt,
@@ -210,12 +212,12 @@ int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, in
  *     mean = sum(x) / H,  rstd = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) * rstd * weight + bias
  * with all arithmetic in fp32 and one rounding of y to x's type.  weight and bias are [H] vectors of w_dtype (0 = fp32,
  * 1 = bf16); either may be NULL (ones / zeros).  mean and rstd are fp32 [rows], kept for the backward pass; either may be
- * NULL.  y may be x itself.  Any H >= 1 and any pointers aligned to their type; 16-byte (bf16) or 32-byte (fp32) aligned rows
- * take the vector path.
+ * NULL.  y may be x itself.  Any H >= 1 and any pointers aligned to their type; x and y that start at the same place of a 16-byte
+ * (bf16) or 32-byte (fp32) unit of memory take the vector paths, others are passed over element by element.
  *
  * The _quantize form delivers y as an MX operand instead (blocks of 32 along H: the K of the product that follows), rounded
  * once from fp32 with the rule of mxfp6_quantize: packed [rows, H/2 | 3H/4 | H] codes and scales [rows, H/32].  H % 32 == 0;
- * x aligned as for the vector path, weight, bias and packed to 16 bytes.
+ * x 16-byte (bf16) or 32-byte (fp32) aligned, weight, bias and packed 16-byte.
  * (Stands next to the reference's fused norm, kernels/layernorm/kernel.cpp, which has neither statistics nor a gradient.)
  */
 int mxfp6_layer_norm(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, void* y,
@@ -229,10 +231,11 @@ int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, co
  * xhat = (x - mean) * rstd and g = dy * weight:
  *     dx = (g - sum(g) / H - xhat * sum(g * xhat) / H) * rstd
  *     dweight = sum over rows(dy * xhat),  dbias = sum over rows(dy)       (fp32 [H] each; either may be NULL)
+ * Any H >= 1 and any pointers aligned to their type, as in the forward pass.
  * The sums over the rows go through per-CTA partials in `workspace` (at least the given number of bytes, 16-byte aligned, owned
  * by this call until the stream has passed it; any contents; not needed when dweight and dbias are both NULL) and are added
  * in a fixed order: equal calls on a device give equal bits.  Two calls that may overlap need a workspace each.
- * rows = 0 gives zero parameter gradients.  (No counterpart in the reference.)
+ * rows = 0 gives zero parameter gradients.  dx may be dy or x itself.  (No counterpart in the reference.)
  */
 size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H);
 int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,

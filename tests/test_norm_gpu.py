@@ -267,6 +267,30 @@ def test_backward_of_no_rows_and_unaligned_rows():
     _check_backward(dy, x, mean, rstd, w, *hk.layer_norm_backward(ys, x, mean, rstd, w))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,H", [(70, 512), (70, 1003), (40, 9000), (40, 9001), (20, 20000)])
+def test_backward_in_place(rows, H, dtype):
+    """dx may be dy or x: the same bits as with a buffer of its own."""
+    x, w, b, dy = _inputs(rows, H, dtype)
+    _, mean, rstd = hk.layer_norm(x, w, b)
+    want = hk.layer_norm_backward(dy, x, mean, rstd, w)
+    code = 0 if dtype == torch.float32 else 1
+    nbytes = hk.lib.mxfp6_layer_norm_backward_workspace_bytes(rows, H)
+    for which in (0, 1):
+        xs, gs = x.clone(), dy.clone()
+        dx = (gs, xs)[which]
+        dw, db, work = torch.empty(H, device=DEV), torch.empty(H, device=DEV), torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+        rc = hk.lib.mxfp6_layer_norm_backward(gs.data_ptr(), xs.data_ptr(), code, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), code, dx.data_ptr(),
+                                              dw.data_ptr(), db.data_ptr(), rows, H, work.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, hk.lib.mxfp6_last_error()
+        for got, ref in zip((dx, dw, db), want):
+            assert torch.equal(got, ref)
+        # without the sums no workspace is asked for
+        rc = hk.lib.mxfp6_layer_norm_backward(dy.data_ptr(), x.data_ptr(), code, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), code, dx.data_ptr(),
+                                              None, None, rows, H, None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(dx, want[0])
+
+
 def test_backward_against_differences():
     """d/dx, d/dw and d/db of sum(dy * y) by central differences of the 64-bit formula, at a few places."""
     rows, H, eps = 5, 40, 1e-5
