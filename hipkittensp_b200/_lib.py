@@ -96,6 +96,21 @@ def _load() -> ctypes.CDLL:
 lib = _load()
 
 
+def _load_ops():
+    """The compiled tensor-level wrappers, bound to the library instance loaded above."""
+    import torch  # noqa: F401  -- the extension links against torch's libraries
+
+    try:
+        from . import _torch_ops
+    except ImportError as e:
+        raise ImportError(f"the _torch_ops extension is missing or does not load ({e}): build it with `python hipkittensp_b200/build.py`") from e
+    _torch_ops.bind(lib._handle, Mxfp6Error)
+    return _torch_ops
+
+
+ops = _load_ops()
+
+
 def check(rc: int) -> None:
     if rc != OK:
         raise Mxfp6Error(rc, lib.mxfp6_last_error().decode())

@@ -1,5 +1,5 @@
 """In-tree build of the native parts: libmxfp6.so (CUDA kernels + C ABI, sm_100a), the stand-alone C++ harness
-matmul_host, and the
+matmul_host, the tensor-level wrappers _torch_ops, and the
 tk_kernel Python extension (pybind11, same module/function names as the reference's binding,
 include/pyutils/pyutils.cuh:55-72 and kernels/gemm/bf16fp32/Makefile:41,51-52).
 
@@ -72,6 +72,31 @@ def build_ext(force: bool = False) -> str:
     return EXT
 
 
+OPS = os.path.join(PKG, "_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def build_torch_ops(force: bool = False) -> str:
+    """The tensor-level wrappers of gemm.py and norm.py (links torch; finds the library's entry points at import)."""
+    import importlib.util
+
+    import pybind11
+
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    if not force and _newer(OPS, [src, os.path.join(ROOT, "include", "mxfp6.h")]):
+        return OPS
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    torch_lib = os.path.join(torch_dir, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           "-I", pybind11.get_include(), "-I", sysconfig.get_paths()["include"], "-I", os.path.join(ROOT, "include"),
+           "-I", os.path.join(torch_dir, "include"), "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(CUDA_HOME, "include"), src, "-o", OPS, "-L", torch_lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+           "-lc10_cuda", "-ltorch_cuda", "-ldl", "-Wl,-rpath," + torch_lib]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
+    return OPS
+
+
 HOST = os.path.join(PKG, "matmul_host")
 
 
@@ -90,7 +115,7 @@ def build_host(force: bool = False) -> str:
 
 
 def build_all(force: bool = False, verbose: bool = False):
-    return build_lib(force, verbose), build_ext(force), build_host(force)
+    return build_lib(force, verbose), build_ext(force), build_host(force), build_torch_ops(force)
 
 
 if __name__ == "__main__":

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import E2M1, E2M3, E3M2, E4M3, E5M2, check, lib
+from ._lib import E2M1, E2M3, E3M2, E4M3, E5M2, check, lib, ops
 
 
 def _accept(t, name: str, dtype) -> None:
@@ -200,77 +200,25 @@ def gemm_scaled(A, scale_A, B, scale_B, row_scale=None, col_scale=None, bias=Non
     """C[m,n] = bf16((acc[m,n] * col_scale[n]) * row_scale[m] + bias[n]) with fp32 vectors row_scale [M], col_scale [N],
     bias [N] (any may be None), applied in the GEMM epilogue: the per-row / per-column scaling of the reference's
     scaled_matmul (kernels/torch_scaled/scaled_matmul.cu:253-265) on top of the MX block scales."""
-    _accept(A, "A", torch.uint8)
-    _accept(B, "B", torch.uint8)
-    _accept(scale_A, "scale_A", torch.uint8)
-    _accept(scale_B, "scale_B", torch.uint8)
-    fb = fmt if fmt_b is None else fmt_b
-    M, N, K = A.shape[0], B.shape[0], _k_of(A, fmt, "A")
-    if _k_of(B, fb, "B") != K:
-        raise RuntimeError("A and B disagree on K")
-    _check_scales(A, B, scale_A, scale_B, K)
-    for name, v, n in (("row_scale", row_scale, M), ("col_scale", col_scale, N), ("bias", bias, N)):
-        if v is not None:
-            if not isinstance(v, torch.Tensor) or v.dtype != torch.float32 or not v.is_contiguous():
-                raise RuntimeError(f"{name} must be a contiguous fp32 tensor")
-            if v.device != A.device:
-                raise RuntimeError("Tensor must be on CUDA device")
-            if v.numel() != n:
-                raise RuntimeError(f"{name} must have {n} elements, has {v.numel()}")
-    if out is None:
-        out = A.new_empty((M, N), dtype=torch.bfloat16)
-    _accept(out, "C", torch.bfloat16)
-    if tuple(out.shape) != (M, N):
-        raise RuntimeError(f"C must be [{M}, {N}]")
-    if out.get_device() != A.get_device():
-        raise RuntimeError("all tensors must be on the same device")
-    ptr = lambda v: 0 if v is None else v.data_ptr()
-    _launch(A, lib.mxfp6_gemm_scaled, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
-            ptr(row_scale), ptr(col_scale), ptr(bias), M, N, K, fmt, fb)
-    return out
+    return ops.gemm_scaled(A, scale_A, B, scale_B, row_scale, col_scale, bias, fmt, fmt if fmt_b is None else fmt_b, out)
 
 
 def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=None):
-    """Allocating convenience wrapper around dispatch_micro; returns C."""
-    M, N = A.shape[0], B.shape[0]
-    if out is None:
-        out = A.new_empty((M, N), dtype=torch.bfloat16)
-    dispatch_micro(A, B, out, scale_A, scale_B, fmt, fmt_b)
-    return out
+    """The product of dispatch_micro with its result allocated here (unless given as `out`); returns C."""
+    return ops.gemm(A, scale_A, B, scale_B, fmt, fmt if fmt_b is None else fmt_b, out, 0)
 
 
 def quantize(x: torch.Tensor, fmt: int = E2M3):
     """fp32 or bf16 [rows,K] on the GPU -> (operand bytes u8 [rows,3K/4] for fp6 / [rows,K] for fp8 / [rows,K/2] for fp4,
     scales u8 [rows,K/32])."""
-    if not x.is_cuda:
-        raise RuntimeError("Tensor must be on CUDA device")
-    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() != 2 or not x.is_contiguous():
-        raise RuntimeError("quantize expects a contiguous 2-D fp32 or bf16 tensor")
-    rows, K = x.shape
-    if K % 32:
-        raise RuntimeError("K must be a multiple of 32")
-    packed = x.new_empty((rows, row_bytes(K, fmt)), dtype=torch.uint8)
-    scales = x.new_empty((rows, K // 32), dtype=torch.uint8)
-    _launch(x, lib.mxfp6_quantize, x.data_ptr(), 0 if x.dtype == torch.float32 else 1, rows, K, fmt,
-            packed.data_ptr(), scales.data_ptr())
-    return packed, scales
+    return ops.quantize(x, fmt)
 
 
 def dequantize(packed: torch.Tensor, scales: torch.Tensor, fmt: int = E2M3, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """(packed, scales) on the GPU -> fp32 or bf16 [rows,K]."""
-    _accept(packed, "packed", torch.uint8)
-    _accept(scales, "scales", torch.uint8)
-    rows, K = packed.shape[0], _k_of(packed, fmt, "packed")
     if dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError("dtype must be torch.float32 or torch.bfloat16")
-    if K % 32 or tuple(scales.shape) != (rows, K // 32):
-        raise RuntimeError("scales must be [rows, K/32]")
-    if scales.get_device() != packed.get_device():
-        raise RuntimeError("all tensors must be on the same device")
-    out = packed.new_empty((rows, K), dtype=dtype)
-    _launch(packed, lib.mxfp6_dequantize_ex, packed.data_ptr(), scales.data_ptr(), rows, K, fmt, out.data_ptr(),
-            0 if dtype == torch.float32 else 1)
-    return out
+    return ops.dequantize(packed, scales, fmt, dtype is torch.bfloat16)
 
 
 def device_status() -> int:
