@@ -170,7 +170,7 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
     P.x = x; P.y = y; P.w = w; P.b = b; P.w_bf16 = w_dtype;
     P.mean = mean; P.rstd = rstd;
     P.q_out = (uint8_t*)packed; P.q_scales = (uint8_t*)scales;
-    P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H; P.eps = eps;
+    P.rows = rows; P.H = (int)H; P.inv_h = (float)(1.0 / (double)H); P.inv_h_low = (float)(1.0 / (double)H - (double)P.inv_h); P.eps = eps;
     P.offset = ln_offset(x, x_dtype);
     const int grid = ln_grid(rows, k.warps, place == kLnOdd && k.warps > 0, (int64_t)d->sm_count * per_sm, &P.step);
     return launch_pdl(k.kern, (unsigned)grid, (unsigned)threads, (size_t)k.smem, (cudaStream_t)stream, P);
@@ -204,7 +204,7 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     P.x = x; P.dy = dy; P.y = dx; P.w = w; P.w_bf16 = w_dtype;
     P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd);
     P.part = sums ? (float*)ws : nullptr;
-    P.rows = rows; P.H = (int)H; P.inv_h = 1.f / (float)H;
+    P.rows = rows; P.H = (int)H; P.inv_h = (float)(1.0 / (double)H); P.inv_h_low = (float)(1.0 / (double)H - (double)P.inv_h);
     P.offset = ln_offset(x, x_dtype);
     const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(place, (int)H) : ln_backward_kernel<__nv_bfloat16>(place, (int)H);
     int parts;

@@ -36,8 +36,11 @@ struct LnParams {
     int64_t step;            // rows from one of a thread's rows to its next
     int H;
     int offset;              // elements from a chunk boundary (16 or 32 bytes) back to the first row's start
-    float inv_h, eps;
+    float inv_h, inv_h_low;  // 1 / H as the sum of two fp32 values
+    float eps;
 };
+// x / H with one rounding of x's size (1 / H rounded to fp32 alone would add as much again to every mean and variance)
+__device__ __forceinline__ float over_h(const LnParams& P, float x) { return fmaf(x, P.inv_h_low, x * P.inv_h); }
 
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -88,8 +91,9 @@ __device__ __forceinline__ void st_row(T* p, const float (&v)[V]) {
         *p = __float2bfloat16_rn(v[0]);
     }
 }
-// V elements of a parameter vector (fill where there is none), from L2: under programmatic dependent launch an L1 line may be older
-// than the preceding kernel's writes
+// V elements of a parameter vector (fill where there is none).  Plain loads, which the wait for the preceding kernel orders and which
+// the CTAs of an SM share in L1 (not the read-only path, which promises nothing about a kernel that was still writing; loads that
+// go past L1 cost 16 x 8192 a microsecond and rows that start anywhere 20 to 40 %)
 template <int V>
 __device__ __forceinline__ void ld_param(const void* w, int is_bf16, int col, float fill, float (&v)[V]) {
     if (!w) {
@@ -98,20 +102,20 @@ __device__ __forceinline__ void ld_param(const void* w, int is_bf16, int col, fl
     } else if (is_bf16) {
         const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(w) + col;
         if constexpr (V == 8) {
-            const uint4 q = __ldcg(reinterpret_cast<const uint4*>(p));
+            const uint4 q = *reinterpret_cast<const uint4*>(p);
             const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(u[i]); v[2 * i + 1] = bf16_hi(u[i]); }
         } else {
-            v[0] = bf16_lo(__ldcg(reinterpret_cast<const unsigned short*>(p)));
+            v[0] = bf16_lo(*reinterpret_cast<const unsigned short*>(p));
         }
     } else {
         const float* p = reinterpret_cast<const float*>(w) + col;
         if constexpr (V == 8) {
-            const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), c = __ldcg(reinterpret_cast<const float4*>(p + 4));
+            const float4 a = *reinterpret_cast<const float4*>(p), c = *reinterpret_cast<const float4*>(p + 4);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
         } else {
-            v[0] = __ldcg(p);
+            v[0] = *p;
         }
     }
 }
@@ -248,13 +252,24 @@ __device__ __forceinline__ void stage_param(const void* w, int is_bf16, float fi
     for (int c = threadIdx.x; c < k.n; c += blockDim.x) {
         float v[8];
         if constexpr (ODD) {
+            // eight loads in flight whatever the chunk holds of the row (one after another, this staging alone took 5 us of a call)
             const int lo = k.lo(c), hi = k.hi(c);
+            int col[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float t[1] = {0.f};
-                if (i >= lo && i < hi) ld_param<1>(w, is_bf16, 8 * c - k.a + i, fill, t);
-                v[i] = t[0];
+            for (int i = 0; i < 8; ++i) col[i] = min(max(8 * c - k.a + i, 0), k.H - 1);
+            if (!w) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fill;
+            } else if (is_bf16) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = bf16_lo(reinterpret_cast<const unsigned short*>(w)[col[i]]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = reinterpret_cast<const float*>(w)[col[i]];
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < lo || i >= hi) v[i] = 0.f;
         } else {
             ld_param<8>(w, is_bf16, 8 * c, fill, v);
         }
@@ -352,7 +367,7 @@ layer_norm_kernel(const LnParams P) {
             for (int i = 0; i < 4; ++i) s2 = __fadd2_rn(s2, v[c][i]);
         float s[1] = {s2.x + s2.y};
         row_sum<1, WARPS>(s, red[par]);
-        const float mean0 = s[0] * P.inv_h;
+        const float mean0 = over_h(P, s[0]);
         float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
         if (ODD && edge) {
 #pragma unroll
@@ -380,8 +395,8 @@ layer_norm_kernel(const LnParams P) {
         }
         float q[2] = {q2.x + q2.y, d2.x + d2.y};
         row_sum<2, WARPS>(q, red2[par]);
-        const float corr = q[1] * P.inv_h;
-        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
+        const float corr = over_h(P, q[1]);
+        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
         if (tid == 0) {
             if (P.mean) P.mean[row] = mean0 + corr;
             if (P.rstd) P.rstd[row] = rstd;
@@ -423,7 +438,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
             for (int i = 0; i < V; ++i) s[0] += v[i];
         }
         row_sum<1, 32>(s, red);
-        const float mean0 = s[0] * P.inv_h;
+        const float mean0 = over_h(P, s[0]);
         float q[2] = {0.f, 0.f};
         for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
             float v[V];
@@ -432,8 +447,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
             for (int i = 0; i < V; ++i) { const float d = v[i] - mean0; q[0] = fmaf(d, d, q[0]); q[1] += d; }
         }
         row_sum<2, 32>(q, red2);
-        const float corr = q[1] * P.inv_h;
-        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, q[0] * P.inv_h), 0.f) + P.eps);
+        const float corr = over_h(P, q[1]);
+        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
         if (threadIdx.x == 0 && P.mean) P.mean[row] = mean0 + corr;
         if (threadIdx.x == 0 && P.rstd) P.rstd[row] = rstd;
         const float shift = -corr * rstd;
@@ -561,7 +576,7 @@ layer_norm_backward_kernel(const LnParams P) {
         }
         float s[2] = {a2.x + a2.y, b2.x + b2.y};
         row_sum<2, WARPS>(s, red[par]);
-        const float m1 = -s[0] * P.inv_h, m2 = -s[1] * P.inv_h;
+        const float m1 = -over_h(P, s[0]), m2 = -over_h(P, s[1]);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -695,7 +710,7 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
         }
         float s[2] = {a2.x + a2.y, b2.x + b2.y};
         row_sum<2, 16>(s, red[par]);
-        const float m1 = -s[0] * P.inv_h, m2 = -s[1] * P.inv_h;
+        const float m1 = -over_h(P, s[0]), m2 = -over_h(P, s[1]);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
@@ -743,7 +758,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const Ln
             for (int i = 0; i < V; ++i) { const float gw = g[i] * w[i]; s[0] += gw; s[1] = fmaf(gw, (v[i] - mean) * rstd, s[1]); }
         }
         row_sum<2, 32>(s, red[par]);
-        const float m1 = s[0] * P.inv_h, m2 = s[1] * P.inv_h;
+        const float m1 = over_h(P, s[0]), m2 = over_h(P, s[1]);
         for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
             float v[V], g[V], w[V];
             unpack<T, V>(ld_raw<T, V>(x + col), v);
