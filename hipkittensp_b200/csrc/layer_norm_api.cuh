@@ -132,6 +132,10 @@ static int64_t ln_parts_most(int64_t rows, int64_t H, int sm_count) {
     return most;
 }
 
+// Elements of a partial vector: whole chunks, wherever in its first one the row starts.
+static int ln_part_ld(int64_t H) { return (int)((H + 14) / 8 * 8); }
+static size_t ln_workspace(int64_t rows, int64_t H, int sm_count) { return (size_t)ln_parts_most(rows, H, sm_count) * 2 * (size_t)ln_part_ld(H) * 4; }
+
 static int ln_check(const char* what, int64_t rows, int64_t H, int x_dtype, int w_dtype) {
     if (rows < 0 || H < 1) return fail(MXFP6_ERR_BAD_ARG, "%s: rows=%lld H=%lld (rows >= 0 and H >= 1)", what, (long long)rows, (long long)H);
     if (rows > 0x7fffffffLL || H > 0x3fffffffLL) return fail(MXFP6_ERR_BAD_ARG, "%s: dimension too large", what);
@@ -196,7 +200,7 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     if ((rc = get_device_state(&d))) return rc;
     const bool sums = dw || db;
     // one size for every type and alignment of such rows
-    const size_t need = sums ? (size_t)ln_parts_most(rows, H, d->sm_count) * 2 * (size_t)H * 4 : 0;
+    const size_t need = sums ? ln_workspace(rows, H, d->sm_count) : 0;
     if (sums && (!ws || ws_bytes < need)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace too small: need %zu bytes, got %zu", what, need, ws ? ws_bytes : 0);
     if (sums && ((uintptr_t)ws & 15)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace must be 16-byte aligned", what);
     const LnRows place = ln_rows(H, x_dtype, w, nullptr, x, dy, dx);
@@ -206,6 +210,7 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     P.part = sums ? (float*)ws : nullptr;
     P.rows = rows; P.H = (int)H; P.inv_h = (float)(1.0 / (double)H); P.inv_h_low = (float)(1.0 / (double)H - (double)P.inv_h);
     P.offset = ln_offset(x, x_dtype);
+    P.part_ld = place == kLnWhole ? (int)H : ln_part_ld(H);
     const LnChoice k = x_dtype == 0 ? ln_backward_kernel<float>(place, (int)H) : ln_backward_kernel<__nv_bfloat16>(place, (int)H);
     int parts;
     if (k.kern) {
@@ -226,7 +231,8 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
         if ((rc = launch_pdl(over, (unsigned)(rows < cap ? rows : cap), 1024, 0, st, P))) return rc;
     }
     if (!sums) return MXFP6_OK;
-    return launch_pdl(layer_norm_fold_kernel, (unsigned)((2 * H + 31) / 32), 1024, 0, st, (const float*)ws, parts, (int)H, dw, db);
+    return launch_pdl(layer_norm_fold_kernel, (unsigned)((2 * H + 31) / 32), 1024, 0, st, (const float*)ws, parts, (int)H, P.part_ld,
+                      k.kern && place == kLnOdd ? 1 : 0, P.offset, dw, db);
 }
 
 }  // namespace mxfp6

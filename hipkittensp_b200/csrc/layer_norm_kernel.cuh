@@ -29,7 +29,8 @@ struct LnParams {
     int w_bf16;              // type of w and b: 0 = fp32, 1 = bf16
     float* mean;             // [rows]; forward: may be null, like rstd
     float* rstd;             // [rows]
-    float* part;             // backward: [grid][2][H] partial sums of dw and db, or null when they are not wanted
+    float* part;             // backward: [grid][2][part_ld] partial sums of dw and db, or null when they are not wanted
+    int part_ld;             // H, or the row's place among its chunks: element col + a of a vector, like the row itself
     uint8_t* q_out;          // forward to an MX operand: codes [rows, H * bits / 8] ...
     uint8_t* q_scales;       // ... and scales [rows, H / 32]
     int64_t rows;
@@ -476,23 +477,16 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
     }
 }
 
-// a thread's column sums to their places in a vector of H
+// a thread's column sums to their chunks of a partial vector
 template <int C, int TPR, bool ODD>
 __device__ __forceinline__ void st_sums(float* out, int tid, const Chunks<ODD>& k, const float2 (&v)[C][4]) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int chunk = tid + c * TPR;
-        float* o = out + 8 * chunk - k.a;
-        if constexpr (ODD) {
-            const float t[8] = {v[c][0].x, v[c][0].y, v[c][1].x, v[c][1].y, v[c][2].x, v[c][2].y, v[c][3].x, v[c][3].y};
-            const int lo = k.lo(chunk), hi = k.hi(chunk);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i >= lo && i < hi) o[i] = t[i];
-        } else if (chunk < k.n) {
-            reinterpret_cast<float4*>(o)[0] = make_float4(v[c][0].x, v[c][0].y, v[c][1].x, v[c][1].y);
-            reinterpret_cast<float4*>(o)[1] = make_float4(v[c][2].x, v[c][2].y, v[c][3].x, v[c][3].y);
-        }
+        if (chunk >= k.n) continue;
+        float4* o = reinterpret_cast<float4*>(out + 8 * chunk);
+        o[0] = make_float4(v[c][0].x, v[c][0].y, v[c][1].x, v[c][1].y);
+        o[1] = make_float4(v[c][2].x, v[c][2].y, v[c][3].x, v[c][3].y);
     }
 }
 
@@ -586,7 +580,7 @@ layer_norm_backward_kernel(const LnParams P) {
         }
     }
     if (!P.part) return;
-    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
+    float* out = P.part + (int64_t)blockIdx.x * 2 * P.part_ld;
     if constexpr (WARPS == 1) {
         // eight warps hold sums of the same columns
         float* fold = reinterpret_cast<float*>(prm);
@@ -603,12 +597,12 @@ layer_norm_backward_kernel(const LnParams P) {
                 float a = 0.f;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) a += fold[r * (TPR * 8 * C) + K.a + col];
-                out[(int64_t)k * P.H + col] = a;
+                out[(int64_t)k * P.part_ld + K.a + col] = a;
             }
         }
     } else {
 st_sums<C, TPR, ODD>(out, tid, K, dw);
-        st_sums<C, TPR, ODD>(out + P.H, tid, K, db);
+        st_sums<C, TPR, ODD>(out + P.part_ld, tid, K, db);
     }
 }
 
@@ -731,9 +725,9 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!P.part) return;
-    float* out = P.part + (int64_t)blockIdx.x * 2 * P.H;
+    float* out = P.part + (int64_t)blockIdx.x * 2 * P.part_ld;
     st_sums<C, TPR, ODD>(out, tid, K, dw);
-    st_sums<C, TPR, ODD>(out + P.H, tid, K, db);
+    st_sums<C, TPR, ODD>(out + P.part_ld, tid, K, db);
 }
 
 // Rows longer than a CTA's registers hold: dx with a second pass over the row, and the parameter gradients by a kernel whose
@@ -789,14 +783,15 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const LnParams 
         dw = fmaf(g[0], (v[0] - __ldcg(P.mean + r)) * __ldcg(P.rstd + r), dw);
         db += g[0];
     }
-    float* out = P.part + (int64_t)blockIdx.y * 2 * P.H;
+    float* out = P.part + (int64_t)blockIdx.y * 2 * P.part_ld;
     out[col] = dw;
-    out[P.H + col] = db;
+    out[P.part_ld + col] = db;
 }
 
-// [parts][2][H] partial sums -> dw [H], db [H] (either may be null): 32 columns per CTA, 32 threads per column, each adding
-// every 32nd partial; the 32 sums meet in shared memory in a fixed order.
-__global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* part, int parts, int H, float* dw, float* db) {
+// [parts][2][ld] partial sums -> dw [H], db [H] (either may be null): 32 columns per CTA, 32 threads per column, each adding
+// every 32nd partial; the 32 sums meet in shared memory in a fixed order.  odd: the vectors of part p start a elements late, as the
+// rows of that CTA do.
+__global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* part, int parts, int H, int ld, int odd, int offset, float* dw, float* db) {
     __shared__ float s[32][33];
     pdl_launch_dependents();
     pdl_wait();
@@ -805,8 +800,9 @@ __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* part
     const int lane = threadIdx.x >> 5;
     float a = 0.f;
     if (col < two_h) {
+        const float* p0 = part + (col < H ? col : col - H + ld);
 #pragma unroll 8
-        for (int p = lane; p < parts; p += 32) a += __ldcg(part + p * two_h + col);
+        for (int p = lane; p < parts; p += 32) a += __ldcg(p0 + (int64_t)p * 2 * ld + (odd ? (offset + (p & 7) * (H & 7)) & 7 : 0));
     }
     s[lane][threadIdx.x & 31] = a;
     __syncthreads();

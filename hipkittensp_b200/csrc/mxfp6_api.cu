@@ -1282,7 +1282,7 @@ extern "C" size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_
     if (rows <= 0 || H < 1 || rows > 0x7fffffffLL || H > 0x3fffffffLL) return 0;
     DeviceState* d = nullptr;
     if (get_device_state(&d)) return 0;
-    return (size_t)ln_parts_most(rows, H, d->sm_count) * 2 * (size_t)H * 4;
+    return ln_workspace(rows, H, d->sm_count);
 }
 
 extern "C" int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,
