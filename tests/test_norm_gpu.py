@@ -291,6 +291,61 @@ def test_backward_in_place(rows, H, dtype):
         assert rc == 0 and torch.equal(dx, want[0])
 
 
+@pytest.mark.parametrize("H", [768, 1001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16])
+def test_parameter_types_and_optional_statistics(H, dtype, wdtype):
+    x, w, b, dy = _inputs(50, H, dtype, wdtype)
+    y, mean, rstd = hk.layer_norm(x, w, b)
+    _check_forward(x, w, b, 1e-5, y, mean, rstd)
+    _check_backward(dy, x, mean, rstd, w, *hk.layer_norm_backward(dy, x, mean, rstd, w))
+    code = {torch.float32: 0, torch.bfloat16: 1}
+    z, stat, st = torch.empty_like(x), torch.full((50,), 7.0, device=DEV), torch.cuda.current_stream().cuda_stream
+    for m, r in ((None, None), (stat.data_ptr(), None), (None, stat.data_ptr())):
+        rc = hk.lib.mxfp6_layer_norm(x.data_ptr(), code[dtype], w.data_ptr(), b.data_ptr(), code[wdtype], z.data_ptr(), m, r, 50, H, 1e-5, st)
+        assert rc == 0 and torch.equal(z, y)
+        assert m is None or torch.equal(stat, mean)
+        assert r is None or torch.equal(stat, rstd)
+    # one of the two sums alone
+    dw, db = hk.layer_norm_backward(dy, x, mean, rstd, w)[1:]
+    nbytes = hk.lib.mxfp6_layer_norm_backward_workspace_bytes(50, H)
+    work, out = torch.empty(nbytes, dtype=torch.uint8, device=DEV), torch.empty(H, device=DEV)
+    for a, c, want in ((out.data_ptr(), None, dw), (None, out.data_ptr(), db)):
+        rc = hk.lib.mxfp6_layer_norm_backward(dy.data_ptr(), x.data_ptr(), code[dtype], mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), code[wdtype], z.data_ptr(),
+                                              a, c, 50, H, work.data_ptr(), nbytes, st)
+        assert rc == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("H", [8192, 8191])
+def test_matrices_past_32_bits(H):
+    """More than 2^31 elements (and 2^32 bytes): the last rows get the bits of a small matrix of the same rows."""
+    rows, n = 270000, 64
+    x = torch.zeros(rows, H, dtype=torch.bfloat16, device=DEV)
+    tail, w, b, dtail = _inputs(n, H, torch.bfloat16, torch.float32)
+    x[-n:] = tail
+    y, mean, rstd = hk.layer_norm(x, w, b)
+    want = hk.layer_norm(tail, w, b)
+    assert torch.equal(y[-n:], want[0]) and torch.equal(mean[-n:], want[1]) and torch.equal(rstd[-n:], want[2])
+    assert torch.equal(y[0], b.to(torch.bfloat16)) and torch.equal(y[rows // 2], b.to(torch.bfloat16))
+    dy = y.zero_()
+    dy[-n:] = dtail
+    dx, dw, db = hk.layer_norm_backward(dy, x, mean, rstd, w)
+    small = hk.layer_norm_backward(dtail, tail, *want[1:], w)
+    assert torch.equal(dx[-n:], small[0]) and not dx[:-n].any()
+    for got, ref in zip((dw, db), small[1:]):          # the same terms in another order (64 of them are not zero)
+        assert ((got - ref).abs() <= 2 * n * U * ref.abs().max()).all()
+    del dy, dx, y
+    if H % 32 == 0:
+        packed, scales, _, _ = hk.layer_norm_quantize(x, w, b, fmt=hk.E2M1)
+        sp, ss, _, _ = hk.layer_norm_quantize(tail, w, b, fmt=hk.E2M1)
+        assert torch.equal(packed[-n:], sp) and torch.equal(scales[-n:], ss)
+        q, qs = hk.quantize(x, hk.E2M1)
+        tq, tqs = hk.quantize(tail, hk.E2M1)
+        assert torch.equal(q[-n:], tq) and torch.equal(qs[-n:], tqs) and not q[:-n].any()
+        d = hk.dequantize(q, qs, hk.E2M1, dtype=torch.bfloat16)
+        assert torch.equal(d[-n:], hk.dequantize(tq, tqs, hk.E2M1, dtype=torch.bfloat16)) and not d[:-n].any()
+
+
 def test_backward_against_differences():
     """d/dx, d/dw and d/db of sum(dy * y) by central differences of the 64-bit formula, at a few places."""
     rows, H, eps = 5, 40, 1e-5
