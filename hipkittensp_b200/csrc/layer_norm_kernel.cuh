@@ -30,7 +30,6 @@ struct LnParams {
     float* mean;             // [rows]; forward: may be null, like rstd
     float* rstd;             // [rows]
     float* part;             // backward: [grid][2][part_ld] partial sums of dw and db, or null when they are not wanted
-    int part_ld;             // H, or the row's place among its chunks: element col + a of a vector, like the row itself
     uint8_t* q_out;          // forward to an MX operand: codes [rows, H * bits / 8] ...
     uint8_t* q_scales;       // ... and scales [rows, H / 32]
     int64_t rows;
@@ -39,6 +38,7 @@ struct LnParams {
     int offset;              // elements from a chunk boundary (16 or 32 bytes) back to the first row's start
     float inv_h, inv_h_low;  // 1 / H as the sum of two fp32 values
     float eps;
+    int part_ld;             // H, or the row's place among its chunks: element col + a of a vector, like the row itself
 };
 // x / H with one rounding of x's size (1 / H rounded to fp32 alone would add as much again to every mean and variance)
 __device__ __forceinline__ float over_h(const LnParams& P, float x) { return fmaf(x, P.inv_h_low, x * P.inv_h); }
