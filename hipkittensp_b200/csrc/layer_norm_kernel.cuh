@@ -146,39 +146,67 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red) {
     }
 }
 
-// Eight consecutive fp32 values of a 32-element block held by four consecutive lanes -> codes and scale.
-template <int FMT>
-__device__ __forceinline__ void mx_store8(const float2 (&v)[4], uint8_t* codes_row, uint8_t* scales_row, int col, bool live) {
-    float amax = amax3(amax3(v[0].x, v[0].y, v[1].x), amax3(v[1].y, v[2].x, v[2].y), fmaxf(fabsf(v[3].x), fabsf(v[3].y)));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int sb = quant_scale_byte(amax, FMT);
-    const float f = quant_inv_scale(sb);
-    float s[8];
+// C chunks of eight fp32 values, each a quarter of a 32-element block held by four consecutive lanes -> codes and scales; chunk c holds
+// the elements from col + c * stride on.  Step by step for all chunks, so that their shuffles are in flight together.
+template <int FMT, int C>
+__device__ __forceinline__ void mx_store(float2 (&v)[C][4], uint8_t* codes_row, uint8_t* scales_row, int col, int stride, int cols) {
+    float amax[C];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 t = __fmul2_rn(v[i], make_float2(f, f));
-        s[2 * i] = t.x; s[2 * i + 1] = t.y;
+    for (int c = 0; c < C; ++c)
+        amax[c] = amax3(amax3(v[c][0].x, v[c][0].y, v[c][1].x), amax3(v[c][1].y, v[c][2].x, v[c][2].y), fmaxf(fabsf(v[c][3].x), fabsf(v[c][3].y)));
+#pragma unroll
+    for (int c = 0; c < C; ++c) amax[c] = fmaxf(amax[c], __shfl_xor_sync(0xffffffffu, amax[c], 1));
+#pragma unroll
+    for (int c = 0; c < C; ++c) amax[c] = fmaxf(amax[c], __shfl_xor_sync(0xffffffffu, amax[c], 2));
+    const int j = (col >> 3) & 3;                   // place of these eight in their block (the stride is a multiple of 32)
+    uint32_t w0[C], w1[C];
+    int sb[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        sb[c] = quant_scale_byte(amax[c], FMT);
+        const float f = quant_inv_scale(sb[c]);
+        float s[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = __fmul2_rn(v[c][i], make_float2(f, f));
+            s[2 * i] = t.x; s[2 * i + 1] = t.y;
+        }
+        if constexpr (FMT == kE2M1) {
+            w0[c] = cvt_oct_e2m1(s);
+            w1[c] = 0;
+        } else {
+            const uint32_t lo = cvt_quad<FMT>(s[0], s[1], s[2], s[3]), hi = cvt_quad<FMT>(s[4], s[5], s[6], s[7]);
+            // 6-bit codes: 24 bits each, 48 a lane
+            w0[c] = fmt_fp8(FMT) ? lo : lo | (hi << 24);
+            w1[c] = fmt_fp8(FMT) ? hi : hi >> 8;
+        }
     }
-    const int j = (col >> 3) & 3;                   // place of these eight in their block
-    if constexpr (FMT == kE2M1) {
-        const uint32_t w = cvt_oct_e2m1(s);
-        if (live) *reinterpret_cast<uint32_t*>(codes_row + col / 2) = w;
-    } else if constexpr (fmt_fp8(FMT)) {
-        const uint2 w = make_uint2(cvt_quad<FMT>(s[0], s[1], s[2], s[3]), cvt_quad<FMT>(s[4], s[5], s[6], s[7]));
-        if (live) *reinterpret_cast<uint2*>(codes_row + col) = w;
+    if constexpr (FMT == kE2M1 || fmt_fp8(FMT)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = col + c * stride;
+            if (at >= cols) continue;
+            if constexpr (FMT == kE2M1) *reinterpret_cast<uint32_t*>(codes_row + at / 2) = w0[c];
+            else *reinterpret_cast<uint2*>(codes_row + at) = make_uint2(w0[c], w1[c]);
+        }
     } else {
-        const uint32_t lo = cvt_quad<FMT>(s[0], s[1], s[2], s[3]), hi = cvt_quad<FMT>(s[4], s[5], s[6], s[7]);      // 24 bits each
-        // 48 bits a lane: four lanes hold 24 bytes, which three of them write, 8 each: lane j the bits from 64 j on, which start at
-        // bit 16 j of its own 48 and run on into its neighbour's
-        const uint32_t w0 = lo | (hi << 24), w1 = hi >> 8;
-        const uint32_t n0 = __shfl_down_sync(0xffffffffu, w0, 1), n1 = __shfl_down_sync(0xffffffffu, w1, 1);
-        const uint32_t a = j == 2 ? w1 : w0, b = j == 2 ? n0 : w1, c = j == 2 ? n1 : n0;
-        const uint32_t o0 = __byte_perm(a, b, j == 0 ? 0x3210 : j == 1 ? 0x5432 : 0x5410);
-        const uint32_t o1 = __byte_perm(b, c, j == 0 ? 0x5410 : j == 1 ? 0x7654 : 0x5432);
-        if (live && j < 3) *reinterpret_cast<uint2*>(codes_row + (col / 32) * 24 + 8 * j) = make_uint2(o0, o1);
+        // four lanes hold 24 bytes, which three of them write, 8 each: lane j the bits from 64 j on, which start at bit 16 j of its
+        // own 48 and run on into its neighbour's
+        uint32_t n0[C], n1[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) { n0[c] = __shfl_down_sync(0xffffffffu, w0[c], 1); n1[c] = __shfl_down_sync(0xffffffffu, w1[c], 1); }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = col + c * stride;
+            const uint32_t a = j == 2 ? w1[c] : w0[c], b = j == 2 ? n0[c] : w1[c], d = j == 2 ? n1[c] : n0[c];
+            const uint32_t o0 = __byte_perm(a, b, j == 0 ? 0x3210 : j == 1 ? 0x5432 : 0x5410);
+            const uint32_t o1 = __byte_perm(b, d, j == 0 ? 0x5410 : j == 1 ? 0x7654 : 0x5432);
+            if (at < cols && j < 3) *reinterpret_cast<uint2*>(codes_row + (at / 32) * 24 + 8 * j) = make_uint2(o0, o1);
+        }
     }
-    if (live && j == 0) scales_row[col / 32] = (uint8_t)sb;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        if (col + c * stride < cols && j == 0) scales_row[(col + c * stride) / 32] = (uint8_t)sb[c];
 }
 
 // ---- rows as chunks of 8 elements
@@ -322,6 +350,9 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     static_assert(!ODD || FMT < 0, "an MX result has whole blocks");
+    // the chunks' codes made together (16384 x 8192 bf16: E2M1 98 us, 104 one by one; E4M3 103, 105) or, where that takes too many
+    // registers, one by one (E2M3 111 us, 124 together)
+    constexpr bool together = FMT == kE2M1 || fmt_fp8(FMT);
     __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
     extern __shared__ float4 prm[];                             // w, then b
     pdl_launch_dependents();
@@ -407,17 +438,21 @@ layer_norm_kernel(const LnParams P) {
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
             const bool live = chunk < K.n;
-            float2 o[4], w[4], b[4];
+            float2 w[4], b[4];
             ld_staged(prm, K.n, live ? chunk : 0, w);
             ld_staged(prm + 2 * K.n, K.n, live ? chunk : 0, b);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                o[i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
-            if constexpr (FMT >= 0)
-                mx_store8<FMT>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, live);
-            else
-                st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, o);
+                v[c][i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
+            if constexpr (FMT < 0) {
+                st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, v[c]);
+            } else if constexpr (!together) {
+                float2 o[1][4] = {{v[c][0], v[c][1], v[c][2], v[c][3]}};
+                mx_store<FMT, 1>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, 0, P.H);
+            }
         }
+        if constexpr (FMT >= 0 && together)
+            mx_store<FMT, C>(v, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * tid, 8 * TPR, P.H);
     }
 }
 
@@ -468,8 +503,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
                 for (int i = 0; i < V; ++i) v[i] = fmaf(fmaf(v[i] - mean0, rstd, shift), w[i], b[i]);
             }
             if constexpr (FMT >= 0) {
-                const float2 o[4] = {make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]), make_float2(v[6], v[7])};
-                mx_store8<FMT>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), col, live);
+                float2 o[1][4] = {{make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]), make_float2(v[6], v[7])}};
+                mx_store<FMT, 1>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), col, 0, P.H);
             } else if (live) {
                 st_row<T, V>(reinterpret_cast<T*>(P.y) + row * P.H + col, v);
             }
