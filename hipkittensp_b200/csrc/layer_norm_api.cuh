@@ -145,6 +145,13 @@ static int ln_check(const char* what, int64_t rows, int64_t H, int x_dtype, int 
 }
 static bool ln_natural(const void* p, int dtype) { return !((uintptr_t)p & (dtype == 0 ? 3 : 1)); }
 
+// Do the ranges share bytes?  A CTA writes its rows while others still read theirs, so a result may lie on an operand of its own
+// shape, row upon row, or apart from it.
+static bool ln_overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t q_bytes) {
+    const uint64_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return a < b ? b - a < p_bytes : a - b < q_bytes;
+}
+
 // elements from the 16- or 32-byte boundary in front of p to p
 static int ln_offset(const void* p, int dtype) { return (int)((uintptr_t)p & (dtype == 0 ? 31 : 15)) / (dtype == 0 ? 4 : 2); }
 
@@ -164,6 +171,11 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
     const LnRows place = ln_rows(H, x_dtype, w, b, x, mx ? x : y, x);
     if (mx && (place != kLnWhole || ((uintptr_t)packed & 15)))
         return fail(MXFP6_ERR_BAD_ARG, "%s: x must be 32-byte (fp32) or 16-byte (bf16) aligned, weight, bias and codes 16-byte", what);
+    const uint64_t bytes = (uint64_t)rows * (uint64_t)H * (x_dtype == 0 ? 4 : 2);
+    if (mx ? ln_overlap(x, bytes, packed, (uint64_t)rows * (uint64_t)(H / 32) * fmt_block_bytes(fmt)) ||
+                 ln_overlap(x, bytes, scales, (uint64_t)rows * (uint64_t)(H / 32))
+           : x != y && ln_overlap(x, bytes, y, bytes))
+        return fail(MXFP6_ERR_BAD_ARG, "%s: the result overlaps x", what);
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
     const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(place, fmt, (int)H) : ln_forward_kernel<__nv_bfloat16>(place, fmt, (int)H);
@@ -196,6 +208,9 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     if (!ln_natural(x, x_dtype) || !ln_natural(dy, x_dtype) || !ln_natural(dx, x_dtype) || !ln_natural(w, w_dtype) ||
         !ln_natural(mean, 0) || !ln_natural(rstd, 0))
         return fail(MXFP6_ERR_BAD_ARG, "%s: misaligned pointer", what);
+    const uint64_t bytes = (uint64_t)rows * (uint64_t)H * (x_dtype == 0 ? 4 : 2);
+    if ((dx != x && ln_overlap(dx, bytes, x, bytes)) || (dx != dy && ln_overlap(dx, bytes, dy, bytes)))
+        return fail(MXFP6_ERR_BAD_ARG, "%s: dx overlaps x or dy without being it", what);
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
     const bool sums = dw || db;

@@ -12,7 +12,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None):
     """y = (x - mean) * rstd * weight + bias over each row of x [rows, H] (fp32 or bf16), in fp32, rounded once to x's type.
 
     weight and bias [H] (fp32 or bf16, the same type) may be None.  Returns (y, mean, rstd), the statistics fp32 [rows] as
-    layer_norm_backward takes them; `out` (may be x) receives y."""
+    layer_norm_backward takes them; `out` (x itself, or apart from it) receives y."""
     return ops.layer_norm(x, weight, bias, eps, out)
 
 

@@ -212,12 +212,12 @@ int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, in
  *     mean = sum(x) / H,  rstd = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) * rstd * weight + bias
  * with all arithmetic in fp32 and one rounding of y to x's type.  weight and bias are [H] vectors of w_dtype (0 = fp32,
  * 1 = bf16); either may be NULL (ones / zeros).  mean and rstd are fp32 [rows], kept for the backward pass; either may be
- * NULL.  y may be x itself.  Any H >= 1 and any pointers aligned to their type; x and y that start at the same place of a 16-byte
- * (bf16) or 32-byte (fp32) unit of memory take the vector paths, others are passed over element by element.
+ * NULL.  y may be x itself; one that overlaps x otherwise is refused.  Any H >= 1 and any pointers aligned to their type; x and y
+ * that start at the same place of a 16-byte (bf16) or 32-byte (fp32) unit of memory take the vector paths, others are passed over element by element.
  *
  * The _quantize form delivers y as an MX operand instead (blocks of 32 along H: the K of the product that follows), rounded
  * once from fp32 with the rule of mxfp6_quantize: packed [rows, H/2 | 3H/4 | H] codes and scales [rows, H/32].  H % 32 == 0;
- * x 16-byte (bf16) or 32-byte (fp32) aligned, weight, bias and packed 16-byte.
+ * x 16-byte (bf16) or 32-byte (fp32) aligned, weight, bias and packed 16-byte; codes and scales apart from x.
  * (Stands next to the reference's fused norm, kernels/layernorm/kernel.cpp, which has neither statistics nor a gradient.)
  */
 int mxfp6_layer_norm(const void* x, int x_dtype, const void* weight, const void* bias, int w_dtype, void* y,
@@ -235,7 +235,8 @@ int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, co
  * The sums over the rows go through per-CTA partials in `workspace` (at least the given number of bytes, 16-byte aligned, owned
  * by this call until the stream has passed it; any contents; not needed when dweight and dbias are both NULL) and are added
  * in a fixed order: equal calls on a device give equal bits.  Two calls that may overlap need a workspace each.
- * rows = 0 gives zero parameter gradients.  dx may be dy or x itself.  (No counterpart in the reference.)
+ * rows = 0 gives zero parameter gradients.  dx may be dy or x itself; one that overlaps them otherwise is
+ * refused.  (No counterpart in the reference.)
  */
 size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H);
 int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,

@@ -41,6 +41,23 @@ def test_c_entry_points_refuse_without_a_device():
     assert L.mxfp6_layer_norm_backward_workspace_bytes(4, 0) == 0
 
 
+def test_results_over_other_rows_are_refused():
+    """A result that lies over its operand, but not row upon row, would be read after it was written."""
+    L, BAD = hk.lib, _lib.ERR_BAD_ARG
+    P, F = 1 << 20, 1 << 30
+    for xd, size in ((0, 4), (1, 2)):
+        span = 5 * 64 * size
+        for shift in (64 * size, span - size, size, -size, -64 * size, size - span):
+            assert L.mxfp6_layer_norm(P, xd, F, F, 0, P + shift, F, F, 5, 64, 1e-5, None) == BAD
+            assert b"overlaps" in L.mxfp6_last_error(), shift
+            for dy, x in ((P, F), (F, P)):
+                assert L.mxfp6_layer_norm_backward(dy, x, xd, F, F, F, 0, P + shift, F, F, 5, 64, F, 1 << 30, None) == BAD
+                assert b"overlaps" in L.mxfp6_last_error(), shift
+        for packed, scales in ((P, F), (P + span - 16, F), (P - 16, F), (F, P), (F, P + span - 1), (F, P - 9)):
+            assert L.mxfp6_layer_norm_quantize(P, xd, F, F, 0, 4, packed, scales, F, F, 5, 64, 1e-5, None) == BAD
+            assert b"overlaps" in L.mxfp6_last_error(), (packed, scales)
+
+
 def test_python_wrappers_refuse():
     x = torch.zeros(4, 64)
     for f in (lambda: hk.layer_norm(x), lambda: hk.layer_norm_quantize(x), lambda: hk.layer_norm_backward(x, x, x[:, 0], x[:, 0])):
