@@ -203,9 +203,21 @@ def gemm_scaled(A, scale_A, B, scale_B, row_scale=None, col_scale=None, bias=Non
     return ops.gemm_scaled(A, scale_A, B, scale_B, row_scale, col_scale, bias, fmt, fmt if fmt_b is None else fmt_b, out)
 
 
-def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=None):
-    """The product of dispatch_micro with its result allocated here (unless given as `out`); returns C."""
-    return ops.gemm(A, scale_A, B, scale_B, fmt, fmt if fmt_b is None else fmt_b, out, 0)
+def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=None, workspace=None):
+    """The product of dispatch_micro with its result allocated here (unless given as `out`); returns C.
+
+    A product with at most 128 rows may add partial sums in a buffer that the library holds once per device, as the other
+    products do.  Calls that may run side by side (on several streams, or in captured graphs) take a `workspace` of
+    gemm_workspace() each; calls in the order of one stream can share it."""
+    return ops.gemm(A, scale_A, B, scale_B, fmt, fmt if fmt_b is None else fmt_b, out, workspace)
+
+
+def gemm_workspace(M: int, N: int, K: int, device=None) -> torch.Tensor:
+    """A zeroed workspace for gemm() on [M,K] x [N,K], of any formats (empty where the sums are never split); a product leaves
+    zero what must be zero, so it serves one call after another, also of other shapes if it is large enough."""
+    device = torch.device("cuda" if device is None else device)
+    with torch.cuda.device(device):
+        return torch.zeros(lib.mxfp6_gemm_workspace_bytes(M, N, K), dtype=torch.uint8, device=device)
 
 
 def quantize(x: torch.Tensor, fmt: int = E2M3):

@@ -139,6 +139,53 @@ def test_caller_workspace(shape):
         check(C.float().cpu().numpy(), *oracle_f64(pa, sa, pb, sb, fa, FP4))
 
 
+@pytest.mark.parametrize("fa", [FP4, R.E4M3])
+def test_side_by_side_with_a_workspace_each(fa):
+    """Products whose tiles are split along K: on two streams at once, then in two captured graphs replayed at once."""
+    M, N, K = 16, 512, 8192
+    assert hk.gemm_workspace(M, N, K).numel() > 0
+    sides = []
+    for seed in (1, 2):
+        host = quantized_inputs("normal", M, N, K, fa, seed, FP4)
+        out = torch.empty(24, M, N, dtype=torch.bfloat16, device="cuda")
+        sides.append((host, [torch.from_numpy(x).cuda() for x in host], hk.gemm_workspace(M, N, K), out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def verify():
+        torch.cuda.synchronize()
+        assert hk.device_status() == 0
+        for host, _, _, out, _ in sides:
+            assert (out == out[0]).all()
+            check(out[0].float().cpu().numpy(), *oracle_f64(*host, fa, FP4))
+            out.zero_()
+        torch.cuda.synchronize()
+
+    for i in range(24):
+        for _, t, ws, out, stream in sides:
+            with torch.cuda.stream(stream):
+                hk.gemm(*t, fmt=fa, fmt_b=FP4, out=out[i], workspace=ws)
+    verify()
+    graphs = []
+    for _, t, ws, out, _ in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for i in range(24):
+                hk.gemm(*t, fmt=fa, fmt_b=FP4, out=out[i], workspace=ws)
+    for graph, (*_, stream) in zip(graphs, sides):
+        with torch.cuda.stream(stream):
+            graph.replay()
+    verify()
+
+
+def test_workspace_refusals():
+    t = [torch.from_numpy(x).cuda() for x in quantized_inputs("normal", 16, 512, 8192, FP4, 1)]
+    ws = hk.gemm_workspace(16, 512, 8192)
+    for bad in (ws[:1024], ws[8:], ws.cpu(), ws.view(torch.float32), ws[::2], 7):
+        with pytest.raises(RuntimeError):
+            hk.gemm(*t, fmt=FP4, workspace=bad)
+    assert hk.gemm_workspace(4096, 4096, 1024).numel() == 0
+
+
 @pytest.mark.parametrize("pair", PAIRS[:2])
 @pytest.mark.parametrize("force", ["128,0,0", "256,0,0", "128,0,1", "256,0,1", "16,1,0", "32,1,1", "64,1,1", "128,1,1", "256,0,0,1"])
 def test_kernel_variants(force, pair):
