@@ -1,5 +1,5 @@
 // Layer norm over the rows of a [rows, H] matrix (fp32 or bf16), its gradient, and the form that hands its result on as an MX
-// operand.  All sums and statistics are fp32.
+// operand.  All sums and statistics are fp32, and 64 bits for the rows whose squares leave the range of fp32.
 //
 //   forward    mean = sum(x) / H,  var = sum((x - mean)^2) / H,  rstd = 1 / sqrt(var + eps),  y = (x - mean) * rstd * w + b
 //   backward   xhat = (x - mean) * rstd,  g = dy * w,
@@ -40,8 +40,13 @@ struct LnParams {
     float eps;
     int part_ld;             // H, or the row's place among its chunks: element col + a of a vector, like the row itself
 };
-// x / H with one rounding of x's size (1 / H rounded to fp32 alone would add as much again to every mean and variance)
+// x / H with one rounding of x's size (1 / H rounded to fp32 alone would add as much again to every mean and variance); x finite
 __device__ __forceinline__ float over_h(const LnParams& P, float x) { return fmaf(x, P.inv_h_low, x * P.inv_h); }
+// ... and an infinite x stays infinite: its product with the low part, which may be 0 or negative, is left out
+__device__ __forceinline__ float over_h_inf(const LnParams& P, float x) {
+    const float t = x * P.inv_h;
+    return isinf(t) ? t : fmaf(x, P.inv_h_low, t);
+}
 
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
@@ -209,6 +214,72 @@ __device__ __forceinline__ void mx_store(float2 (&v)[C][4], uint8_t* codes_row, 
         if (col + c * stride < cols && j == 0) scales_row[(col + c * stride) / 32] = (uint8_t)sb[c];
 }
 
+// A row that fp32 statistics cannot carry, by the TPR = 32 * WARPS threads that share it, in 64 bits and straight from memory: the sum
+// or the sum of squares overflows (values past about 1e17), the squares vanish below the range and eps does not cover them, or
+// the row holds an infinity or a NaN (whose mean and rstd come out as the formulas give them).  Not inlined: no
+// register of the usual path is held for it.
+template <int WARPS>
+__device__ __forceinline__ double row_sum64(double v, double* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (WARPS > 1) {
+        __syncthreads();                                        // (what the buffer held has been read)
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int w = 0; w < WARPS; ++w) v += red[w];
+    }
+    return v;
+}
+template <typename T, int WARPS, int FMT>
+__device__ __noinline__ void norm_row_64(const LnParams P, int64_t row, int tid, double* red) {
+    constexpr int TPR = 32 * WARPS;
+    const T* x = reinterpret_cast<const T*>(P.x) + row * P.H;
+    auto at = [&](int col) {
+        float v[1];
+        unpack<T, 1>(ld_raw<T, 1>(x + col), v);
+        return (double)v[0];
+    };
+    double s = 0.0, q = 0.0;
+    for (int col = tid; col < P.H; col += TPR) s += at(col);
+    const double mean = row_sum64<WARPS>(s, red) / P.H;
+    for (int col = tid; col < P.H; col += TPR) {
+        const double d = at(col) - mean;
+        q += d * d;
+    }
+    const double rstd = 1.0 / sqrt(row_sum64<WARPS>(q, red) / P.H + (double)P.eps);
+    if (tid == 0) {
+        if (P.mean) P.mean[row] = (float)mean;
+        if (P.rstd) P.rstd[row] = (float)rstd;
+    }
+    auto result = [&](int col) {
+        float w[1], b[1];
+        ld_param<1>(P.w, P.w_bf16, col, 1.f, w);
+        ld_param<1>(P.b, P.w_bf16, col, 0.f, b);
+        return (float)((at(col) - mean) * rstd * (double)w[0] + (double)b[0]);
+    };
+    if constexpr (FMT < 0) {
+        for (int col = tid; col < P.H; col += TPR) {
+            const float v[1] = {result(col)};
+            st_row<T, 1>(reinterpret_cast<T*>(P.y) + row * P.H + col, v);
+        }
+    } else {
+        // every thread makes the same number of rounds: the lanes of a block exchange their largest magnitudes
+        for (int c0 = 0; c0 < P.H; c0 += 8 * TPR) {
+            const int col = c0 + 8 * tid;
+            float v[8];
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) v[i] = col < P.H ? result(col + i) : 0.f;
+            float2 o[1][4] = {{make_float2(v[0], v[1]), make_float2(v[2], v[3]), make_float2(v[4], v[5]), make_float2(v[6], v[7])}};
+            mx_store<FMT, 1>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), col, 0, P.H);
+        }
+    }
+}
+// Does the sum of squares of a row say that it is such a row?  (A sum that is not finite makes it so too.)  Below 2^-100 it has lost digits to
+// the end of the range, which matter where eps is small beside the variance.  (The bound is made here: as a member of LnParams it moved
+// the registers of the MX forms about, E2M3 113 -> 119 us.)
+__device__ __forceinline__ bool beyond_fp32(const LnParams& P, float q) { return !(q >= (P.eps < 0x1p-70f ? 0x1p-100f : 0.f) && q <= 3.402823466e38f); }
+
 // ---- rows as chunks of 8 elements
 // Rows of whole, aligned chunks (ODD = false) are n = H / 8 chunks.  Other rows are cut at the same 16- or 32-byte boundaries of
 // memory: the row starts `a` elements behind a boundary, its first and last chunk may hold neighbours' elements (which are
@@ -350,10 +421,11 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS, WARPS == 1 ? 2 
 layer_norm_kernel(const LnParams P) {
     constexpr int TPR = 32 * WARPS;
     static_assert(!ODD || FMT < 0, "an MX result has whole blocks");
-    // the chunks' codes made together (16384 x 8192 bf16: E2M1 98 us, 104 one by one; E4M3 103, 105) or, where that takes too many
+    // the chunks' codes made together (16384 x 8192 bf16: E2M1 100 us, 104 one by one; E4M3 100, 105) or, where that takes too many
     // registers, one by one (E2M3 111 us, 124 together)
     constexpr bool together = FMT == kE2M1 || fmt_fp8(FMT);
     __shared__ float red[2][WARPS], red2[2][2 * WARPS];         // [row parity]
+    __shared__ double red64[WARPS];
     extern __shared__ float4 prm[];                             // w, then b
     pdl_launch_dependents();
     pdl_wait();
@@ -371,9 +443,12 @@ layer_norm_kernel(const LnParams P) {
             for (int c = 0; c < C; ++c) ld_chunk<T, ODD>(x, at, inner, tid + c * TPR, K, raw[c]);
         }
     };
+    auto begin = [&](int64_t r) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};           // elements outside the row stay zero
-    load(row);
+        for (int c = 0; c < C; ++c) raw[c] = Raw<T, 8>{};       // elements outside the row stay zero
+        load(r);
+    };
+    begin(row);
     stage_param(P.w, P.w_bf16, 1.f, K, prm);
     stage_param(P.b, P.w_bf16, 0.f, K, prm + 2 * K.n);
     // does this warp hold elements outside the row?  (one decision per row; the same for all of this thread's rows)
@@ -382,7 +457,8 @@ layer_norm_kernel(const LnParams P) {
     for (int c = 0; c < C; ++c) inside = inside && K.whole(tid + c * TPR);
     const bool edge = !__all_sync(0xffffffffu, inside);
     __syncthreads();
-    for (int par = 0; row < P.rows; row += P.step, par ^= 1) {
+    for (int par = 0;; par ^= 1) {
+      for (; row < P.rows; row += P.step, par ^= 1) {
         float2 v[C][4];
         if constexpr (ODD) {
             if (edge)
@@ -427,6 +503,7 @@ layer_norm_kernel(const LnParams P) {
         }
         float q[2] = {q2.x + q2.y, d2.x + d2.y};
         row_sum<2, WARPS>(q, red2[par]);
+        if (beyond_fp32(P, q[0])) break;                        // (equal for all threads of the row)
         const float corr = over_h(P, q[1]);
         const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
         if (tid == 0) {
@@ -453,6 +530,12 @@ layer_norm_kernel(const LnParams P) {
         }
         if constexpr (FMT >= 0 && together)
             mx_store<FMT, C>(v, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * tid, 8 * TPR, P.H);
+      }
+      if (row >= P.rows) break;
+      // (the call stands outside the loop over the rows: inside it E2M1 takes 105 us instead of 101, E4M3 106 instead of 101)
+      norm_row_64<T, WARPS, FMT>(P, row, tid, red64);
+      row += P.step;
+      begin(row);
     }
 }
 
@@ -461,6 +544,7 @@ layer_norm_kernel(const LnParams P) {
 template <typename T, int V, int FMT>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P) {
     __shared__ float red[32], red2[64];
+    __shared__ double red64[32];
     pdl_launch_dependents();
     pdl_wait();
     const T* x = reinterpret_cast<const T*>(P.x);
@@ -483,6 +567,10 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const LnParams P)
             for (int i = 0; i < V; ++i) { const float d = v[i] - mean0; q[0] = fmaf(d, d, q[0]); q[1] += d; }
         }
         row_sum<2, 32>(q, red2);
+        if (beyond_fp32(P, q[0])) {
+            norm_row_64<T, 32, FMT>(P, row, threadIdx.x, red64);
+            continue;
+        }
         const float corr = over_h(P, q[1]);
         const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
         if (threadIdx.x == 0 && P.mean) P.mean[row] = mean0 + corr;
@@ -605,7 +693,7 @@ layer_norm_backward_kernel(const LnParams P) {
         }
         float s[2] = {a2.x + a2.y, b2.x + b2.y};
         row_sum<2, WARPS>(s, red[par]);
-        const float m1 = -over_h(P, s[0]), m2 = -over_h(P, s[1]);
+        const float m1 = -over_h_inf(P, s[0]), m2 = -over_h_inf(P, s[1]);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -739,7 +827,7 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
         }
         float s[2] = {a2.x + a2.y, b2.x + b2.y};
         row_sum<2, 16>(s, red[par]);
-        const float m1 = -over_h(P, s[0]), m2 = -over_h(P, s[1]);
+        const float m1 = -over_h_inf(P, s[0]), m2 = -over_h_inf(P, s[1]);
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int chunk = tid + c * TPR;
@@ -787,7 +875,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const Ln
             for (int i = 0; i < V; ++i) { const float gw = g[i] * w[i]; s[0] += gw; s[1] = fmaf(gw, (v[i] - mean) * rstd, s[1]); }
         }
         row_sum<2, 32>(s, red[par]);
-        const float m1 = over_h(P, s[0]), m2 = over_h(P, s[1]);
+        const float m1 = over_h_inf(P, s[0]), m2 = over_h_inf(P, s[1]);
         for (int col = threadIdx.x * V; col < P.H; col += 1024 * V) {
             float v[V], g[V], w[V];
             unpack<T, V>(ld_raw<T, V>(x + col), v);

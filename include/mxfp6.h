@@ -210,7 +210,9 @@ int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, in
 /*
  * Layer norm over the rows of x [rows, H] (x_dtype 0 = fp32, 1 = bf16), the step in front of a projection:
  *     mean = sum(x) / H,  rstd = 1 / sqrt(sum((x - mean)^2) / H + eps),  y = (x - mean) * rstd * weight + bias
- * with all arithmetic in fp32 and one rounding of y to x's type.  weight and bias are [H] vectors of w_dtype (0 = fp32,
+ * with all arithmetic in fp32 and one rounding of y to x's type; a row whose sums leave the range of fp32 (finite values past about
+ * 1e17, or squares that vanish beside a tiny eps) is worked out in 64 bits, and one that holds an infinity or a NaN has the mean
+ * that its sum gives and a NaN for rstd and for all of y.  weight and bias are [H] vectors of w_dtype (0 = fp32,
  * 1 = bf16); either may be NULL (ones / zeros).  mean and rstd are fp32 [rows], kept for the backward pass; either may be
  * NULL.  y may be x itself; one that overlaps x otherwise is refused.  Any H >= 1 and any pointers aligned to their type; x and y
  * that start at the same place of a 16-byte (bf16) or 32-byte (fp32) unit of memory take the vector paths, others are passed over element by element.
