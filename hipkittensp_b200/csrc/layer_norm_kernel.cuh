@@ -345,6 +345,15 @@ __device__ __forceinline__ void mask_chunk(const Chunks<true>& k, int chunk, Raw
             r.u[i] &= (2 * i >= lo && 2 * i < hi ? 0xffffu : 0u) | (2 * i + 1 >= lo && 2 * i + 1 < hi ? 0xffff0000u : 0u);
     }
 }
+// `value` for the elements of a chunk that belong to other rows
+__device__ __forceinline__ void fill_outside(const Chunks<true>& k, int chunk, float value, float2 (&v)[4]) {
+    const int lo = k.lo(chunk), hi = k.hi(chunk);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (2 * i < lo || 2 * i >= hi) v[i].x = value;
+        if (2 * i + 1 < lo || 2 * i + 1 >= hi) v[i].y = value;
+    }
+}
 // Parameter vectors in shared memory, as fp32 whatever their type and filled where they are absent: float4 planes of n chunks
 // (the low halves, then the high halves), so that neighbouring threads read neighbouring 16 bytes.
 template <bool ODD>
@@ -670,6 +679,12 @@ layer_norm_backward_kernel(const LnParams P) {
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) { unpack2<T>(rx[c], xh[c]); unpack2<T>(rg[c], g[c]); }
+        if constexpr (ODD) {
+            // (dy is zero outside the row, and so are its products, unless the zero that stands there for x lies infinitely many rstd from the mean)
+            if (edge && isinf(mean * rstd))
+#pragma unroll
+                for (int c = 0; c < C; ++c) fill_outside(K, tid + c * TPR, mean, xh[c]);
+        }
         load(row + P.step);
         float2 a2 = make_float2(0.f, 0.f), b2 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -814,6 +829,9 @@ __global__ void __launch_bounds__(512, 1) layer_norm_backward_wide_kernel(const 
             float2 xh[4], g[4], w[4];
             take(sx + (par * C + c) * SLOT, chunk, xh);
             take(sg + (par * C + c) * SLOT, chunk, g);
+            if constexpr (ODD) {
+                if (!K.whole(chunk)) fill_outside(K, chunk, mean, xh);      // (0 - mean may be infinitely many rstd)
+            }
             ld_staged(prm, K.n, chunk, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

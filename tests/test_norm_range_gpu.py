@@ -35,8 +35,14 @@ def _check(x, w, b, eps, y, mean, rstd):
     assert ((rstd.double() - rr).abs() <= rel * rr + 2.0 ** -150).all()
     xw = (xhat * w.double()).abs()
     tol = w.double().abs() * (rr * dm)[:, None] + xw * (rel + 4 * U)[:, None] + 2 * U * (xw + b.double().abs()) + _half_step(y.dtype) * ry.abs() * 1.01 + 1e-38
-    bad = (y.double() - ry).abs() > tol
+    bad = ~((y.double() - ry).abs() <= tol)             # (a NaN is bad)
     assert not bad.any(), f"rows {bad.any(1).nonzero().flatten().tolist()}"
+
+
+def _check_gradient(x, dy, w, mean, rstd):
+    got = hk.layer_norm_backward(dy, x, mean, rstd, w)
+    assert all(torch.isfinite(t).all() for t in got)
+    _check_backward(dy, x, mean, rstd, w, *got)
 
 
 def _large(H, dtype):
@@ -80,7 +86,7 @@ def test_gradient_of_large_rows(H, dtype):
     x, dy = _large(H, dtype)[:13], _noise(13, H, 9).to(dtype)
     w, b = _parameters(H, dtype)
     _, mean, rstd = hk.layer_norm(x, w, b)
-    _check_backward(dy, x, mean, rstd, w, *hk.layer_norm_backward(dy, x, mean, rstd, w))
+    _check_gradient(x, dy, w, mean, rstd)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -142,3 +148,15 @@ def test_gradient_sums_that_overflow_stay_infinite(H, dtype):
     mean, rstd = torch.zeros(3, device=DEV), torch.ones(3, device=DEV)
     dx = hk.layer_norm_backward(dy, x, mean, rstd)[0]
     assert torch.isneginf(dx[1]).all() and not dx[[0, 2]].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [33, 256, 700, 1001, 4001, 8190, 9001, 16001, 20001])
+def test_gradient_of_constant_rows_far_from_zero(H, dtype):
+    """Rows of one large value: xhat is 0 and rstd 1 / sqrt(eps), and a mean that is an infinite number of rstd from 0 reaches no element."""
+    x = torch.full((9, H), 2e36, dtype=dtype, device=DEV)
+    x[::2] = _noise(5, H, 3).to(dtype)
+    dy = _noise(9, H, 4).to(dtype)
+    w, b = _parameters(H, dtype)
+    _, mean, rstd = hk.layer_norm(x, w, b)
+    _check_gradient(x, dy, w, mean, rstd)
