@@ -105,6 +105,7 @@ void dispatch_micro(py::object A, py::object B, py::object C, py::object scale_A
     {
         DeviceGuard guard(a.device);
         const uint64_t stream = handles().current_stream(a.device);
+        py::gil_scoped_release unlocked;          // a launch may wait for the device, and the device for a callback that needs the lock
         rc = mxfp6_gemm(reinterpret_cast<const void*>(a.ptr), reinterpret_cast<const void*>(sa.ptr),
                         reinterpret_cast<const void*>(b.ptr), reinterpret_cast<const void*>(sb.ptr),
                         reinterpret_cast<void*>(c.ptr), M, N, K, fmt, fmt, reinterpret_cast<void*>(stream));

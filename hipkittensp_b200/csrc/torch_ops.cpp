@@ -91,7 +91,10 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> o
         if (t->get_device() != a.get_device()) refuse("all tensors must be on the same device");
 }
 
+// Neither an allocation nor a launch holds the interpreter lock: both may wait for the device (a full queue, memory that is freed to make
+// room, the library's first scratch buffer), and what the device waits for may be a callback that needs the lock.
 at::Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
+    py::gil_scoped_release unlocked;
     return at::detail::empty_cuda(size, dtype, like.device(), std::nullopt);
 }
 
@@ -110,8 +113,13 @@ void check(int rc) {
 template <typename F>
 void launch(const at::Tensor& t, F entry) {
     const c10::DeviceIndex dev = (c10::DeviceIndex)t.get_device();
-    c10::cuda::CUDAGuard guard(dev);
-    check(entry((void*)c10::cuda::getCurrentCUDAStream(dev).stream()));
+    int rc;
+    {
+        py::gil_scoped_release unlocked;
+        c10::cuda::CUDAGuard guard(dev);
+        rc = entry((void*)c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    check(rc);
 }
 
 // ---------------------------------------------------------------------------------- products
@@ -260,9 +268,14 @@ py::tuple layer_norm_backward(py::handle DY, py::handle X, py::handle mean, py::
     if (mean.is_none() || rstd.is_none()) refuse("Expected a torch.Tensor");
     const float *m = (const float*)vector_of(mean, "mean", n.rows, n.x, false, nullptr), *r = (const float*)vector_of(rstd, "rstd", n.rows, n.x, false, nullptr);
     at::Tensor dx = empty({n.rows, n.H}, n.x.scalar_type(), n.x), dw = empty({n.H}, at::kFloat, n.x), db = empty({n.H}, at::kFloat, n.x);
+    size_t bytes;
+    {
+        py::gil_scoped_release unlocked;
+        c10::cuda::CUDAGuard guard((c10::DeviceIndex)n.x.get_device());
+        bytes = lib.mxfp6_layer_norm_backward_workspace_bytes(n.rows, n.H);
+    }
+    at::Tensor work = empty({(int64_t)bytes}, at::kByte, n.x);
     launch(n.x, [&](void* st) {
-        const size_t bytes = lib.mxfp6_layer_norm_backward_workspace_bytes(n.rows, n.H);
-        at::Tensor work = empty({(int64_t)bytes}, at::kByte, n.x);
         return lib.mxfp6_layer_norm_backward(dy.const_data_ptr(), n.x.const_data_ptr(), n.code, m, r, n.w, n.wcode, dx.mutable_data_ptr(),
                                          (float*)dw.mutable_data_ptr(), (float*)db.mutable_data_ptr(), n.rows, n.H, work.mutable_data_ptr(), bytes, st);
     });

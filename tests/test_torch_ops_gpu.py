@@ -1,0 +1,84 @@
+"""The compiled wrappers (_torch_ops): what they hold and raise around a call of the library.  The library is replaced by one whose entry
+points sleep, or given no memory; no kernel is involved."""
+import ctypes
+import os
+import re
+import subprocess
+import threading
+import time
+
+import pytest
+import torch
+
+import hipkittensp_b200 as hk
+from hipkittensp_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+PKG = os.path.dirname(os.path.abspath(hk.__file__))
+
+
+@pytest.fixture(scope="module")
+def sleeping_library(tmp_path_factory):
+    """Every entry point the wrappers use, each taking 0.4 s and doing nothing."""
+    src = open(os.path.join(PKG, "csrc", "torch_ops.cpp")).read()
+    names = re.findall(r"X\((mxfp6_\w+)\)", src)
+    assert "mxfp6_gemm_ws" in names and "mxfp6_layer_norm_backward" in names
+    body = "#include <stddef.h>\n#include <unistd.h>\n"
+    for n in names:
+        if n == "mxfp6_last_error":
+            body += f'const char* {n}(void) {{ return "none"; }}\n'
+        elif n.endswith("_bytes"):
+            body += f"size_t {n}(void) {{ return 256; }}\n"
+        else:
+            body += f"int {n}(void) {{ usleep(400000); return 0; }}\n"
+    d = tmp_path_factory.mktemp("lib")
+    c, so = d / "sleep.c", d / "libsleep.so"
+    c.write_text(body)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(so), str(c)], check=True)
+    return ctypes.CDLL(str(so))
+
+
+def _calls():
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8, device="cuda")
+    a, s, x = u8(32, 128), u8(32, 4), torch.zeros(32, 128, device="cuda")
+    stat = torch.zeros(32, device="cuda")
+    return {
+        "gemm": lambda: hk.gemm(a, s, a, s, fmt=hk.E4M3),
+        "gemm with a workspace": lambda: hk.gemm(a, s, a, s, fmt=hk.E4M3, workspace=u8(512)),
+        "gemm_scaled": lambda: hk.gemm_scaled(a, s, a, s, fmt=hk.E4M3),
+        "quantize": lambda: hk.quantize(x),
+        "dequantize": lambda: hk.dequantize(a, s, hk.E4M3),
+        "layer_norm": lambda: hk.layer_norm(x),
+        "layer_norm_quantize": lambda: hk.layer_norm_quantize(x),
+        "layer_norm_backward": lambda: hk.layer_norm_backward(x, x, stat, stat),
+    }
+
+
+def test_other_threads_run_while_a_call_waits(sleeping_library):
+    """A call that waits in the library lets Python's other threads run: a launch may block on a full queue, whose callbacks may need
+    the interpreter."""
+    calls = _calls()
+    ticks, stop = [], threading.Event()
+
+    def tick():
+        while not stop.wait(0.01):
+            ticks.append(time.monotonic())
+
+    thread = threading.Thread(target=tick)
+    _lib.ops.bind(sleeping_library._handle, _lib.Mxfp6Error)
+    try:
+        thread.start()
+        for name, call in calls.items():
+            t0 = time.monotonic()
+            call()
+            t1 = time.monotonic()
+            assert t1 - t0 >= 0.35, name
+            # (at most every 10 ms in 400: a quarter of what may be)
+            assert sum(t0 + 0.02 < t < t1 - 0.02 for t in ticks) >= 10, f"{name} held the interpreter"
+    finally:
+        stop.set()
+        thread.join()
+        _lib.ops.bind(_lib.lib._handle, _lib.Mxfp6Error)
+    x = torch.randn(8, 64, device="cuda")
+    assert torch.isfinite(hk.layer_norm(x)[0]).all()
