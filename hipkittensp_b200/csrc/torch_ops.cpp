@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
@@ -286,6 +287,14 @@ py::tuple layer_norm_backward(py::handle DY, py::handle X, py::handle mean, py::
 
 PYBIND11_MODULE(_torch_ops, m) {
     m.doc() = "tensor-level entry points over libmxfp6 (see gemm.py and norm.py)";
+    // errors of torch's allocator keep their Python types (torch.OutOfMemoryError among them)
+    py::register_local_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const c10::Error&) {
+            torch::translate_exception_to_python(p);
+        }
+    });
     m.def("bind", [](uintptr_t handle, py::object error_class) {
 #define X(name)                                                                              \
         lib.name = reinterpret_cast<decltype(&::name)>(dlsym(reinterpret_cast<void*>(handle), #name)); \

@@ -82,3 +82,19 @@ def test_other_threads_run_while_a_call_waits(sleeping_library):
         _lib.ops.bind(_lib.lib._handle, _lib.Mxfp6Error)
     x = torch.randn(8, 64, device="cuda")
     assert torch.isfinite(hk.layer_norm(x)[0]).all()
+
+
+def test_out_of_memory_keeps_its_type():
+    """A result that does not fit raises torch.OutOfMemoryError, as torch.empty does."""
+    codes, scales = torch.zeros(4096, 65536, dtype=torch.uint8, device="cuda"), torch.zeros(4096, 4096, dtype=torch.uint8, device="cuda")
+    x = torch.zeros(1 << 16, 4096, device="cuda")
+    torch.cuda.empty_cache()
+    held = torch.cuda.memory_reserved() + (64 << 20)
+    torch.cuda.set_per_process_memory_fraction(held / torch.cuda.get_device_properties(0).total_memory)
+    try:
+        for call in (lambda: torch.empty(1 << 30, device="cuda"), lambda: hk.dequantize(codes, scales, hk.E2M1), lambda: hk.quantize(x), lambda: hk.layer_norm(x)):
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert hk.layer_norm(x[:8])[0].shape == (8, 4096)
