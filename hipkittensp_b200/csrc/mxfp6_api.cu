@@ -138,6 +138,18 @@ struct DeviceState {
 static std::mutex g_mu;
 static DeviceState g_dev[64];
 
+// Zeros device memory before it returns.  On a stream of its own: a plain cudaMemset is queued on the legacy default stream, behind whatever
+// that holds and unordered with the non-blocking streams a kernel that uses the memory may be launched on next.
+static int zero_now(void* p, size_t bytes) {
+    cudaStream_t s = nullptr;
+    CUDA_TRY(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking));
+    cudaError_t e = cudaMemsetAsync(p, 0, bytes, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    (void)cudaStreamDestroy(s);
+    CUDA_TRY(e);
+    return MXFP6_OK;
+}
+
 static int get_device_state(DeviceState** out, int* dev_out = nullptr) {
     int dev = 0;
     CUDA_TRY(cudaGetDevice(&dev));
@@ -153,7 +165,7 @@ static int get_device_state(DeviceState** out, int* dev_out = nullptr) {
         if (d.cc_major != 10) return fail(MXFP6_ERR_UNSUPPORTED, "device %d is sm_%d0; this library is sm_100a only", dev, d.cc_major);
         d.wait_cycles = (unsigned long long)khz * (unsigned long long)options().wait_ms;
         CUDA_TRY(cudaGetSymbolAddress((void**)&d.status, g_status_word));
-        CUDA_TRY(cudaMemset(d.status, 0, sizeof(int) * 4));
+        if (const int rc = zero_now(d.status, sizeof(int) * 4)) return rc;
         d.init = true;
     }
     *out = &d;
@@ -550,7 +562,10 @@ static int own_scratch(DeviceState& d, size_t bytes, cudaStream_t st, void** out
             want = bytes;
             CUDA_TRY(cudaMalloc(&p, want));
         }
-        CUDA_TRY(cudaMemset(p, 0, want));
+        if (const int rc = zero_now(p, want)) {
+            (void)cudaFree(p);
+            return rc;
+        }
         d.ws_all.emplace_back(p, want);
         d.ws = p;
         d.ws_bytes = want;
@@ -1300,10 +1315,11 @@ extern "C" int mxfp6_device_status(int* status_out) {
     CUDA_TRY(cudaMemcpy(h, d->status, sizeof h, cudaMemcpyDeviceToHost));
     if (status_out) *status_out = h[0];
     if (h[0] != 0) {
-        CUDA_TRY(cudaMemset(d->status, 0, sizeof h));
+        if ((rc = zero_now(d->status, sizeof h))) return rc;
         // arrival counters of split tiles may be left non-zero by an aborted launch
         std::lock_guard<std::mutex> lk(g_mu);
-        for (auto& w : d->ws_all) CUDA_TRY(cudaMemset(w.first, 0, w.second));
+        for (auto& w : d->ws_all)
+            if ((rc = zero_now(w.first, w.second))) return rc;
         return fail(MXFP6_ERR_DEVICE_WAIT, "a bounded wait ran out on the device: role %d, CTA %d", h[0] & 0xff, h[0] >> 8);
     }
     return MXFP6_OK;
