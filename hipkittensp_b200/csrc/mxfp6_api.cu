@@ -466,12 +466,32 @@ static bool dest_by_tma(const Dest& dst) {
     for (int i = 0; i < dst.n; ++i) ok = ok && !((uintptr_t)dst.c[i] & 15);
     return ok;
 }
-static Plan plan_for(const void* sfa, const void* sfb, const Dest& dst, int64_t M, int64_t N, int64_t K, int sm_count,
-                     bool requant = false, int kelems = 128, int min_rows = 80) {
+// What the operands' formats say about the plan.
+struct FormatPlan { bool f4; int kelems, min_rows; };
+static FormatPlan format_plan(int fmt_a, int fmt_b, int64_t K) {
+    const bool a4 = fmt_a == MXFP4_E2M1, b4 = fmt_b == MXFP4_E2M1, f4 = a4 && b4 && options().f4;      // the 4-bit MMA takes two E2M1 operands
+    // 4-bit weights or activations: the even-rows form pays from fewer rows per CTA than for the wider formats (whose rule is left as
+    // it was).  Its time goes with K alone, the K-split form's with N * K; M = 16, even-rows / K-split: 70 rows (N = 20480), K = 8192
+    // 18.2 / 21.0 us for E2M1 x E2M1 and 27.2 / 29.6 us for E4M3 x E2M1; 49 rows, K = 4096 11.5 / 13.5 and 16.2 / 16.3 us;
+    // 49 rows, K = 8192 17.7 / 17.3 and 27.2 / 23.5 us.
+    return {f4, f4 ? 256 : 128, a4 || b4 ? (K <= 4096 ? 48 : 64) : 80};
+}
+// The one choice of every entry point, and of the test hook.
+static Plan plan_for(int n_dst, int64_t M, int64_t N, int64_t K, int sm_count, bool requant, int fmt_a, int fmt_b) {
     // several destinations are written untransposed from whole tiles; a re-quantised result needs tiles that start on
     // multiples of 32 rows and columns
-    (void)sfa; (void)sfb; (void)dst;
-    return make_plan(M, N, K, sm_count, true, dst.n > 1, !requant, kelems, min_rows);
+    const FormatPlan f = format_plan(fmt_a, fmt_b, K);
+    return make_plan(M, N, K, sm_count, true, n_dst > 1, !requant, f.kelems, f.min_rows);
+}
+// Scratch that serves a problem of any formats: the most that a kind of plan asks for.
+static size_t scratch_for_any(int64_t M, int64_t N, int64_t K, int sm_count) {
+    size_t most = 0;
+    for (int fa : {MXFP6_E2M3, MXFP4_E2M1})
+        for (int fb : {MXFP6_E2M3, MXFP4_E2M1}) {
+            const size_t n = plan_for(1, M, N, K, sm_count, false, fa, fb).ws_bytes;
+            if (n > most) most = n;
+        }
+    return most;
 }
 
 // Everything a call passes in.  Two calls with equal keys launch the same kernel with the same arguments, so the
@@ -630,14 +650,9 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     DeviceState& d = *dp;
     const Options& o = options();
     const bool sf_tma = scales_by_tma(sfa, sfb, K);
-    const bool f4 = fmt_a == MXFP4_E2M1 && fmt_b == MXFP4_E2M1 && o.f4;      // the 4-bit MMA takes two E2M1 operands
-    const int kelems = f4 ? 256 : 128;
-    // 4-bit weights or activations: the even-rows form pays from fewer rows per CTA than for the wider formats (whose rule is left as
-    // it was).  Its time goes with K alone, the K-split form's with N * K; M = 16, even-rows / K-split: 70 rows (N = 20480), K = 8192
-    // 18.2 / 21.0 us for E2M1 x E2M1 and 27.2 / 29.6 us for E4M3 x E2M1; 49 rows, K = 4096 11.5 / 13.5 and 16.2 / 16.3 us;
-    // 49 rows, K = 8192 17.7 / 17.3 and 27.2 / 23.5 us.
-    const int min_rows = fmt_a == MXFP4_E2M1 || fmt_b == MXFP4_E2M1 ? (K <= 4096 ? 48 : 64) : 80;
-    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d.sm_count, q_fmt >= 0, kelems, min_rows);
+    const bool f4 = format_plan(fmt_a, fmt_b, K).f4;
+    const int kelems = format_plan(fmt_a, fmt_b, K).kelems;
+    const Plan pl = plan_for(dst.n, M, N, K, d.sm_count, q_fmt >= 0, fmt_a, fmt_b);
 
     Recipe r;
     r.key = key;
@@ -920,10 +935,7 @@ extern "C" size_t mxfp6_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
     DeviceState* d = nullptr;
     if (get_device_state(&d)) return 0;
-    // the formats are not known here: the 4-bit path splits its (longer) K-blocks a little differently
-    const size_t wide = make_plan(M, N, K, d->sm_count).ws_bytes;
-    const size_t f4 = make_plan(M, N, K, d->sm_count, true, false, true, 256).ws_bytes;
-    return wide > f4 ? wide : f4;
+    return scratch_for_any(M, N, K, d->sm_count);
 }
 
 extern "C" int mxfp6_gemm_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,
@@ -1139,7 +1151,8 @@ extern "C" int mxfp6_gemm_noalloc(const void* a, const void* sfa, const void* b,
         scratch = g_builtin_scratch_addr[dev];
     }
     const Dest dst{{c}, 1, N};
-    const Plan pl = plan_for(sfa, sfb, dst, M, N, K, d->sm_count);      // the plan the common path will make
+    if (!fmt_valid(fmt_a) || !fmt_valid(fmt_b)) return fail(MXFP6_ERR_BAD_ARG, "format must be " MXFP6_FORMATS);
+    const Plan pl = plan_for(1, M, N, K, d->sm_count, false, fmt_a, fmt_b);      // the plan the common path will make
     if (pl.ws_bytes > kBuiltinScratchBytes)
         return fail(MXFP6_ERR_BAD_ARG,
                     "mxfp6_gemm_noalloc: M=%lld N=%lld K=%lld needs %zu bytes of scratch but the built-in buffer holds %zu; "
@@ -1349,9 +1362,15 @@ extern "C" int mxfp6_debug_option(const char* name, const char* value) {
 }
 
 extern "C" int mxfp6_debug_plan(int64_t M, int64_t N, int64_t K, int sm_count, int n_dst, int requant, int* out12) {
-    if (!out12 || M <= 0 || N <= 0 || K <= 0 || K % 128 || sm_count < 2 || n_dst < 1 || n_dst > 8)
+    return mxfp6_debug_plan_fmt(M, N, K, sm_count, n_dst, requant, MXFP6_E2M3, MXFP6_E2M3, out12, nullptr);
+}
+
+extern "C" int mxfp6_debug_plan_fmt(int64_t M, int64_t N, int64_t K, int sm_count, int n_dst, int requant, int fmt_a, int fmt_b, int* out12,
+                                    size_t* scratch2) {
+    if (!out12 || M <= 0 || N <= 0 || K <= 0 || K % 128 || sm_count < 2 || n_dst < 1 || n_dst > 8 || !fmt_valid(fmt_a) || !fmt_valid(fmt_b))
         return fail(MXFP6_ERR_BAD_ARG, "debug_plan: bad argument");
-    const Plan p = make_plan(M, N, K, sm_count, true, n_dst > 1, !requant);
+    const Plan p = plan_for(n_dst, M, N, K, sm_count, requant != 0, fmt_a, fmt_b);
+    if (scratch2) { scratch2[0] = p.ws_bytes; scratch2[1] = scratch_for_any(M, N, K, sm_count); }
     const int v[12] = {p.bn, p.swap, p.streamk, p.pair, p.ctas, p.p_tile, p.q_tile, p.tiles_p, p.tiles_q, p.grid,
                        p.tail_first, p.tail_split};
     memcpy(out12, v, sizeof v);

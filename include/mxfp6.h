@@ -278,6 +278,10 @@ int mxfp6_debug_option(const char* name, const char* value);
  * the reference, whose tiling is fixed at compile time: kernels/gemm/bf16fp32/256_256_64_32_with16x32.cpp:23-32.)
  */
 int mxfp6_debug_plan(int64_t M, int64_t N, int64_t K, int sm_count, int n_dst, int requant, int* out12);
+/* ... for operands of these formats (the form above answers for E2M3; K-blocks and the rule for skinny problems differ for E2M1), and,
+ * unless NULL, the scratch bytes that this plan needs and those that mxfp6_gemm_workspace_bytes reports for the shape. */
+int mxfp6_debug_plan_fmt(int64_t M, int64_t N, int64_t K, int sm_count, int n_dst, int requant, int fmt_a, int fmt_b, int* out12,
+                         size_t* scratch2);
 
 /*
  * Diagnostic: TMA-loads one 128-row x 128-element box of a packed operand (rows row0.., elements
