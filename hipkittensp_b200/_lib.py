@@ -20,7 +20,7 @@ OK, ERR_BAD_ARG, ERR_CUDA, ERR_DEVICE_WAIT, ERR_UNSUPPORTED = 0, 1, 2, 3, 4
 
 # every symbol include/mxfp6.h declares
 SYMBOLS = ("mxfp6_version", "mxfp6_last_error", "mxfp6_gemm", "mxfp6_gemm_workspace_bytes", "mxfp6_gemm_ws",
-           "mxfp6_gemm_noalloc", "mxfp6_gemm_multi", "mxfp6_gemm_copy_gather", "mxfp6_copy_gather_scratch_bytes", "mxfp6_gemm_ex", "mxfp6_gemm_requant", "mxfp6_gemm_scaled",
+           "mxfp6_gemm_ex_ws", "mxfp6_gemm_requant_ws", "mxfp6_gemm_scaled_ws", "mxfp6_gemm_multi_ws", "mxfp6_gemm_noalloc", "mxfp6_gemm_multi", "mxfp6_gemm_copy_gather", "mxfp6_copy_gather_scratch_bytes", "mxfp6_gemm_ex", "mxfp6_gemm_requant", "mxfp6_gemm_scaled",
            "mxfp6_quantize", "mxfp6_dequantize", "mxfp6_dequantize_ex", "mxfp6_layer_norm", "mxfp6_layer_norm_quantize", "mxfp6_layer_norm_backward",
            "mxfp6_layer_norm_backward_workspace_bytes", "mxfp6_device_status", "mxfp6_debug_tma_dump", "mxfp6_debug_wait_timeout", "mxfp6_debug_option", "mxfp6_debug_plan", "mxfp6_debug_plan_fmt")
 
@@ -66,6 +66,9 @@ def _load() -> ctypes.CDLL:
     lib.mxfp6_gemm_workspace_bytes.argtypes = [i64, i64, i64]
     lib.mxfp6_gemm_ws.restype = ci
     lib.mxfp6_gemm_ws.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, ci, ci, vp, sz, vp]
+    for name in ("ex", "requant", "scaled", "multi"):            # the same with a workspace and its size in front of the stream
+        plain, with_ws = getattr(lib, "mxfp6_gemm_" + name), getattr(lib, f"mxfp6_gemm_{name}_ws")
+        with_ws.restype, with_ws.argtypes = ci, plain.argtypes[:-1] + [vp, sz, vp]
     lib.mxfp6_quantize.restype = ci
     lib.mxfp6_quantize.argtypes = [vp, ci, i64, i64, ci, vp, vp, vp]
     lib.mxfp6_dequantize.restype = ci

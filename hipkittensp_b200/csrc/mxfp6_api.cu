@@ -483,13 +483,15 @@ static Plan plan_for(int n_dst, int64_t M, int64_t N, int64_t K, int sm_count, b
     const FormatPlan f = format_plan(fmt_a, fmt_b, K);
     return make_plan(M, N, K, sm_count, true, n_dst > 1, !requant, f.kelems, f.min_rows);
 }
-// Scratch that serves a problem of any formats: the most that a kind of plan asks for.
+// Scratch that serves a problem of any formats, with a plain or a re-quantised result: the most that a kind of plan asks for.
 static size_t scratch_for_any(int64_t M, int64_t N, int64_t K, int sm_count) {
     size_t most = 0;
     for (int fa : {MXFP6_E2M3, MXFP4_E2M1})
         for (int fb : {MXFP6_E2M3, MXFP4_E2M1}) {
-            const size_t n = plan_for(1, M, N, K, sm_count, false, fa, fb).ws_bytes;
-            if (n > most) most = n;
+            for (const bool requant : {false, true}) {       // (a re-quantised result stays split where the plain product is not)
+                const size_t n = plan_for(1, M, N, K, sm_count, requant, fa, fb).ws_bytes;
+                if (n > most) most = n;
+            }
         }
     return most;
 }
@@ -943,14 +945,28 @@ extern "C" int mxfp6_gemm_ws(const void* a, const void* sfa, const void* b, cons
     return gemm_impl(a, sfa, b, sfb, Dest{{c}, 1, N}, M, N, K, fmt_a, fmt_b, workspace, workspace_bytes, kWsCaller, stream);
 }
 
-extern "C" int mxfp6_gemm_ex(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,
-                             int64_t K, int fmt_a, int fmt_b, unsigned flags, void* stream) {
+// scratch for a call: the library's, or the caller's
+struct Scratch { WsMode mode; void* ws; size_t bytes; };
+constexpr Scratch kOwnScratch{kWsOwn, nullptr, 0};
+
+static int gemm_ex(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N, int64_t K, int fmt_a,
+                   int fmt_b, unsigned flags, const Scratch& s, void* stream) {
     if (flags & ~(unsigned)MXFP6_FLAG_B_STATIC) return fail(MXFP6_ERR_BAD_ARG, "unknown flag bits 0x%x", flags);
-    return gemm_impl(a, sfa, b, sfb, Dest{{c}, 1, N}, M, N, K, fmt_a, fmt_b, nullptr, 0, kWsOwn, stream, flags);
+    return gemm_impl(a, sfa, b, sfb, Dest{{c}, 1, N}, M, N, K, fmt_a, fmt_b, s.ws, s.bytes, s.mode, stream, flags);
 }
 
-extern "C" int mxfp6_gemm_requant(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales,
-                                  int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, int out_fmt, void* stream) {
+extern "C" int mxfp6_gemm_ex(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,
+                             int64_t K, int fmt_a, int fmt_b, unsigned flags, void* stream) {
+    return gemm_ex(a, sfa, b, sfb, c, M, N, K, fmt_a, fmt_b, flags, kOwnScratch, stream);
+}
+
+extern "C" int mxfp6_gemm_ex_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,
+                                int64_t K, int fmt_a, int fmt_b, unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] { return gemm_ex(a, sfa, b, sfb, c, M, N, K, fmt_a, fmt_b, flags, {kWsCaller, workspace, workspace_bytes}, stream); });
+}
+
+static int gemm_requant(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales, int64_t M, int64_t N,
+                        int64_t K, int fmt_a, int fmt_b, int out_fmt, const Scratch& s, void* stream) {
     if (!fmt_valid(out_fmt)) return fail(MXFP6_ERR_BAD_ARG, "requant: bad output format %d", out_fmt);
     if (N % 64 != 0) return fail(MXFP6_ERR_BAD_ARG, "requant: N=%lld must be a multiple of 64", (long long)N);
     if (M > 0 && N > 0 && (!out || !out_scales)) return fail(MXFP6_ERR_BAD_ARG, "requant: null output");
@@ -961,7 +977,18 @@ extern "C" int mxfp6_gemm_requant(const void* a, const void* sfa, const void* b,
         CUDA_TRY(cudaMemsetAsync(out_scales, 0, (size_t)M * (N / 32), (cudaStream_t)stream));
         return MXFP6_OK;
     }
-    return gemm_impl(a, sfa, b, sfb, Dest{{out}, 1, N}, M, N, K, fmt_a, fmt_b, nullptr, 0, kWsOwn, stream, 0, out, out_scales, out_fmt);
+    return gemm_impl(a, sfa, b, sfb, Dest{{out}, 1, N}, M, N, K, fmt_a, fmt_b, s.ws, s.bytes, s.mode, stream, 0, out, out_scales, out_fmt);
+}
+
+extern "C" int mxfp6_gemm_requant(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales,
+                                  int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, int out_fmt, void* stream) {
+    return gemm_requant(a, sfa, b, sfb, out, out_scales, M, N, K, fmt_a, fmt_b, out_fmt, kOwnScratch, stream);
+}
+
+extern "C" int mxfp6_gemm_requant_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales,
+                                     int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, int out_fmt, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+    return guarded([&] { return gemm_requant(a, sfa, b, sfb, out, out_scales, M, N, K, fmt_a, fmt_b, out_fmt, {kWsCaller, workspace, workspace_bytes}, stream); });
 }
 
 // C = bias broadcast along rows: what the scaled GEMM yields for K = 0
@@ -970,9 +997,8 @@ __global__ void bias_fill_kernel(__nv_bfloat16* c, const float* bias, int64_t M,
         c[i] = __float2bfloat16_rn(__fadd_rn(0.f, bias[i % N]));
 }
 
-extern "C" int mxfp6_gemm_scaled(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
-                                 const float* scale_a, const float* scale_b, const float* bias,
-                                 int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, void* stream) {
+static int gemm_scaled(const void* a, const void* sfa, const void* b, const void* sfb, void* c, const float* scale_a, const float* scale_b,
+                       const float* bias, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, const Scratch& s, void* stream) {
     if (((uintptr_t)scale_a & 3) || ((uintptr_t)scale_b & 15) || ((uintptr_t)bias & 15))
         return fail(MXFP6_ERR_BAD_ARG, "scaled: scale_a must be 4-byte aligned, scale_b and bias 16-byte aligned");
     if (K == 0 && bias && M > 0 && N > 0) {
@@ -986,19 +1012,43 @@ extern "C" int mxfp6_gemm_scaled(const void* a, const void* sfa, const void* b, 
     }
     Affine aff;
     aff.scale_m = scale_a; aff.scale_n = scale_b; aff.bias_n = bias;
-    return gemm_impl(a, sfa, b, sfb, Dest{{c}, 1, N}, M, N, K, fmt_a, fmt_b, nullptr, 0, kWsOwn, stream, 0, nullptr, nullptr, -1, aff);
+    return gemm_impl(a, sfa, b, sfb, Dest{{c}, 1, N}, M, N, K, fmt_a, fmt_b, s.ws, s.bytes, s.mode, stream, 0, nullptr, nullptr, -1, aff);
 }
 
-extern "C" int mxfp6_gemm_multi(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
-                                int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
-                                void* stream) {
+extern "C" int mxfp6_gemm_scaled(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
+                                 const float* scale_a, const float* scale_b, const float* bias,
+                                 int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, void* stream) {
+    return gemm_scaled(a, sfa, b, sfb, c, scale_a, scale_b, bias, M, N, K, fmt_a, fmt_b, kOwnScratch, stream);
+}
+
+extern "C" int mxfp6_gemm_scaled_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
+                                    const float* scale_a, const float* scale_b, const float* bias,
+                                    int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+    return guarded([&] { return gemm_scaled(a, sfa, b, sfb, c, scale_a, scale_b, bias, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream); });
+}
+
+static int gemm_multi(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst, int n_dst, int64_t ldc, int64_t M,
+                      int64_t N, int64_t K, int fmt_a, int fmt_b, const Scratch& s, void* stream) {
     if (!c_dst) return fail(MXFP6_ERR_BAD_ARG, "null destination list");
     if (n_dst < 1 || n_dst > 8) return fail(MXFP6_ERR_BAD_ARG, "1 to 8 destinations, got %d", n_dst);
     Dest d{};
     for (int i = 0; i < n_dst; ++i) d.c[i] = c_dst[i];
     d.n = n_dst;
     d.ldc = ldc;
-    return gemm_impl(a, sfa, b, sfb, d, M, N, K, fmt_a, fmt_b, nullptr, 0, kWsOwn, stream);
+    return gemm_impl(a, sfa, b, sfb, d, M, N, K, fmt_a, fmt_b, s.ws, s.bytes, s.mode, stream);
+}
+
+extern "C" int mxfp6_gemm_multi(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
+                                int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
+                                void* stream) {
+    return gemm_multi(a, sfa, b, sfb, c_dst, n_dst, ldc, M, N, K, fmt_a, fmt_b, kOwnScratch, stream);
+}
+
+extern "C" int mxfp6_gemm_multi_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
+                                   int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] { return gemm_multi(a, sfa, b, sfb, c_dst, n_dst, ldc, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream); });
 }
 
 // ---------------------------------------------------------------------------------- GEMM with a copy-engine gather

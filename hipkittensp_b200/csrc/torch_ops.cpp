@@ -23,7 +23,7 @@ namespace py = pybind11;
 namespace {
 
 // The entry points of the library instance the package has loaded (it may be another build than the one next to this file).
-#define MX_ENTRIES(X) X(mxfp6_last_error) X(mxfp6_gemm_ex) X(mxfp6_gemm_ws) X(mxfp6_gemm_scaled) X(mxfp6_quantize) X(mxfp6_dequantize_ex) X(mxfp6_layer_norm) \
+#define MX_ENTRIES(X) X(mxfp6_last_error) X(mxfp6_gemm_ex) X(mxfp6_gemm_ws) X(mxfp6_gemm_scaled) X(mxfp6_gemm_scaled_ws) X(mxfp6_quantize) X(mxfp6_dequantize_ex) X(mxfp6_layer_norm) \
     X(mxfp6_layer_norm_quantize) X(mxfp6_layer_norm_backward) X(mxfp6_layer_norm_backward_workspace_bytes)
 struct Library {
 #define X(name) decltype(&::name) name = nullptr;
@@ -145,31 +145,36 @@ at::Tensor result(const Operands& o, py::handle out) {
     return c;
 }
 
+// a caller's workspace, or none
+struct Workspace {
+    bool own = true;             // the library's
+    void* ptr = nullptr;
+    size_t bytes = 0;
+};
+Workspace workspace_of(const Operands& o, py::handle workspace) {
+    if (workspace.is_none()) return {};
+    const at::Tensor& w = tensor_of(workspace);
+    if (!w.is_contiguous()) refuse("Tensor must be contiguous");
+    if (w.scalar_type() != at::kByte) refuse("workspace must be torch.uint8");
+    if (!w.is_cuda() || w.get_device() != o.a.get_device()) refuse("all tensors must be on the same device");
+    return {false, w.mutable_data_ptr(), (size_t)w.numel()};
+}
+
 py::object gemm(py::handle A, py::handle scale_A, py::handle B, py::handle scale_B, int fmt, int fmt_b, py::handle out, py::handle workspace) {
     const Operands o = operands(A, scale_A, B, scale_B, fmt, fmt_b);
     if (o.K % 128) refuse("K must be a multiple of 128");
-    void* ws = nullptr;
-    size_t ws_bytes = 0;
-    const bool own = workspace.is_none();
-    if (!own) {
-        const at::Tensor& w = tensor_of(workspace);
-        if (!w.is_contiguous()) refuse("Tensor must be contiguous");
-        if (w.scalar_type() != at::kByte) refuse("workspace must be torch.uint8");
-        if (!w.is_cuda() || w.get_device() != o.a.get_device()) refuse("all tensors must be on the same device");
-        ws = w.mutable_data_ptr();
-        ws_bytes = (size_t)w.numel();
-    }
+    const Workspace ws = workspace_of(o, workspace);
     at::Tensor c = result(o, out);
     launch(o.a, [&](void* st) {
         const void *a = o.a.const_data_ptr(), *sa = o.sa.const_data_ptr(), *b = o.b.const_data_ptr(), *sb = o.sb.const_data_ptr();
-        return own ? lib.mxfp6_gemm_ex(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, 0, st)
-                   : lib.mxfp6_gemm_ws(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, ws, ws_bytes, st);
+        return ws.own ? lib.mxfp6_gemm_ex(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, 0, st)
+                      : lib.mxfp6_gemm_ws(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, ws.ptr, ws.bytes, st);
     });
     return out.is_none() ? wrap(std::move(c)) : py::reinterpret_borrow<py::object>(out);
 }
 
 py::object gemm_scaled(py::handle A, py::handle scale_A, py::handle B, py::handle scale_B, py::handle row_scale, py::handle col_scale, py::handle bias,
-                       int fmt, int fmt_b, py::handle out) {
+                       int fmt, int fmt_b, py::handle out, py::handle workspace) {
     const Operands o = operands(A, scale_A, B, scale_B, fmt, fmt_b);
     auto vec = [&](py::handle h, const char* name, int64_t n) -> const float* {
         if (h.is_none()) return nullptr;
@@ -181,10 +186,12 @@ py::object gemm_scaled(py::handle A, py::handle scale_A, py::handle B, py::handl
         return (const float*)t.const_data_ptr();
     };
     const float *r = vec(row_scale, "row_scale", o.M), *cs = vec(col_scale, "col_scale", o.N), *bs = vec(bias, "bias", o.N);
+    const Workspace ws = workspace_of(o, workspace);
     at::Tensor c = result(o, out);
     launch(o.a, [&](void* st) {
-        return lib.mxfp6_gemm_scaled(o.a.const_data_ptr(), o.sa.const_data_ptr(), o.b.const_data_ptr(), o.sb.const_data_ptr(), c.mutable_data_ptr(), r, cs, bs,
-                                 o.M, o.N, o.K, fmt, fmt_b, st);
+        const void *a = o.a.const_data_ptr(), *sa = o.sa.const_data_ptr(), *b = o.b.const_data_ptr(), *sb = o.sb.const_data_ptr();
+        return ws.own ? lib.mxfp6_gemm_scaled(a, sa, b, sb, c.mutable_data_ptr(), r, cs, bs, o.M, o.N, o.K, fmt, fmt_b, st)
+                      : lib.mxfp6_gemm_scaled_ws(a, sa, b, sb, c.mutable_data_ptr(), r, cs, bs, o.M, o.N, o.K, fmt, fmt_b, ws.ptr, ws.bytes, st);
     });
     return out.is_none() ? wrap(std::move(c)) : py::reinterpret_borrow<py::object>(out);
 }

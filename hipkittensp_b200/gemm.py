@@ -68,14 +68,27 @@ def _launch(t, entry, *args) -> None:
         check(rc)
 
 
-def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None = None, b_static: bool = False) -> None:
+def _workspace(t, device: int) -> tuple[int, int]:
+    """Address and bytes of a caller's workspace."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError("Expected a torch.Tensor")
+    if not t.is_contiguous():
+        raise RuntimeError("Tensor must be contiguous")
+    if t.dtype != torch.uint8:
+        raise RuntimeError("workspace must be torch.uint8")
+    if not t.is_cuda or t.get_device() != device:
+        raise RuntimeError("all tensors must be on the same device")
+    return t.data_ptr(), t.numel()
+
+
+def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None = None, b_static: bool = False, workspace=None) -> None:
     """C[M,N] (bf16, in place) = A[M,K] @ B[N,K]^T.
 
     A [M,3K/4] u8 and B [N,3K/4] u8 are packed fp6, [rows,K] u8 for the fp8 formats or [rows,K/2] u8 for fp4 (format
     `fmt`; `fmt_b` if B differs),
     scale_A [M,K/32] u8 and scale_B [N,K/32] u8 are E8M0 bytes.  M is taken from A, N from C,
     K from A, as the reference does (256_256_64_32_with16x32.cpp:52-54).  b_static=True promises that B and
-    scale_B are not written by the work queued just before this call (see MXFP6_FLAG_B_STATIC)."""
+    scale_B are not written by the work queued just before this call (see MXFP6_FLAG_B_STATIC).  workspace: as gemm() takes it."""
     _accept(A, "A", torch.uint8)
     _accept(B, "B", torch.uint8)
     _accept(C, "C", torch.bfloat16)
@@ -95,15 +108,17 @@ def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None
     device = A.get_device()
     if B.get_device() != device or C.get_device() != device or scale_A.get_device() != device or scale_B.get_device() != device:
         raise RuntimeError("all tensors must be on the same device")
-    _launch(A, lib.mxfp6_gemm_ex, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), C.data_ptr(),
-            M, N, K, fmt, fb, _lib.FLAG_B_STATIC if b_static else 0)
+    ws = () if workspace is None else _workspace(workspace, device)
+    _launch(A, lib.mxfp6_gemm_ex_ws if ws else lib.mxfp6_gemm_ex, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), C.data_ptr(),
+            M, N, K, fmt, fb, _lib.FLAG_B_STATIC if b_static else 0, *ws)
 
 
-def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2M3) -> None:
+def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2M3, workspace=None) -> None:
     """The [M,N] product written into the column window [col_offset, col_offset+N) of every matrix in `dests`.
 
     dests: bf16 tensors [M, ldc] that share one row stride; dests[0] is local, the others may be views of
-    peer GPUs' memory (symmetric memory): the kernel's epilogue pushes each finished tile to all of them."""
+    peer GPUs' memory (symmetric memory): the kernel's epilogue pushes each finished tile to all of them.
+    workspace: as gemm() takes it, of use with one destination (several are never written from partial sums)."""
     import ctypes
 
     _accept(A, "A", torch.uint8)
@@ -124,8 +139,9 @@ def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2
         if col_offset < 0 or col_offset + N > d.shape[1]:
             raise RuntimeError("column window outside the destination")
     ptrs = (ctypes.c_void_p * len(dests))(*[d.data_ptr() + 2 * col_offset for d in dests])
-    _launch(A, lib.mxfp6_gemm_multi, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
-            ldc, M, N, K, fmt, fmt)
+    ws = () if workspace is None else _workspace(workspace, A.get_device())
+    _launch(A, lib.mxfp6_gemm_multi_ws if ws else lib.mxfp6_gemm_multi, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
+            ldc, M, N, K, fmt, fmt, *ws)
 
 
 def _check_scales(A, B, scale_A, scale_B, K: int) -> None:
@@ -174,9 +190,9 @@ def dispatch_copy_gather(A, B, dests, col_offset: int, scale_A, scale_B, scratch
             strip_tiles, streams, len(copy_streams))
 
 
-def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out_fmt: int = E2M3):
+def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out_fmt: int = E2M3, workspace=None):
     """C = A @ B^T delivered as an MX operand for the next layer: (operand bytes [M, 3N/4 | N | N/2], scales [M, N/32]),
-    quantised in the GEMM epilogue from the fp32 accumulators (blocks of 32 along N)."""
+    quantised in the GEMM epilogue from the fp32 accumulators (blocks of 32 along N).  workspace: as gemm() takes it."""
     _accept(A, "A", torch.uint8)
     _accept(B, "B", torch.uint8)
     _accept(scale_A, "scale_A", torch.uint8)
@@ -188,33 +204,35 @@ def gemm_requant(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = No
     _check_scales(A, B, scale_A, scale_B, K)
     if N % 64:
         raise RuntimeError("N must be a multiple of 64")
+    ws = () if workspace is None else _workspace(workspace, A.get_device())
     out = A.new_empty((M, row_bytes(N, out_fmt)))
     scales = A.new_empty((M, N // 32))
-    _launch(A, lib.mxfp6_gemm_requant, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
-            scales.data_ptr(), M, N, K, fmt, fb, out_fmt)
+    _launch(A, lib.mxfp6_gemm_requant_ws if ws else lib.mxfp6_gemm_requant, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), out.data_ptr(),
+            scales.data_ptr(), M, N, K, fmt, fb, out_fmt, *ws)
     return out, scales
 
 
 def gemm_scaled(A, scale_A, B, scale_B, row_scale=None, col_scale=None, bias=None, fmt: int = E2M3,
-                fmt_b: int | None = None, out=None):
+                fmt_b: int | None = None, out=None, workspace=None):
     """C[m,n] = bf16((acc[m,n] * col_scale[n]) * row_scale[m] + bias[n]) with fp32 vectors row_scale [M], col_scale [N],
     bias [N] (any may be None), applied in the GEMM epilogue: the per-row / per-column scaling of the reference's
-    scaled_matmul (kernels/torch_scaled/scaled_matmul.cu:253-265) on top of the MX block scales."""
-    return ops.gemm_scaled(A, scale_A, B, scale_B, row_scale, col_scale, bias, fmt, fmt if fmt_b is None else fmt_b, out)
+    scaled_matmul (kernels/torch_scaled/scaled_matmul.cu:253-265) on top of the MX block scales.  workspace: as gemm() takes it."""
+    return ops.gemm_scaled(A, scale_A, B, scale_B, row_scale, col_scale, bias, fmt, fmt if fmt_b is None else fmt_b, out, workspace)
 
 
 def gemm(A, scale_A, B, scale_B, fmt: int = E2M3, fmt_b: int | None = None, out=None, workspace=None):
     """The product of dispatch_micro with its result allocated here (unless given as `out`); returns C.
 
-    A product with at most 128 rows may add partial sums in a buffer that the library holds once per device, as the other
-    products do.  Calls that may run side by side (on several streams, or in captured graphs) take a `workspace` of
-    gemm_workspace() each; calls in the order of one stream can share it."""
+    A product with at most 128 rows may add partial sums in a buffer that the library holds once per device, as gemm_scaled, gemm_requant,
+    dispatch_micro and dispatch_multi do.  Calls that may run side by side (on several streams, or in captured graphs that are
+    replayed side by side) take a `workspace` of gemm_workspace() each; calls in the order of one stream can share it."""
     return ops.gemm(A, scale_A, B, scale_B, fmt, fmt if fmt_b is None else fmt_b, out, workspace)
 
 
 def gemm_workspace(M: int, N: int, K: int, device=None) -> torch.Tensor:
-    """A zeroed workspace for gemm() on [M,K] x [N,K], of any formats (empty where the sums are never split); a product leaves
-    zero what must be zero, so it serves one call after another, also of other shapes if it is large enough."""
+    """A zeroed workspace for a product of [M,K] x [N,K] by any of the entry points, of any formats (empty where the sums are never
+    split); a product leaves zero what must be zero, so it serves one call after another, also of other shapes if it is large
+    enough.  The zeros are written on the current stream."""
     device = torch.device("cuda" if device is None else device)
     with torch.cuda.device(device):
         return torch.zeros(lib.mxfp6_gemm_workspace_bytes(M, N, K), dtype=torch.uint8, device=device)

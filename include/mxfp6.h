@@ -71,8 +71,8 @@ const char* mxfp6_last_error(void);
  *   b   [N, 3K/4] u8 (fp6), [N, K] u8 (fp8) or [N, K/2] u8 (fp4)   sfb [N, K/32] u8    fmt_b likewise
  *   c   [M, N] bf16, written in place
  * Shapes that split output tiles along K use a per-device scratch buffer that the library
- * allocates on first need (cudaMalloc) and keeps; concurrent calls on different streams of one
- * device must use mxfp6_gemm_ws with their own scratch instead.  A scratch buffer is never freed or
+ * allocates on first need (cudaMalloc) and keeps; calls that may overlap on one device (different streams, graphs replayed side by
+ * side) must use the _ws form with their own scratch instead, for this and for every product below.  A scratch buffer is never freed or
  * moved once a launch has been given it (a CUDA graph captured earlier keeps replaying into it): a shape
  * that needs more gets an additional, larger buffer.  That allocation cannot happen while the stream is
  * being captured; the call then fails with MXFP6_ERR_BAD_ARG and says so -- run the shape once before
@@ -120,7 +120,8 @@ int mxfp6_gemm_scaled(const void* a, const void* sfa, const void* b, const void*
                       const float* scale_a, const float* scale_b, const float* bias,
                       int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, void* stream);
 
-/* Scratch bytes mxfp6_gemm_ws needs for this shape on the current device (0 if none). */
+/* Scratch bytes the _ws forms need for this shape on the current device, whatever the formats and the kind of result (0 if none of them
+ * splits tiles). */
 size_t mxfp6_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
 /* Same as mxfp6_gemm with caller-provided scratch (256-byte aligned, zero-filled once before its
@@ -129,6 +130,22 @@ size_t mxfp6_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mxfp6_gemm_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
                   int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* mxfp6_gemm_ex, mxfp6_gemm_requant, mxfp6_gemm_scaled and mxfp6_gemm_multi (which may split tiles when it has one destination) with
+ * caller-provided scratch, as mxfp6_gemm_ws takes it. */
+int mxfp6_gemm_ex_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
+                     int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, unsigned flags,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int mxfp6_gemm_requant_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales,
+                          int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, int out_fmt,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int mxfp6_gemm_scaled_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c,
+                         const float* scale_a, const float* scale_b, const float* bias,
+                         int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int mxfp6_gemm_multi_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
+                        int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The GEMM with its [M,N] result written to n_dst (1..8) destinations at once: c_dst[i] points at the first

@@ -41,9 +41,9 @@ def test_split_work_follows_the_longer_k_blocks():
 
 
 @pytest.mark.parametrize("sm", [148, 132, 16])
-def test_reported_workspace_serves_every_format(sm):
+def test_reported_workspace_serves_every_format_and_result(sm):
     for shape in SHAPES + MORE:
-        needs = [debug_plan(*shape, sm, fmt_a=a, fmt_b=b) for a, b in PAIRS]
+        needs = [debug_plan(*shape, sm, requant=r, fmt_a=a, fmt_b=b) for a, b in PAIRS for r in (False, True)]
         assert max(p["scratch"] for p in needs) == needs[0]["workspace"]
 
 

@@ -50,3 +50,127 @@ def test_first_split_product_on_a_side_stream_while_the_default_stream_is_busy()
     out = subprocess.run([sys.executable, "-c", _FIRST_CALL, ROOT], capture_output=True, text=True, timeout=600)
     assert "FIRST_CALL_OK" in out.stdout, out.stdout[-2000:] + out.stderr[-2000:]
     assert "still busy: True" in out.stdout          # (the case is the one that is meant)
+
+
+# ---------------------------------------------------------------------------------- a workspace for each of several products
+def _operands(M, N, K, seed, fa, fb):
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    t = [*hk.quantize(n(M, K), fa), *hk.quantize(0.02 * n(N, K), fb)]
+    return t, (torch.exp(0.3 * n(M)), torch.exp(0.3 * n(N)), n(N))
+
+
+def _products():
+    """entry point -> call(operands, vectors, formats, workspace) -> results"""
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    def micro(t, v, fa, fb, ws):
+        c = torch.empty(t[0].shape[0], t[2].shape[0], dtype=torch.bfloat16, device="cuda")
+        hk.dispatch_micro(t[0], t[2], c, t[1], t[3], fa, fb, workspace=ws)
+        return (c,)
+
+    def micro_static(t, v, fa, fb, ws):
+        c = torch.empty(t[0].shape[0], t[2].shape[0], dtype=torch.bfloat16, device="cuda")
+        hk.dispatch_micro(t[0], t[2], c, t[1], t[3], fa, fb, b_static=True, workspace=ws)
+        return (c,)
+
+    def multi(t, v, fa, fb, ws):
+        c = torch.zeros(t[0].shape[0], t[2].shape[0] + 64, dtype=torch.bfloat16, device="cuda")
+        hk.dispatch_multi(t[0], t[2], [c], 64, t[1], t[3], fa, workspace=ws)
+        return (c,)
+
+    return {"gemm": lambda t, v, fa, fb, ws: (hk.gemm(*t, fmt=fa, fmt_b=fb, workspace=ws),),
+            "dispatch_micro": micro, "dispatch_micro b_static": micro_static, "dispatch_multi": multi,
+            "gemm_scaled": lambda t, v, fa, fb, ws: (hk.gemm_scaled(*t, *v, fmt=fa, fmt_b=fb, workspace=ws),),
+            "gemm_requant": lambda t, v, fa, fb, ws: hk.gemm_requant(*t, fmt=fa, fmt_b=fb, out_fmt=hk.E4M3, workspace=ws)}
+
+
+@pytest.mark.parametrize("entry", ["gemm", "dispatch_micro", "dispatch_micro b_static", "dispatch_multi", "gemm_scaled", "gemm_requant"])
+@pytest.mark.parametrize("formats", [("E2M1", "E2M1"), ("E2M3", "E2M3"), ("E4M3", "E2M1")])
+def test_products_side_by_side_with_a_workspace_each(entry, formats):
+    """Products whose tiles are split along K on two streams at once, then in two captured graphs replayed at once: the bits of each alone."""
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    fa, fb = (getattr(hk, f) for f in formats)
+    if entry == "dispatch_multi":
+        fb = fa                                         # (one format for both sides)
+    M, N, K = 16, 512, 8192
+    call = _products()[entry]
+    sides = []
+    for seed in (1, 2):
+        t, v = _operands(M, N, K, seed, fa, fb)
+        ws = hk.gemm_workspace(M, N, K)
+        assert ws.numel() > 0
+        want = [r.clone() for r in call(t, v, fa, fb, ws)]
+        sides.append((t, v, ws, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    assert not torch.equal(sides[0][3][0], sides[1][3][0])
+
+    def verify(results):
+        torch.cuda.synchronize()
+        assert hk.device_status() == 0
+        for (_, _, _, want, _), got in zip(sides, results):
+            for r in got:
+                assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+    results = ([], [])
+    for _ in range(24):
+        for (t, v, ws, _, stream), got in zip(sides, results):
+            with torch.cuda.stream(stream):
+                got.append(call(t, v, fa, fb, ws))
+    verify(results)
+    graphs, results = [], []
+    for t, v, ws, _, _ in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append([call(t, v, fa, fb, ws) for _ in range(24)])
+    for got in results:
+        for r in got:
+            for x in r:
+                x.zero_()
+    torch.cuda.synchronize()
+    for graph, (*_, stream) in zip(graphs, sides):
+        with torch.cuda.stream(stream):
+            graph.replay()
+    verify(results)
+
+
+@pytest.mark.parametrize("shape", [(16, 24320, 1024), (16, 640, 1024), (32, 15040, 1024), (64, 640, 384), (100, 24064, 512)])
+def test_the_reported_workspace_is_enough_for_every_product(shape):
+    """Exactly the bytes the library asks for, also where only the re-quantising product splits its tiles."""
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    M, N, K = shape
+    for fa, fb in ((hk.E2M1, hk.E2M1), (hk.E4M3, hk.E2M1), (hk.E2M3, hk.E2M3)):
+        t, v = _operands(M, N, K, 5, fa, fb)
+        ws = hk.gemm_workspace(M, N, K)
+        for entry, call in _products().items():
+            if entry == "dispatch_multi" and fa != fb:
+                continue
+            got, want = call(t, v, fa, fb, ws), call(t, v, fa, fb, None)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), entry
+    assert hk.device_status() == 0
+
+
+def test_bad_workspaces_are_refused():
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    t, v = _operands(16, 512, 8192, 1, hk.E2M3, hk.E2M3)
+    ws = hk.gemm_workspace(16, 512, 8192)
+    for entry, call in _products().items():
+        for bad in (ws[:1024], ws[8:], ws.cpu(), ws.view(torch.float32), ws[::2], 7):
+            with pytest.raises(RuntimeError):
+                call(t, v, hk.E2M3, hk.E2M3, bad)
+                pytest.fail(f"{entry} took it")
