@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import E2M3
-from .gemm import dispatch_micro, row_bytes
+from .gemm import dispatch_micro, gemm_workspace, row_bytes
 
 
 class HostGemm:
@@ -30,9 +30,21 @@ class HostGemm:
         self.s_in = torch.cuda.Stream(self.device)
         self.s_mm = torch.cuda.Stream(self.device)
         self.s_out = torch.cuda.Stream(self.device)
+        # Split products run on a stream of this object's own, beside whatever the caller's streams hold: they get scratch of their own.
+        self.workspace = gemm_workspace(M, N, K, self.device)
+        # The buffers' memory may be in use by work that the current stream has yet to do, and must not be handed out again
+        # before these streams are done with it.
+        for st in (self.s_in, self.s_mm, self.s_out):
+            st.wait_stream(torch.cuda.current_stream(self.device))
+        for s in self.slots:
+            for name, users in (("a", (self.s_in, self.s_mm)), ("sa", (self.s_in, self.s_mm)), ("b", (self.s_in, self.s_mm)), ("sb", (self.s_in, self.s_mm)),
+                                ("c", (self.s_mm, self.s_out))):
+                for st in users:
+                    s[name].record_stream(st)
+        self.workspace.record_stream(self.s_mm)
         self.n = 0
         # gemm(slot) runs the kernel(s) of one call on the current stream and returns the tensor to copy out
-        self._gemm = gemm or (lambda s: (dispatch_micro(s["a"], s["b"], s["c"], s["sa"], s["sb"], self.fmt), s["c"])[1])
+        self._gemm = gemm or (lambda s: (dispatch_micro(s["a"], s["b"], s["c"], s["sa"], s["sb"], self.fmt, workspace=self.workspace), s["c"])[1])
 
     def __call__(self, a_host, sa_host, b_host, sb_host, out_host):
         """Queue one GEMM: operands from host tensors (pinned for true asynchrony), result into out_host."""

@@ -174,3 +174,66 @@ def test_bad_workspaces_are_refused():
             with pytest.raises(RuntimeError):
                 call(t, v, hk.E2M3, hk.E2M3, bad)
                 pytest.fail(f"{entry} took it")
+
+
+# ---------------------------------------------------------------------------------- objects that own their buffers
+def _host_case(M, N, K, seed):
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    t, _ = _operands(M, N, K, seed, hk.E2M3, hk.E2M3)
+    want = hk.gemm(*t, workspace=hk.gemm_workspace(M, N, K)).cpu()
+    torch.cuda.synchronize()
+    return t, [x.cpu().pin_memory() for x in t], torch.empty(M, N, dtype=torch.bfloat16).pin_memory(), want
+
+
+def test_host_pipeline_beside_products_of_the_caller():
+    """HostGemm's split products run on its own stream while the caller's run on theirs: each with scratch of its own."""
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    M, N, K = 16, 512, 8192
+    t, pinned, out, want = _host_case(M, N, K, 3)
+    pipes = [hk.HostGemm(M, N, K) for _ in range(2)]
+    outs = [[torch.empty_like(out).pin_memory() for _ in range(16)] for _ in pipes]
+    mine = []
+    for i in range(16):
+        for p, o in zip(pipes, outs):
+            p(*pinned, o[i])
+        mine.append(hk.gemm(*t))
+    for p in pipes:
+        p.synchronize()
+    torch.cuda.synchronize()
+    assert hk.device_status() == 0
+    for o in outs:
+        assert all(torch.equal(x, want) for x in o)
+    assert all(torch.equal(x.cpu(), want) for x in mine)
+
+
+def test_host_pipeline_made_while_its_memory_is_still_in_use():
+    """Its buffers may be memory that queued work of the current stream has yet to write (freed on the host, as torch's allocator allows), and
+    that is handed out again as soon as the object is gone."""
+    import torch
+
+    import hipkittensp_b200 as hk
+
+    M, N, K = 16, 512, 8192
+    _, pinned, out, want = _host_case(M, N, K, 4)
+    for _ in range(3):
+        junk = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in [x.numel() for x in pinned] * 2 + [2 * M * N] * 2]
+        torch.cuda._sleep(50_000_000)
+        for j in junk:
+            j.fill_(0x7f)
+        del junk, j
+        pipe = hk.HostGemm(M, N, K)
+        pipe(*pinned, out)
+        done = pipe.s_out
+        del pipe
+        other = [torch.full((x.numel(),), 0x7f, dtype=torch.uint8, device="cuda") for x in pinned]
+        done.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del other
+    assert hk.device_status() == 0
