@@ -33,7 +33,7 @@ import torch
 import torch.distributed as dist
 
 from ._lib import E2M3
-from .gemm import dispatch_micro
+from .gemm import dispatch_micro, gemm_workspace
 
 
 def shard_bounds(N: int, world: int, rank: int) -> tuple[int, int]:
@@ -58,6 +58,11 @@ def assemble_columns(gathered: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _scratch(M: int, N: int, K: int, device):
+    """Scratch of an operator's own for a local product that is split along K: two operators may run side by side."""
+    return gemm_workspace(M, N, K, device) if device is not None and torch.device(device).type == "cuda" else None
+
+
 class ColumnParallelGemm:
     """Holds the communicator and the reusable buffers of one sharded GEMM shape."""
 
@@ -72,6 +77,7 @@ class ColumnParallelGemm:
         self.M, self.N, self.K, self.fmt = M, N, K, fmt
         self.lo, self.hi = shard_bounds(N, self.world, self.rank)
         self.device = device
+        self.workspace = _scratch(M, self.hi - self.lo, K, device)
         on_gpu = device is not None and torch.device(device).type == "cuda"
         if gather is None:
             gather = "fused" if (on_gpu and self.world > 1) else "nccl"
@@ -124,9 +130,9 @@ class ColumnParallelGemm:
             from .gemm import dispatch_multi
 
             # (into the buffer of the latest call: no peer is written, so no ordering is needed)
-            dispatch_multi(A, B_shard, self.dests[:1], self.lo, scale_A, scale_B_shard, self.fmt)
+            dispatch_multi(A, B_shard, self.dests[:1], self.lo, scale_A, scale_B_shard, self.fmt, workspace=self.workspace)
         else:
-            dispatch_micro(A, B_shard, self.c_shard, scale_A, scale_B_shard, self.fmt)
+            dispatch_micro(A, B_shard, self.c_shard, scale_A, scale_B_shard, self.fmt, workspace=self.workspace)
         return self.c_shard
 
     def gather(self) -> torch.Tensor:
@@ -171,6 +177,7 @@ class RowParallelGemm:
         self.rank = dist.get_rank(group) if dist.is_initialized() else 0
         self.M, self.N, self.K, self.fmt = M, N, K, fmt
         self.lo, self.hi = shard_bounds(M, self.world, self.rank)
+        self.workspace = _scratch(self.hi - self.lo, N, K, device)
         self.push = gather and self.world > 1
         self.symm = None
         if self.push:
@@ -202,5 +209,5 @@ class RowParallelGemm:
             dispatch_multi(A_rows, B, self.dests, 0, scale_A_rows, scale_B, self.fmt)
             self.symm.barrier()
             return self.c_full
-        dispatch_micro(A_rows, B, self.c_rows, scale_A_rows, scale_B, self.fmt)
+        dispatch_micro(A_rows, B, self.c_rows, scale_A_rows, scale_B, self.fmt, workspace=self.workspace)
         return self.c_rows

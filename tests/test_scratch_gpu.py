@@ -237,3 +237,29 @@ def test_host_pipeline_made_while_its_memory_is_still_in_use():
         assert torch.equal(out, want)
         del other
     assert hk.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["ColumnParallelGemm", "RowParallelGemm"])
+def test_sharded_operators_side_by_side(kind):
+    """Two operators (of one rank each) on two streams: split products with scratch of their own."""
+    import torch
+
+    import hipkittensp_b200 as hk
+    from hipkittensp_b200 import sharded
+
+    M, N, K = 16, 512, 8192
+    sides = []
+    for seed in (1, 2):
+        t, _ = _operands(M, N, K, seed, hk.E2M3, hk.E2M3)
+        want = hk.gemm(*t, workspace=hk.gemm_workspace(M, N, K))
+        sides.append((getattr(sharded, kind)(M, N, K, device="cuda"), t, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(24):
+        for op, t, _, stream in sides:
+            with torch.cuda.stream(stream):
+                op(*t)
+    torch.cuda.synchronize()
+    assert hk.device_status() == 0
+    assert sides[0][0].workspace.data_ptr() != sides[1][0].workspace.data_ptr()
+    for op, t, want, _ in sides:
+        assert torch.equal(op(*t), want)
