@@ -158,7 +158,8 @@ __device__ __forceinline__ float quant_inv_scale(int sb) {          // 2^-(sb-12
 __device__ __forceinline__ void quant_store_lanes(float x, int fmt, uint8_t* q_out, size_t q_ld, uint8_t* q_scales,
                                                   int n_cols, int row, int col0, bool row_valid) {
     const int lane = threadIdx.x & 31;
-    const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(x))));
+    // (the maximum runs on the bits, where a NaN would come out on top: it does not count, as in the other forms)
+    const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, x == x ? __float_as_uint(fabsf(x)) : 0u));
     const int sb = quant_scale_byte(amax, fmt);
     const uint32_t code = cvt_one(x * quant_inv_scale(sb), fmt);
     const bool fp8 = fmt == kE4M3 || fmt == kE5M2;

@@ -211,7 +211,7 @@ int mxfp6_gemm_noalloc(const void* a, const void* sfa, const void* b, const void
  * Block quantiser: src [rows, K] (src_dtype 0 = fp32, 1 = bf16), K % 32 == 0  ->
  * packed [rows, 3K/4] (fp6), [rows, K] (fp8) or [rows, K/2] (fp4) + scales [rows, K/32].  Scale exponent = floor(log2(amax)) - 2
  * (E2M3, E2M1), - 4 (E3M2), - 8 (E4M3) or - 15 (E5M2); elements rounded to nearest even and saturated (a NaN does not count
- * towards amax and is stored as the largest magnitude).  The step in front of the GEMM; the
+ * towards amax and is stored as the largest magnitude, as a NaN in the fp8 formats).  The step in front of the GEMM; the
  * reference's fp8 harness does it on the host (kernels/gemm/fp8fp32/FP8_8wave/8_wave.cu:258-268).
  */
 int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt,
