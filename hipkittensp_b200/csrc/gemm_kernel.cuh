@@ -179,6 +179,9 @@ struct GemmCfg {
     static constexpr int STAGES_MAX = RUNTIME_RING ? 8 : STAGES;           // barrier pairs provided (see GemmParams::n_stages)
     static constexpr int QATOMS = (BN + 127) / 128;      // 128-row scale atoms on the Q side
     static constexpr int RAW_SLOTS = (BN >= 256 || CTAS_ == 2) ? 2 : 4;  // each raw slab covers 4 K-blocks (16 scale bytes per row)
+    // The two re-tiling warps alternate groups: with an even number of slots a slot always belongs to the same warp.  With an odd number a
+    // warp could wait for round n + 2 of a slot while round n + 1 has not landed, and a parity wait then returns at once on round n.
+    static_assert(RAW_SLOTS % 2 == 0, "a scale slot belongs to one re-tiling warp");
     static constexpr int RAW_Q_ROWS = BN < 32 ? 32 : BN;
     static constexpr int RAW_BYTES = (BM + RAW_Q_ROWS) * 16;
     static constexpr int ATOM_BYTES = 512 * (1 + QATOMS);  // scale atoms of 128 elements: P atom + Q atoms

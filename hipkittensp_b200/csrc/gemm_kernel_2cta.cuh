@@ -38,6 +38,7 @@ struct PairCfg {
     static constexpr int OUT_BUFS = 2;
     static constexpr int OUT_BYTES = BM * OUT_COLS * 2;
     static constexpr int RAW_SLOTS = 2;
+    static_assert(RAW_SLOTS % 2 == 0, "a scale slot belongs to one re-tiling warp (see GemmCfg)");
     static constexpr int RAW_BYTES = (BM + BN) * 16;      // own P rows + all 256 Q rows, 16 scale bytes each
     static constexpr int ATOM_BYTES = 512 * 3;            // P atom + two Q atoms of one K-block
     static constexpr int GROUP_BYTES = 4 * ATOM_BYTES;    // the 4 K-blocks one raw slab covers
