@@ -108,7 +108,7 @@ def _load_ops():
     try:
         from . import _torch_ops
     except ImportError as e:
-        raise ImportError(f"the _torch_ops extension is missing or does not load ({e}): build it with `python hipkittensp_b200/build.py`") from e
+        raise ImportError(f"the _torch_ops extension is missing or does not load ({e}): build it with `python hipkittensp_b200/build.py --force`") from e
     _torch_ops.bind(lib._handle, Mxfp6Error)
     return _torch_ops
 

@@ -73,16 +73,20 @@ def build_ext(force: bool = False) -> str:
 
 
 OPS = os.path.join(PKG, "_torch_ops" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+OPS_STAMP = os.path.join(PKG, "_torch_ops.built_for")     # the torch it was compiled against
 
 
 def build_torch_ops(force: bool = False) -> str:
     """The tensor-level wrappers of gemm.py and norm.py (links torch; finds the library's entry points at import)."""
+    import importlib.metadata
     import importlib.util
 
     import pybind11
 
     src = os.path.join(CSRC, "torch_ops.cpp")
-    if not force and _newer(OPS, [src, os.path.join(ROOT, "include", "mxfp6.h")]):
+    torch_version = importlib.metadata.version("torch")
+    built_for = open(OPS_STAMP).read() if os.path.exists(OPS_STAMP) else None
+    if not force and built_for == torch_version and _newer(OPS, [src, os.path.join(ROOT, "include", "mxfp6.h")]):
         return OPS
     torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
     torch_lib = os.path.join(torch_dir, "lib")
@@ -94,6 +98,8 @@ def build_torch_ops(force: bool = False) -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("g++ failed:\n" + res.stdout + res.stderr)
+    with open(OPS_STAMP, "w") as f:
+        f.write(torch_version)
     return OPS
 
 
