@@ -49,7 +49,7 @@ const at::Tensor& matrix(py::handle h, const char* name, at::ScalarType dtype) {
     if (!t.is_contiguous()) refuse("Tensor must be contiguous");
     if (!t.is_cuda()) refuse("Tensor must be on CUDA device");
     if (t.dim() > 4) refuse("Expected Tensor.ndim <= 4");
-    if (t.scalar_type() != dtype) refuse(std::string(name) + " must be " + name_of(dtype) + ", got " + std::string(c10::toString(t.scalar_type())));
+    if (t.scalar_type() != dtype) refuse(std::string(name) + " must be " + name_of(dtype) + ", got " + std::string(py::str(h.attr("dtype"))));
     if (t.dim() != 2) refuse(std::string(name) + " must be 2-D");
     return t;
 }
@@ -161,10 +161,19 @@ Workspace workspace_of(const Operands& o, py::handle workspace) {
 }
 
 py::object gemm(py::handle A, py::handle scale_A, py::handle B, py::handle scale_B, int fmt, int fmt_b, py::handle out, py::handle workspace) {
-    const Operands o = operands(A, scale_A, B, scale_B, fmt, fmt_b);
+    // the checks of dispatch_micro, in its order and words
+    const at::Tensor &a = matrix(A, "A", at::kByte), &b = matrix(B, "B", at::kByte);
+    const at::Tensor* given = out.is_none() ? nullptr : &matrix(out, "C", at::kBFloat16);
+    const at::Tensor &sa = matrix(scale_A, "scale_A", at::kByte), &sb = matrix(scale_B, "scale_B", at::kByte);
+    const Operands o{a, sa, b, sb, a.size(0), given ? given->size(1) : b.size(0), k_of(a, fmt, "A")};
     if (o.K % 128) refuse("K must be a multiple of 128");
+    if (given && given->size(0) != o.M) refuse("C.shape[0] must equal A.shape[0]");
+    if (b.size(0) != o.N || k_of(b, fmt_b, "B") != o.K) refuse("B must be [N, 3K/4] (fp6), [N, K] (fp8) or [N, K/2] (fp4) with the K of A");
+    if (sa.size(0) != o.M || sa.size(1) != o.K / 32 || sb.size(0) != o.N || sb.size(1) != o.K / 32) refuse("scales must be [rows, K/32]");
+    same_device(a, {&b, &sa, &sb});
+    if (given) same_device(a, {given});
     const Workspace ws = workspace_of(o, workspace);
-    at::Tensor c = result(o, out);
+    at::Tensor c = given ? *given : empty({o.M, o.N}, at::kBFloat16, a);
     launch(o.a, [&](void* st) {
         const void *a = o.a.const_data_ptr(), *sa = o.sa.const_data_ptr(), *b = o.b.const_data_ptr(), *sb = o.sb.const_data_ptr();
         return ws.own ? lib.mxfp6_gemm_ex(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, 0, st)

@@ -98,3 +98,24 @@ def test_out_of_memory_keeps_its_type():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert hk.layer_norm(x[:8])[0].shape == (8, 4096)
+
+
+def test_gemm_refuses_in_the_words_of_dispatch_micro():
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8, device="cuda")
+    c = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    A, B, sA, sB, C = u8(32, 256), u8(48, 256), u8(32, 8), u8(48, 8), c(32, 48)
+    bad = [(1, B, C, sA, sB), (A.t(), B, C, sA, sB), (A.cpu(), B, C, sA, sB), (A.int(), B, C, sA, sB), (A[0], B, C, sA, sB), (A.view(1, 1, 1, 32, 256), B, C, sA, sB),
+           (A, 2, C, sA, sB), (A, B.cpu(), C, sA, sB), (A, B, C.float(), sA, sB), (A, B, C, sA.int(), sB), (A, B, C, sA, sB[0]),
+           (u8(32, 96), B, C, sA, sB), (A, B, c(31, 48), sA, sB), (A, B, c(32, 47), sA, sB), (A, u8(47, 256), C, sA, sB), (A, u8(48, 128), C, sA, sB),
+           (A, B, C, u8(32, 4), sB), (A, B, C, sA, u8(47, 8))]
+    for i, (a, b, out, sa, sb) in enumerate(bad):
+        texts = []
+        for call in (lambda: hk.dispatch_micro(a, b, out, sa, sb, hk.E4M3), lambda: hk.gemm(a, sa, b, sb, hk.E4M3, out=out)):
+            with pytest.raises(RuntimeError) as e:
+                call()
+            texts.append(str(e.value))
+        assert texts[0] == texts[1], i
+    # fp6 rows that are not whole groups of four codes, and B with another K where the result is allocated
+    for call in (lambda: hk.gemm(u8(32, 98), sA, B, sB), lambda: hk.gemm(A, sA, u8(48, 128), sB, hk.E4M3)):
+        with pytest.raises(RuntimeError, match="must be 3K/4 bytes|B must be"):
+            call()
