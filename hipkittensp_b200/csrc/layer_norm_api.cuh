@@ -152,6 +152,19 @@ static bool ln_overlap(const void* p, uint64_t p_bytes, const void* q, uint64_t 
     return a < b ? b - a < p_bytes : a - b < q_bytes;
 }
 
+struct LnRange { const char* name; const void* p; uint64_t bytes; };
+// A result that lies on an operand, or on another result, whose bytes other CTAs read or write at any time (null ranges lie nowhere).
+static int ln_apart(const char* what, std::initializer_list<LnRange> results, std::initializer_list<LnRange> operands, bool among = false) {
+    for (const LnRange* r = results.begin(); r != results.end(); ++r) {
+        if (!r->p) continue;
+        for (const LnRange& o : operands)
+            if (o.p && ln_overlap(r->p, r->bytes, o.p, o.bytes)) return fail(MXFP6_ERR_BAD_ARG, "%s: %s overlaps %s", what, r->name, o.name);
+        for (const LnRange* q = r + 1; among && q != results.end(); ++q)
+            if (q->p && ln_overlap(r->p, r->bytes, q->p, q->bytes)) return fail(MXFP6_ERR_BAD_ARG, "%s: %s overlaps %s", what, r->name, q->name);
+    }
+    return MXFP6_OK;
+}
+
 // elements from the 16- or 32-byte boundary in front of p to p
 static int ln_offset(const void* p, int dtype) { return (int)((uintptr_t)p & (dtype == 0 ? 31 : 15)) / (dtype == 0 ? 4 : 2); }
 
@@ -176,6 +189,13 @@ static int ln_forward(const char* what, const void* x, int x_dtype, const void* 
                  ln_overlap(x, bytes, scales, (uint64_t)rows * (uint64_t)(H / 32))
            : x != y && ln_overlap(x, bytes, y, bytes))
         return fail(MXFP6_ERR_BAD_ARG, "%s: the result overlaps x", what);
+    {
+        const uint64_t params = (uint64_t)H * (w_dtype == 0 ? 4 : 2), stats = (uint64_t)rows * 4;
+        const LnRange y_range{"the result", mx ? packed : y, mx ? (uint64_t)rows * (uint64_t)(H / 32) * fmt_block_bytes(fmt) : bytes},
+            scale_range{"the scales", mx ? scales : nullptr, (uint64_t)rows * (uint64_t)(H / 32)}, mean_range{"mean", mean, stats}, rstd_range{"rstd", rstd, stats};
+        if ((rc = ln_apart(what, {y_range, scale_range, mean_range, rstd_range}, {{"weight", w, params}, {"bias", b, params}}, true))) return rc;
+        if ((rc = ln_apart(what, {mean_range, rstd_range}, {{"x", x, bytes}}))) return rc;
+    }
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
     const LnChoice k = x_dtype == 0 ? ln_forward_kernel<float>(place, fmt, (int)H) : ln_forward_kernel<__nv_bfloat16>(place, fmt, (int)H);
@@ -211,6 +231,10 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     const uint64_t bytes = (uint64_t)rows * (uint64_t)H * (x_dtype == 0 ? 4 : 2);
     if ((dx != x && ln_overlap(dx, bytes, x, bytes)) || (dx != dy && ln_overlap(dx, bytes, dy, bytes)))
         return fail(MXFP6_ERR_BAD_ARG, "%s: dx overlaps x or dy without being it", what);
+    const uint64_t params = (uint64_t)H * (w_dtype == 0 ? 4 : 2), sum_bytes = (uint64_t)H * 4, stats = (uint64_t)rows * 4;
+    const LnRange dx_range{"dx", dx, bytes}, dw_range{"dweight", dw, sum_bytes}, db_range{"dbias", db, sum_bytes}, x_range{"x", x, bytes}, dy_range{"dy", dy, bytes},
+        w_range{"weight", w, params}, mean_range{"mean", mean, stats}, rstd_range{"rstd", rstd, stats};
+    if ((rc = ln_apart(what, {dx_range}, {w_range, mean_range, rstd_range}))) return rc;
     DeviceState* d = nullptr;
     if ((rc = get_device_state(&d))) return rc;
     const bool sums = dw || db;
@@ -218,6 +242,10 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     const size_t need = sums ? ln_workspace(rows, H, d->sm_count) : 0;
     if (sums && (!ws || ws_bytes < need)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace too small: need %zu bytes, got %zu", what, need, ws ? ws_bytes : 0);
     if (sums && ((uintptr_t)ws & 15)) return fail(MXFP6_ERR_BAD_ARG, "%s: workspace must be 16-byte aligned", what);
+    // (the sums are written when all else has been read, but into no other result, and the workspace while rows are read and written)
+    if (sums && ((rc = ln_apart(what, {{"the workspace", ws, need}}, {dx_range, dw_range, db_range, x_range, dy_range, w_range, mean_range, rstd_range})) ||
+                 (rc = ln_apart(what, {dx_range, dw_range, db_range}, {}, true))))
+        return rc;
     const LnRows place = ln_rows(H, x_dtype, w, nullptr, x, dy, dx);
     LnParams P{};
     P.x = x; P.dy = dy; P.y = dx; P.w = w; P.w_bf16 = w_dtype;

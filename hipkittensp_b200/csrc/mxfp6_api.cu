@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <atomic>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <mutex>

@@ -231,7 +231,7 @@ int mxfp6_dequantize_ex(const void* packed, const void* scales, int64_t rows, in
  * 1e17, or squares that vanish beside a tiny eps) is worked out in 64 bits, and one that holds an infinity or a NaN has the mean
  * that its sum gives and a NaN for rstd and for all of y.  weight and bias are [H] vectors of w_dtype (0 = fp32,
  * 1 = bf16); either may be NULL (ones / zeros).  mean and rstd are fp32 [rows], kept for the backward pass; either may be
- * NULL.  y may be x itself; one that overlaps x otherwise is refused.  Any H >= 1 and any pointers aligned to their type; x and y
+ * NULL.  y may be x itself; one that overlaps x otherwise is refused, like any result that overlaps a parameter or another result.  Any H >= 1 and any pointers aligned to their type; x and y
  * that start at the same place of a 16-byte (bf16) or 32-byte (fp32) unit of memory take the vector paths, others are passed over element by element.
  *
  * The _quantize form delivers y as an MX operand instead (blocks of 32 along H: the K of the product that follows), rounded
@@ -254,8 +254,8 @@ int mxfp6_layer_norm_quantize(const void* x, int x_dtype, const void* weight, co
  * The sums over the rows go through per-CTA partials in `workspace` (at least the given number of bytes, 16-byte aligned, owned
  * by this call until the stream has passed it; any contents; not needed when dweight and dbias are both NULL) and are added
  * in a fixed order: equal calls on a device give equal bits.  Two calls that may overlap need a workspace each.
- * rows = 0 gives zero parameter gradients.  dx may be dy or x itself; one that overlaps them otherwise is
- * refused.  (No counterpart in the reference.)
+ * rows = 0 gives zero parameter gradients.  dx may be dy or x itself; one that overlaps them otherwise, or lies on weight, mean or
+ * rstd, is refused, and so are results that share bytes and a workspace that lies on an operand or a result.  (No counterpart in the reference.)
  */
 size_t mxfp6_layer_norm_backward_workspace_bytes(int64_t rows, int64_t H);
 int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dtype, const float* mean, const float* rstd,

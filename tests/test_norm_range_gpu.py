@@ -160,3 +160,28 @@ def test_gradient_of_constant_rows_far_from_zero(H, dtype):
     w, b = _parameters(H, dtype)
     _, mean, rstd = hk.layer_norm(x, w, b)
     _check_gradient(x, dy, w, mean, rstd)
+
+
+def test_results_that_share_bytes_are_refused():
+    x, dy = _noise(8, 64, 1), _noise(8, 64, 2)
+    w, b = _parameters(64, torch.float32)
+    flat = torch.zeros(8 * 64 + 64, device=DEV)
+    flat[512:] = w
+    with pytest.raises(RuntimeError, match="overlaps weight"):
+        hk.layer_norm(x, flat[512:], b, out=flat[8:520].view(8, 64))
+    hk.layer_norm(x, flat[512:], b, out=flat[:512].view(8, 64))                       # neighbours
+    assert torch.equal(flat[512:], w) and torch.equal(flat[:512].view(8, 64), hk.layer_norm(x, w, b)[0])
+    _, mean, rstd = hk.layer_norm(x, w, b)
+    need = hk.lib.mxfp6_layer_norm_backward_workspace_bytes(8, 64)
+    buf = torch.zeros(need + 4096, dtype=torch.uint8, device=DEV)
+    dx, sums, st = torch.empty_like(x), torch.empty(128, device=DEV), torch.cuda.current_stream().cuda_stream
+
+    def call(dw, db, ws):
+        return hk.lib.mxfp6_layer_norm_backward(dy.data_ptr(), x.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), 0, dx.data_ptr(), dw, db, 8, 64, ws, need, st)
+
+    s, p = sums.data_ptr(), buf.data_ptr()
+    assert call(s, s + 256, p) == 0
+    for bad in ((s, s, p), (s, s + 252, p), (dx.data_ptr(), s, p), (s, dx.data_ptr() + 2044, p), (p, s, p), (s, p + need - 4, p)):
+        assert call(*bad) == 1 and b"overlaps" in hk.lib.mxfp6_last_error(), bad
+    for t in (dx, x, dy, w, mean, rstd):
+        assert call(s, s + 256, t.data_ptr()) == 1 and b"overlaps" in hk.lib.mxfp6_last_error()
