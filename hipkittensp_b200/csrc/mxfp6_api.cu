@@ -35,7 +35,7 @@ static int fail(int code, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
-    g_err = buf;
+    try { g_err = buf; } catch (...) {}
     return code;
 }
 // No C++ exception leaves a C entry point (the tables of kernels and tensor maps allocate).
@@ -597,10 +597,10 @@ static int own_scratch(DeviceState& d, size_t bytes, cudaStream_t st, void** out
     return MXFP6_OK;
 }
 
-static int gemm_impl(const void* a, const void* sfa, const void* b, const void* sfb, const Dest& dst, int64_t M, int64_t N,
+static int gemm_unguarded(const void* a, const void* sfa, const void* b, const void* sfb, const Dest& dst, int64_t M, int64_t N,
                      int64_t K, int fmt_a, int fmt_b, void* ws, size_t ws_bytes, int ws_mode, void* stream,
-                     unsigned flags = 0, void* q_out = nullptr, void* q_scales = nullptr, int q_fmt = -1,
-                     const Affine& aff = Affine{}, const Signal& sig = Signal{}) {
+                     unsigned flags, void* q_out, void* q_scales, int q_fmt,
+                     const Affine& aff, const Signal& sig) {
     cudaStream_t st = (cudaStream_t)stream;
     // ---- the recipe of an identical earlier call
     int dev = -1;
@@ -821,6 +821,14 @@ static int gemm_impl(const void* a, const void* sfa, const void* b, const void* 
     t_cache->slot[t_cache->next++ % kRecipeSlots] = r;
     return MXFP6_OK;
 }
+static int gemm_impl(const void* a, const void* sfa, const void* b, const void* sfb, const Dest& dst, int64_t M, int64_t N,
+                     int64_t K, int fmt_a, int fmt_b, void* ws, size_t ws_bytes, int ws_mode, void* stream,
+                     unsigned flags = 0, void* q_out = nullptr, void* q_scales = nullptr, int q_fmt = -1,
+                     const Affine& aff = Affine{}, const Signal& sig = Signal{}) {
+    return guarded([&] {
+        return gemm_unguarded(a, sfa, b, sfb, dst, M, N, K, fmt_a, fmt_b, ws, ws_bytes, ws_mode, stream, flags, q_out, q_scales, q_fmt, aff, sig);
+    });
+}
 
 // ---------------------------------------------------------------------------------- quantise / dequantise
 template <typename T> __device__ __forceinline__ void load4(const T* p, float (&x)[4]);
@@ -963,7 +971,7 @@ extern "C" int mxfp6_gemm_ex(const void* a, const void* sfa, const void* b, cons
 
 extern "C" int mxfp6_gemm_ex_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* c, int64_t M, int64_t N,
                                 int64_t K, int fmt_a, int fmt_b, unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
-    return guarded([&] { return gemm_ex(a, sfa, b, sfb, c, M, N, K, fmt_a, fmt_b, flags, {kWsCaller, workspace, workspace_bytes}, stream); });
+    return gemm_ex(a, sfa, b, sfb, c, M, N, K, fmt_a, fmt_b, flags, {kWsCaller, workspace, workspace_bytes}, stream);
 }
 
 static int gemm_requant(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales, int64_t M, int64_t N,
@@ -989,7 +997,7 @@ extern "C" int mxfp6_gemm_requant(const void* a, const void* sfa, const void* b,
 extern "C" int mxfp6_gemm_requant_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* out, void* out_scales,
                                      int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, int out_fmt, void* workspace,
                                      size_t workspace_bytes, void* stream) {
-    return guarded([&] { return gemm_requant(a, sfa, b, sfb, out, out_scales, M, N, K, fmt_a, fmt_b, out_fmt, {kWsCaller, workspace, workspace_bytes}, stream); });
+    return gemm_requant(a, sfa, b, sfb, out, out_scales, M, N, K, fmt_a, fmt_b, out_fmt, {kWsCaller, workspace, workspace_bytes}, stream);
 }
 
 // C = bias broadcast along rows: what the scaled GEMM yields for K = 0
@@ -1026,7 +1034,7 @@ extern "C" int mxfp6_gemm_scaled_ws(const void* a, const void* sfa, const void* 
                                     const float* scale_a, const float* scale_b, const float* bias,
                                     int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b, void* workspace, size_t workspace_bytes,
                                     void* stream) {
-    return guarded([&] { return gemm_scaled(a, sfa, b, sfb, c, scale_a, scale_b, bias, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream); });
+    return gemm_scaled(a, sfa, b, sfb, c, scale_a, scale_b, bias, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream);
 }
 
 static int gemm_multi(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst, int n_dst, int64_t ldc, int64_t M,
@@ -1049,7 +1057,7 @@ extern "C" int mxfp6_gemm_multi(const void* a, const void* sfa, const void* b, c
 extern "C" int mxfp6_gemm_multi_ws(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
                                    int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
                                    void* workspace, size_t workspace_bytes, void* stream) {
-    return guarded([&] { return gemm_multi(a, sfa, b, sfb, c_dst, n_dst, ldc, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream); });
+    return gemm_multi(a, sfa, b, sfb, c_dst, n_dst, ldc, M, N, K, fmt_a, fmt_b, {kWsCaller, workspace, workspace_bytes}, stream);
 }
 
 // ---------------------------------------------------------------------------------- GEMM with a copy-engine gather
@@ -1105,7 +1113,7 @@ extern "C" size_t mxfp6_copy_gather_scratch_bytes(int64_t M, int64_t N, int stri
     return (size_t)gather_blocks(M, N, strip_tiles).total() * 2 * sizeof(unsigned int);
 }
 
-extern "C" int mxfp6_gemm_copy_gather(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
+static int gemm_copy_gather_unguarded(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
                                       int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
                                       void* scratch, size_t scratch_bytes, int strip_tiles, void* const* copy_streams,
                                       int n_copy_streams, void* stream) {
@@ -1173,6 +1181,13 @@ extern "C" int mxfp6_gemm_copy_gather(const void* a, const void* sfa, const void
     return MXFP6_OK;
 }
 
+extern "C" int mxfp6_gemm_copy_gather(const void* a, const void* sfa, const void* b, const void* sfb, void* const* c_dst,
+                                      int n_dst, int64_t ldc, int64_t M, int64_t N, int64_t K, int fmt_a, int fmt_b,
+                                      void* scratch, size_t scratch_bytes, int strip_tiles, void* const* copy_streams,
+                                      int n_copy_streams, void* stream) {
+    return guarded([&] { return gemm_copy_gather_unguarded(a, sfa, b, sfb, c_dst, n_dst, ldc, M, N, K, fmt_a, fmt_b, scratch, scratch_bytes, strip_tiles, copy_streams, n_copy_streams, stream); });
+}
+
 // ---------------------------------------------------------------------------------- GEMM without allocation
 // Scratch that is part of the library image: every GPU that loads libmxfp6.so holds these 8 MiB until the
 // process exits.  In host code `g_builtin_scratch` is only a handle for the symbol, not a device address;
@@ -1213,7 +1228,7 @@ extern "C" int mxfp6_gemm_noalloc(const void* a, const void* sfa, const void* b,
     return gemm_impl(a, sfa, b, sfb, dst, M, N, K, fmt_a, fmt_b, scratch, kBuiltinScratchBytes, kWsBuiltin, stream);
 }
 
-extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt, void* packed, void* scales,
+static int quantize_unguarded(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt, void* packed, void* scales,
                               void* stream) {
     if (rows < 0 || K < 0 || K % 32) return fail(MXFP6_ERR_BAD_ARG, "quantize: rows=%lld K=%lld (K must be a multiple of 32)", (long long)rows, (long long)K);
     if (!fmt_valid(fmt)) return fail(MXFP6_ERR_BAD_ARG, "quantize: bad format %d", fmt);
@@ -1283,6 +1298,11 @@ extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int6
 #undef QK
     CUDA_TRY(cudaGetLastError());
     return MXFP6_OK;
+}
+
+extern "C" int mxfp6_quantize(const void* src, int src_dtype, int64_t rows, int64_t K, int fmt, void* packed, void* scales,
+                              void* stream) {
+    return guarded([&] { return quantize_unguarded(src, src_dtype, rows, K, fmt, packed, scales, stream); });
 }
 
 template <int F, typename T>
@@ -1370,7 +1390,7 @@ extern "C" int mxfp6_layer_norm_backward(const void* dy, const void* x, int x_dt
     return guarded([&] { return ln_backward(dy, x, x_dtype, mean, rstd, weight, w_dtype, dx, dweight, dbias, rows, H, workspace, workspace_bytes, stream); });
 }
 
-extern "C" int mxfp6_device_status(int* status_out) {
+static int device_status_unguarded(int* status_out) {
     DeviceState* d = nullptr;
     int rc = get_device_state(&d);
     if (rc) return rc;
@@ -1387,6 +1407,10 @@ extern "C" int mxfp6_device_status(int* status_out) {
         return fail(MXFP6_ERR_DEVICE_WAIT, "a bounded wait ran out on the device: role %d, CTA %d", h[0] & 0xff, h[0] >> 8);
     }
     return MXFP6_OK;
+}
+
+extern "C" int mxfp6_device_status(int* status_out) {
+    return guarded([&] { return device_status_unguarded(status_out); });
 }
 
 extern "C" int mxfp6_debug_wait_timeout(int budget_us, void* stream) {
@@ -1428,7 +1452,7 @@ extern "C" int mxfp6_debug_plan_fmt(int64_t M, int64_t N, int64_t K, int sm_coun
     return MXFP6_OK;
 }
 
-extern "C" int mxfp6_debug_tma_dump(const void* packed, int64_t rows, int64_t K, int64_t row0, int64_t k0, void* out16k,
+static int debug_tma_dump_unguarded(const void* packed, int64_t rows, int64_t K, int64_t row0, int64_t k0, void* out16k,
                                     void* stream) {
     if (!packed || !out16k || K <= 0 || K % 128 || k0 % 128 || rows <= 0) return fail(MXFP6_ERR_BAD_ARG, "tma_dump: bad argument");
     if ((uintptr_t)packed & 31) return fail(MXFP6_ERR_BAD_ARG, "tma_dump: operand must be 32-byte aligned");
@@ -1443,4 +1467,9 @@ extern "C" int mxfp6_debug_tma_dump(const void* packed, int64_t rows, int64_t K,
     tma_dump_kernel<<<1, 128, 16384 + 2048, (cudaStream_t)stream>>>(tm, (int)k0, (int)row0, tx, d->wait_cycles / 20, (uint8_t*)out16k, d->status);
     CUDA_TRY(cudaGetLastError());
     return MXFP6_OK;
+}
+
+extern "C" int mxfp6_debug_tma_dump(const void* packed, int64_t rows, int64_t K, int64_t row0, int64_t k0, void* out16k,
+                                    void* stream) {
+    return guarded([&] { return debug_tma_dump_unguarded(packed, rows, K, row0, k0, out16k, stream); });
 }

@@ -1,0 +1,51 @@
+"""Out of host memory inside a C entry point: an error code, not a C++ exception that ends the process."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+# A process that has used up its address space, but for blocks smaller than the table of recent launches that a thread's first product makes.
+_CHILD = r"""
+import ctypes, resource, sys
+sys.path.insert(0, sys.argv[1])
+import hipkittensp_b200 as hk
+from hipkittensp_b200 import _lib
+L, entry = hk.lib, sys.argv[2]
+one = (ctypes.c_void_p * 1)(0x1000)
+P = 0x1000
+calls = {
+    "gemm": lambda: L.mxfp6_gemm(P, P, P, P, P, 16, 16, 100, 0, 0, None),
+    "gemm_ws": lambda: L.mxfp6_gemm_ws(P, P, P, P, P, 16, 16, 100, 0, 0, None, 0, None),
+    "gemm_ex": lambda: L.mxfp6_gemm_ex(P, P, P, P, P, 16, 16, 100, 0, 0, 0, None),
+    "gemm_ex_ws": lambda: L.mxfp6_gemm_ex_ws(P, P, P, P, P, 16, 16, 100, 0, 0, 0, None, 0, None),
+    "gemm_requant": lambda: L.mxfp6_gemm_requant(P, P, P, P, P, P, 16, 64, 100, 0, 0, 0, None),
+    "gemm_scaled": lambda: L.mxfp6_gemm_scaled(P, P, P, P, P, None, None, None, 16, 16, 100, 0, 0, None),
+    "gemm_multi": lambda: L.mxfp6_gemm_multi(P, P, P, P, one, 1, 16, 16, 16, 100, 0, 0, None),
+    "gemm_noalloc": lambda: L.mxfp6_gemm_noalloc(P, P, P, P, P, 16, 16, 100, 0, 0, None),
+}
+call = calls[entry]
+pages = int(open("/proc/self/statm").read().split()[0])
+resource.setrlimit(resource.RLIMIT_AS, (pages * resource.getpagesize() + (8 << 20),) * 2)
+held = []
+for size in (1 << 20, 256 << 10, 120 << 10, 60 << 10, 30 << 10):
+    try:
+        while True:
+            held.append(bytearray(size))
+    except MemoryError:
+        pass
+rc = call()
+msg = L.mxfp6_last_error()
+held.clear()
+assert rc == _lib.ERR_CUDA and msg == b"out of host memory", (rc, msg)
+assert call() == _lib.ERR_BAD_ARG and b"multiple of 128" in L.mxfp6_last_error()
+print("HOST_MEMORY_OK")
+"""
+
+
+@pytest.mark.parametrize("entry", ["gemm", "gemm_ws", "gemm_ex", "gemm_ex_ws", "gemm_requant", "gemm_scaled", "gemm_multi", "gemm_noalloc"])
+def test_products(entry):
+    out = subprocess.run([sys.executable, "-c", _CHILD, ROOT, entry], capture_output=True, text=True, timeout=300)
+    assert "HOST_MEMORY_OK" in out.stdout, (out.returncode, out.stdout[-500:], out.stderr[-1000:])
