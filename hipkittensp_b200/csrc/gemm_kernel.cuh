@@ -582,17 +582,17 @@ mxfp6_gemm_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_constan
                                          sfb | ((2 * (k & 1)) << 30), (kb > sg.k0 || k > 0) ? 1u : 0u);
                         }
                     } else {
-                    const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
-                    const uint32_t sfb = sfa + 4;
-                    const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
-                    tc_cp_32x128b_warpx4(sfa, smem_desc_sf(atom));
+                        const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
+                        const uint32_t sfb = sfa + 4;
+                        const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
+                        tc_cp_32x128b_warpx4(sfa, smem_desc_sf(atom));
 #pragma unroll
-                    for (int q = 0; q < Cfg::QATOMS; ++q) tc_cp_32x128b_warpx4(sfb + 4 * q, smem_desc_sf(atom + 512 * (1 + q)));
+                        for (int q = 0; q < Cfg::QATOMS; ++q) tc_cp_32x128b_warpx4(sfb + 4 * q, smem_desc_sf(atom + 512 * (1 + q)));
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        mma_mxf8f6f4(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(P.idesc, k),
-                                     sfa | (k << 30), sfb | (k << 30), (kb > sg.k0 || k > 0) ? 1u : 0u);
-                    }
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            mma_mxf8f6f4(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(P.idesc, k),
+                                         sfa | (k << 30), sfb | (k << 30), (kb > sg.k0 || k > 0) ? 1u : 0u);
+                        }
                     }
                     tc_commit(bar_empty(s));
                     if (group_done) tc_commit(bar_atom_empty(g));

@@ -282,17 +282,17 @@ mxfp6_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_p, const __grid_co
                                                   sfa | ((2 * (k & 1)) << 30), sfb | ((2 * (k & 1)) << 30), (kb > 0 || k > 0) ? 1u : 0u);
                             }
                         } else {
-                        const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
-                        const uint32_t sfb = sfa + 4;
-                        const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
-                        tc_cp_32x128b_warpx4_pair(sfa, smem_desc_sf(atom));
-                        tc_cp_32x128b_warpx4_pair(sfb, smem_desc_sf(atom + 512));
-                        tc_cp_32x128b_warpx4_pair(sfb + 4, smem_desc_sf(atom + 1024));
+                            const uint32_t sfa = tmem_base + Cfg::SF_COL + (n_kb & 1) * 16;
+                            const uint32_t sfb = sfa + 4;
+                            const uint32_t atom = atom_base + g * Cfg::GROUP_BYTES + (kb & 3) * Cfg::ATOM_BYTES;
+                            tc_cp_32x128b_warpx4_pair(sfa, smem_desc_sf(atom));
+                            tc_cp_32x128b_warpx4_pair(sfb, smem_desc_sf(atom + 512));
+                            tc_cp_32x128b_warpx4_pair(sfb + 4, smem_desc_sf(atom + 1024));
 #pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            mma_mxf8f6f4_pair(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(idesc, k),
-                                              sfa | (k << 30), sfb | (k << 30), (kb > 0 || k > 0) ? 1u : 0u);
-                        }
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                mma_mxf8f6f4_pair(acc, adesc + 2 * k, bdesc + 2 * k, idesc_with_sf(idesc, k),
+                                                  sfa | (k << 30), sfb | (k << 30), (kb > 0 || k > 0) ? 1u : 0u);
+                            }
                         }
                         tc_commit_pair(bar_empty(s), 3);
                         if (group_done) tc_commit_pair(bar_atom_empty(g), 3);

@@ -467,84 +467,84 @@ layer_norm_kernel(const LnParams P) {
     const bool edge = !__all_sync(0xffffffffu, inside);
     __syncthreads();
     for (int par = 0;; par ^= 1) {
-      for (; row < P.rows; row += P.step, par ^= 1) {
-        float2 v[C][4];
-        if constexpr (ODD) {
-            if (edge)
+        for (; row < P.rows; row += P.step, par ^= 1) {
+            float2 v[C][4];
+            if constexpr (ODD) {
+                if (edge)
 #pragma unroll
-                for (int c = 0; c < C; ++c) mask_chunk<T>(K, tid + c * TPR, raw[c]);
-        }
+                    for (int c = 0; c < C; ++c) mask_chunk<T>(K, tid + c * TPR, raw[c]);
+            }
 #pragma unroll
-        for (int c = 0; c < C; ++c) unpack2<T>(raw[c], v[c]);
-        load(row + P.step);
-        float2 s2 = make_float2(0.f, 0.f);
+            for (int c = 0; c < C; ++c) unpack2<T>(raw[c], v[c]);
+            load(row + P.step);
+            float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s2 = __fadd2_rn(s2, v[c][i]);
-        float s[1] = {s2.x + s2.y};
-        row_sum<1, WARPS>(s, red[par]);
-        const float mean0 = over_h(P, s[0]);
-        float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
-        if (ODD && edge) {
+                for (int i = 0; i < 4; ++i) s2 = __fadd2_rn(s2, v[c][i]);
+            float s[1] = {s2.x + s2.y};
+            row_sum<1, WARPS>(s, red[par]);
+            const float mean0 = over_h(P, s[0]);
+            float2 q2 = make_float2(0.f, 0.f), d2 = make_float2(0.f, 0.f);
+            if (ODD && edge) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int lo = K.lo(tid + c * TPR), hi = K.hi(tid + c * TPR);
+                for (int c = 0; c < C; ++c) {
+                    const int lo = K.lo(tid + c * TPR), hi = K.hi(tid + c * TPR);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 m = make_float2(2 * i >= lo && 2 * i < hi ? -mean0 : 0.f, 2 * i + 1 >= lo && 2 * i + 1 < hi ? -mean0 : 0.f);
-                    v[c][i] = __fadd2_rn(v[c][i], m);
-                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
-                    d2 = __fadd2_rn(d2, v[c][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 m = make_float2(2 * i >= lo && 2 * i < hi ? -mean0 : 0.f, 2 * i + 1 >= lo && 2 * i + 1 < hi ? -mean0 : 0.f);
+                        v[c][i] = __fadd2_rn(v[c][i], m);
+                        q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                        d2 = __fadd2_rn(d2, v[c][i]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float m = ODD || tid + c * TPR < K.n ? -mean0 : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[c][i] = __fadd2_rn(v[c][i], make_float2(m, m));
+                        q2 = __ffma2_rn(v[c][i], v[c][i], q2);
+                        d2 = __fadd2_rn(d2, v[c][i]);
+                    }
                 }
             }
-        } else {
+            float q[2] = {q2.x + q2.y, d2.x + d2.y};
+            row_sum<2, WARPS>(q, red2[par]);
+            if (beyond_fp32(P, q[0])) break;                        // (equal for all threads of the row)
+            const float corr = over_h(P, q[1]);
+            const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
+            if (tid == 0) {
+                if (P.mean) P.mean[row] = mean0 + corr;
+                if (P.rstd) P.rstd[row] = rstd;
+            }
+            const float shift = -corr * rstd;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const float m = ODD || tid + c * TPR < K.n ? -mean0 : 0.f;
+                const int chunk = tid + c * TPR;
+                const bool live = chunk < K.n;
+                float2 w[4], b[4];
+                ld_staged(prm, K.n, live ? chunk : 0, w);
+                ld_staged(prm + 2 * K.n, K.n, live ? chunk : 0, b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[c][i] = __fadd2_rn(v[c][i], make_float2(m, m));
-                    q2 = __ffma2_rn(v[c][i], v[c][i], q2);
-                    d2 = __fadd2_rn(d2, v[c][i]);
+                for (int i = 0; i < 4; ++i)
+                    v[c][i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
+                if constexpr (FMT < 0) {
+                    st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, v[c]);
+                } else if constexpr (!together) {
+                    float2 o[1][4] = {{v[c][0], v[c][1], v[c][2], v[c][3]}};
+                    mx_store<FMT, 1>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, 0, P.H);
                 }
             }
+            if constexpr (FMT >= 0 && together)
+                mx_store<FMT, C>(v, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * tid, 8 * TPR, P.H);
         }
-        float q[2] = {q2.x + q2.y, d2.x + d2.y};
-        row_sum<2, WARPS>(q, red2[par]);
-        if (beyond_fp32(P, q[0])) break;                        // (equal for all threads of the row)
-        const float corr = over_h(P, q[1]);
-        const float rstd = 1.f / sqrtf(fmaxf(fmaf(-corr, corr, over_h(P, q[0])), 0.f) + P.eps);
-        if (tid == 0) {
-            if (P.mean) P.mean[row] = mean0 + corr;
-            if (P.rstd) P.rstd[row] = rstd;
-        }
-        const float shift = -corr * rstd;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int chunk = tid + c * TPR;
-            const bool live = chunk < K.n;
-            float2 w[4], b[4];
-            ld_staged(prm, K.n, live ? chunk : 0, w);
-            ld_staged(prm + 2 * K.n, K.n, live ? chunk : 0, b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[c][i] = __ffma2_rn(__ffma2_rn(v[c][i], make_float2(rstd, rstd), make_float2(shift, shift)), w[i], b[i]);
-            if constexpr (FMT < 0) {
-                st_chunk<T, ODD>(reinterpret_cast<T*>(P.y) + row * P.H - K.a, chunk, K, v[c]);
-            } else if constexpr (!together) {
-                float2 o[1][4] = {{v[c][0], v[c][1], v[c][2], v[c][3]}};
-                mx_store<FMT, 1>(o, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * chunk, 0, P.H);
-            }
-        }
-        if constexpr (FMT >= 0 && together)
-            mx_store<FMT, C>(v, P.q_out + row * (P.H / 32) * fmt_block_bytes(FMT), P.q_scales + row * (P.H / 32), 8 * tid, 8 * TPR, P.H);
-      }
-      if (row >= P.rows) break;
-      // (the call stands outside the loop over the rows: inside it E2M1 takes 105 us instead of 101, E4M3 106 instead of 101)
-      norm_row_64<T, WARPS, FMT>(P, row, tid, red64);
-      row += P.step;
-      begin(row);
+        if (row >= P.rows) break;
+        // (the call stands outside the loop over the rows: inside it E2M1 takes 105 us instead of 101, E4M3 106 instead of 101)
+        norm_row_64<T, WARPS, FMT>(P, row, tid, red64);
+        row += P.step;
+        begin(row);
     }
 }
 
@@ -739,7 +739,7 @@ layer_norm_backward_kernel(const LnParams P) {
             }
         }
     } else {
-st_sums<C, TPR, ODD>(out, tid, K, dw);
+        st_sums<C, TPR, ODD>(out, tid, K, dw);
         st_sums<C, TPR, ODD>(out + P.part_ld, tid, K, db);
     }
 }
