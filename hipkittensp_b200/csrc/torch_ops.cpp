@@ -92,10 +92,7 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> o
         if (t->get_device() != a.get_device()) refuse("all tensors must be on the same device");
 }
 
-// Neither an allocation nor a launch holds the interpreter lock: both may wait for the device (a full queue, memory that is freed to make
-// room, the library's first scratch buffer), and what the device waits for may be a callback that needs the lock.
 at::Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const at::Tensor& like) {
-    py::gil_scoped_release unlocked;
     return at::detail::empty_cuda(size, dtype, like.device(), std::nullopt);
 }
 
@@ -110,7 +107,9 @@ void check(int rc) {
     throw py::error_already_set();
 }
 
-// entry(stream) on torch's current stream of t's device, with that device current
+// entry(stream) on torch's current stream of t's device, with that device current and without the interpreter lock: a call's allocations, which
+// stand in its entry, and its launch may wait for the device (a full queue, memory that is freed to make room, the library's first
+// scratch buffer), and what the device waits for may be a callback that needs the lock.  (Released once per call: 0.1 us.)
 template <typename F>
 void launch(const at::Tensor& t, F entry) {
     const c10::DeviceIndex dev = (c10::DeviceIndex)t.get_device();
@@ -137,8 +136,9 @@ Operands operands(py::handle A, py::handle scale_A, py::handle B, py::handle sca
     same_device(a, {&b, &sa, &sb});
     return o;
 }
-at::Tensor result(const Operands& o, py::handle out) {
-    if (out.is_none()) return empty({o.M, o.N}, at::kBFloat16, o.a);
+// the matrix a caller gives for the result; undefined when None
+at::Tensor given_result(const Operands& o, py::handle out) {
+    if (out.is_none()) return {};
     const at::Tensor& c = matrix(out, "C", at::kBFloat16);
     if (c.size(0) != o.M || c.size(1) != o.N) refuse("C must be [" + std::to_string(o.M) + ", " + std::to_string(o.N) + "]");
     same_device(o.a, {&c});
@@ -173,8 +173,9 @@ py::object gemm(py::handle A, py::handle scale_A, py::handle B, py::handle scale
     same_device(a, {&b, &sa, &sb});
     if (given) same_device(a, {given});
     const Workspace ws = workspace_of(o, workspace);
-    at::Tensor c = given ? *given : empty({o.M, o.N}, at::kBFloat16, a);
+    at::Tensor c = given ? *given : at::Tensor();
     launch(o.a, [&](void* st) {
+        if (!c.defined()) c = empty({o.M, o.N}, at::kBFloat16, o.a);
         const void *a = o.a.const_data_ptr(), *sa = o.sa.const_data_ptr(), *b = o.b.const_data_ptr(), *sb = o.sb.const_data_ptr();
         return ws.own ? lib.mxfp6_gemm_ex(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, 0, st)
                       : lib.mxfp6_gemm_ws(a, sa, b, sb, c.mutable_data_ptr(), o.M, o.N, o.K, fmt, fmt_b, ws.ptr, ws.bytes, st);
@@ -196,8 +197,9 @@ py::object gemm_scaled(py::handle A, py::handle scale_A, py::handle B, py::handl
     };
     const float *r = vec(row_scale, "row_scale", o.M), *cs = vec(col_scale, "col_scale", o.N), *bs = vec(bias, "bias", o.N);
     const Workspace ws = workspace_of(o, workspace);
-    at::Tensor c = result(o, out);
+    at::Tensor c = given_result(o, out);
     launch(o.a, [&](void* st) {
+        if (!c.defined()) c = empty({o.M, o.N}, at::kBFloat16, o.a);
         const void *a = o.a.const_data_ptr(), *sa = o.sa.const_data_ptr(), *b = o.b.const_data_ptr(), *sb = o.sb.const_data_ptr();
         return ws.own ? lib.mxfp6_gemm_scaled(a, sa, b, sb, c.mutable_data_ptr(), r, cs, bs, o.M, o.N, o.K, fmt, fmt_b, st)
                       : lib.mxfp6_gemm_scaled_ws(a, sa, b, sb, c.mutable_data_ptr(), r, cs, bs, o.M, o.N, o.K, fmt, fmt_b, ws.ptr, ws.bytes, st);
@@ -213,8 +215,10 @@ py::tuple quantize(py::handle X, int fmt) {
         refuse("quantize expects a contiguous 2-D fp32 or bf16 tensor");
     const int64_t rows = x.size(0), K = x.size(1);
     if (K % 32) refuse("K must be a multiple of 32");
-    at::Tensor packed = empty({rows, row_bytes(K, fmt)}, at::kByte, x), scales = empty({rows, K / 32}, at::kByte, x);
+    at::Tensor packed, scales;
     launch(x, [&](void* st) {
+        packed = empty({rows, row_bytes(K, fmt)}, at::kByte, x);
+        scales = empty({rows, K / 32}, at::kByte, x);
         return lib.mxfp6_quantize(x.const_data_ptr(), x.scalar_type() == at::kFloat ? 0 : 1, rows, K, fmt, packed.mutable_data_ptr(), scales.mutable_data_ptr(), st);
     });
     return py::make_tuple(wrap(std::move(packed)), wrap(std::move(scales)));
@@ -225,8 +229,11 @@ py::object dequantize(py::handle P, py::handle S, int fmt, bool bf16) {
     const int64_t rows = p.size(0), K = k_of(p, fmt, "packed");
     if (K % 32 || s.size(0) != rows || s.size(1) != K / 32) refuse("scales must be [rows, K/32]");
     same_device(p, {&s});
-    at::Tensor out = empty({rows, K}, bf16 ? at::kBFloat16 : at::kFloat, p);
-    launch(p, [&](void* st) { return lib.mxfp6_dequantize_ex(p.const_data_ptr(), s.const_data_ptr(), rows, K, fmt, out.mutable_data_ptr(), bf16 ? 1 : 0, st); });
+    at::Tensor out;
+    launch(p, [&](void* st) {
+        out = empty({rows, K}, bf16 ? at::kBFloat16 : at::kFloat, p);
+        return lib.mxfp6_dequantize_ex(p.const_data_ptr(), s.const_data_ptr(), rows, K, fmt, out.mutable_data_ptr(), bf16 ? 1 : 0, st);
+    });
     return wrap(std::move(out));
 }
 
@@ -250,15 +257,16 @@ Norm norm_of(py::handle X, py::handle weight, py::handle bias) {
 py::tuple layer_norm(py::handle X, py::handle weight, py::handle bias, double eps, py::handle out) {
     const Norm n = norm_of(X, weight, bias);
     at::Tensor y;
-    if (out.is_none()) {
-        y = empty({n.rows, n.H}, n.x.scalar_type(), n.x);
-    } else {
+    if (!out.is_none()) {
         int code = 0;
         y = rows_of(out, "out", &code);
         if (y.sizes() != n.x.sizes() || code != n.code || y.get_device() != n.x.get_device()) refuse("out must have the shape, dtype and device of x");
     }
-    at::Tensor mean = empty({n.rows}, at::kFloat, n.x), rstd = empty({n.rows}, at::kFloat, n.x);
+    at::Tensor mean, rstd;
     launch(n.x, [&](void* st) {
+        if (!y.defined()) y = empty({n.rows, n.H}, n.x.scalar_type(), n.x);
+        mean = empty({n.rows}, at::kFloat, n.x);
+        rstd = empty({n.rows}, at::kFloat, n.x);
         return lib.mxfp6_layer_norm(n.x.const_data_ptr(), n.code, n.w, n.b, n.wcode, y.mutable_data_ptr(), (float*)mean.mutable_data_ptr(),
                                 (float*)rstd.mutable_data_ptr(), n.rows, n.H, (float)eps, st);
     });
@@ -268,9 +276,12 @@ py::tuple layer_norm(py::handle X, py::handle weight, py::handle bias, double ep
 py::tuple layer_norm_quantize(py::handle X, py::handle weight, py::handle bias, double eps, int fmt) {
     const Norm n = norm_of(X, weight, bias);
     if (n.H % 32) refuse("H must be a multiple of 32");
-    at::Tensor packed = empty({n.rows, row_bytes(n.H, fmt)}, at::kByte, n.x), scales = empty({n.rows, n.H / 32}, at::kByte, n.x);
-    at::Tensor mean = empty({n.rows}, at::kFloat, n.x), rstd = empty({n.rows}, at::kFloat, n.x);
+    at::Tensor packed, scales, mean, rstd;
     launch(n.x, [&](void* st) {
+        packed = empty({n.rows, row_bytes(n.H, fmt)}, at::kByte, n.x);
+        scales = empty({n.rows, n.H / 32}, at::kByte, n.x);
+        mean = empty({n.rows}, at::kFloat, n.x);
+        rstd = empty({n.rows}, at::kFloat, n.x);
         return lib.mxfp6_layer_norm_quantize(n.x.const_data_ptr(), n.code, n.w, n.b, n.wcode, fmt, packed.mutable_data_ptr(), scales.mutable_data_ptr(),
                                          (float*)mean.mutable_data_ptr(), (float*)rstd.mutable_data_ptr(), n.rows, n.H, (float)eps, st);
     });
@@ -284,15 +295,13 @@ py::tuple layer_norm_backward(py::handle DY, py::handle X, py::handle mean, py::
     if (dy.sizes() != n.x.sizes() || code != n.code || dy.get_device() != n.x.get_device()) refuse("dy must have the shape, dtype and device of x");
     if (mean.is_none() || rstd.is_none()) refuse("Expected a torch.Tensor");
     const float *m = (const float*)vector_of(mean, "mean", n.rows, n.x, false, nullptr), *r = (const float*)vector_of(rstd, "rstd", n.rows, n.x, false, nullptr);
-    at::Tensor dx = empty({n.rows, n.H}, n.x.scalar_type(), n.x), dw = empty({n.H}, at::kFloat, n.x), db = empty({n.H}, at::kFloat, n.x);
-    size_t bytes;
-    {
-        py::gil_scoped_release unlocked;
-        c10::cuda::CUDAGuard guard((c10::DeviceIndex)n.x.get_device());
-        bytes = lib.mxfp6_layer_norm_backward_workspace_bytes(n.rows, n.H);
-    }
-    at::Tensor work = empty({(int64_t)bytes}, at::kByte, n.x);
+    at::Tensor dx, dw, db;
     launch(n.x, [&](void* st) {
+        dx = empty({n.rows, n.H}, n.x.scalar_type(), n.x);
+        dw = empty({n.H}, at::kFloat, n.x);
+        db = empty({n.H}, at::kFloat, n.x);
+        const size_t bytes = lib.mxfp6_layer_norm_backward_workspace_bytes(n.rows, n.H);
+        at::Tensor work = empty({(int64_t)bytes}, at::kByte, n.x);
         return lib.mxfp6_layer_norm_backward(dy.const_data_ptr(), n.x.const_data_ptr(), n.code, m, r, n.w, n.wcode, dx.mutable_data_ptr(),
                                          (float*)dw.mutable_data_ptr(), (float*)db.mutable_data_ptr(), n.rows, n.H, work.mutable_data_ptr(), bytes, st);
     });
