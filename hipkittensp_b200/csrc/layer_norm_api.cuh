@@ -258,7 +258,7 @@ static int ln_backward(const void* dy, const void* x, int x_dtype, const float* 
     int parts;
     if (k.kern) {
         parts = ln_grid(rows, k.warps, place == kLnOdd, ln_backward_cap(k.warps, d->sm_count, rows, x_dtype == 0 ? 4 : 2), &P.step);
-        if (k.smem > 48 * 1024 && (rc = ensure_smem_attr(*d, (const void*)k.kern, 4 * kLnBackwardWide + 64 + 2 * 2 * 4 * 512 * 16))) return rc;
+        if (k.smem > 32 * 1024 && (rc = ensure_smem_attr(*d, (const void*)k.kern, 4 * kLnBackwardWide + 64 + 2 * 2 * 4 * 512 * 16))) return rc;
         if ((rc = launch_pdl(k.kern, (unsigned)parts, (unsigned)(k.warps == 1 ? 256 : 32 * k.warps), (size_t)k.smem, st, P))) return rc;
     } else {
         parts = ln_parts_columns(rows, H, d->sm_count);

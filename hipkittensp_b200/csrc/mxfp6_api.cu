@@ -302,7 +302,8 @@ static int resident_ctas(DeviceState& d, const void* kern, int threads, int smem
     std::lock_guard<std::mutex> lk(g_mu);
     int& n = d.ctas_per_sm[{kern, smem}];
     if (n == 0) {
-        if (smem > 48 * 1024) CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 132 * 1024));
+        // (whatever the amount: the 48 KB that need no such call hold a kernel's static shared memory too)
+        CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 132 * 1024));
         CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, (size_t)smem));
     }
     if (n < 1) return fail(MXFP6_ERR_CUDA, "a kernel of %d threads does not fit an SM", threads);

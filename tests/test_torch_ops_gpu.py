@@ -119,3 +119,44 @@ def test_gemm_refuses_in_the_words_of_dispatch_micro():
     for call in (lambda: hk.gemm(u8(32, 98), sA, B, sB), lambda: hk.gemm(A, sA, u8(48, 128), sB, hk.E4M3)):
         with pytest.raises(RuntimeError, match="must be 3K/4 bytes|B must be"):
             call()
+
+
+def test_calls_from_several_threads():
+    """Four threads with a stream each, whose calls may now overlap on the host too: the bits of a thread alone."""
+    def operands(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        n = lambda *s: torch.randn(*s, device="cuda", generator=g)
+        x, w, dy = n(24, 1024 + 32 * seed), n(1024 + 32 * seed), n(24, 1024 + 32 * seed)
+        B, sB = hk.quantize(0.05 * n(512, 1024), hk.E2M1)
+        return x, w, dy, B, sB, hk.gemm_workspace(24, 512, 1024)
+
+    def step(x, w, dy, B, sB, ws):
+        A, sA, mean, rstd = hk.layer_norm_quantize(x, w, None, fmt=hk.E2M1)
+        y = hk.layer_norm(x, w)[0]
+        P, sP = hk.quantize(y[:, :1024].contiguous(), hk.E2M1)
+        return (A, sA, y, hk.gemm(P, sP, B, sB, hk.E2M1, workspace=ws), hk.gemm_scaled(P, sP, B, sB, fmt=hk.E2M1, workspace=ws), hk.dequantize(A, sA, hk.E2M1),
+                *hk.layer_norm_backward(dy, x, mean, rstd, w))
+
+    cases = [operands(i) for i in range(4)]
+    want = [[t.clone() for t in step(*c)] for c in cases]
+    torch.cuda.synchronize()
+    wrong, errors = [], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(100):
+                    got = step(*cases[i])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append((i, k))
+        except BaseException as e:      # noqa: BLE001 -- reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and not wrong, (errors[:1], wrong[:5])
+    assert hk.device_status() == 0
