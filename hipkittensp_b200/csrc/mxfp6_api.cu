@@ -463,8 +463,10 @@ enum WsMode : int { kWsOwn = 0,       // the library's per-device buffer, alloca
 static bool scales_by_tma(const void* sfa, const void* sfb, int64_t K) {
     return ((K / 32) % 16 == 0) && !((uintptr_t)sfa & 15) && !((uintptr_t)sfb & 15) && !options().no_sf_tma;
 }
-static bool dest_by_tma(const Dest& dst) {
-    bool ok = (dst.ldc % 8) == 0;      // the pair kernel stores C by TMA: 16-byte aligned destinations and row stride
+static bool dest_by_tma(const Dest& dst, int64_t N) {
+    // TMA stores of C want 16-byte aligned destinations and row stride, and rows of whole 16-byte units: a store is clipped to the map in
+    // such units, so with N % 8 != 0 (a window of a wider matrix) it writes zeros into the columns behind the window.
+    bool ok = (dst.ldc % 8) == 0 && (N % 8) == 0;
     for (int i = 0; i < dst.n; ++i) ok = ok && !((uintptr_t)dst.c[i] & 15);
     return ok;
 }
@@ -661,9 +663,9 @@ static int gemm_unguarded(const void* a, const void* sfa, const void* b, const v
     Recipe r;
     r.key = key;
     if (sig.flag) {
-        if (!pl.pair || pl.ws_bytes || q_fmt >= 0 || dst.n != 1 || !dest_by_tma(dst) || options().c_plain || sig.cols < 1 || !sig.counter)
+        if (!pl.pair || pl.ws_bytes || q_fmt >= 0 || dst.n != 1 || !dest_by_tma(dst, N) || options().c_plain || sig.cols < 1 || !sig.counter)
             return fail(MXFP6_ERR_BAD_ARG, "completion flags need the CTA-pair kernel with TMA stores of C (M > 128, N >= 256, "
-                                           "16-byte aligned C and row stride) and one destination");
+                                           "N a multiple of 8, 16-byte aligned C and row stride) and one destination");
         r.counter_ptr = sig.counter;
         r.counter_bytes = (size_t)ceil_div(pl.tiles_p, options().group_p) * ceil_div(pl.tiles_q, sig.cols) * sizeof(unsigned int);
     }
@@ -748,11 +750,11 @@ static int gemm_unguarded(const void* a, const void* sfa, const void* b, const v
     for (int i = 1; i < dst.n; ++i) P.c_more[i - 1] = (__nv_bfloat16*)dst.c[i];
     P.ndst = dst.n;
     P.push_rotate = o.push_rotate;
-    P.c_tma = (q_fmt >= 0 || (dest_by_tma(dst) && !o.c_plain)) ? 1 : 0;
-    P.c_vec16 = (dest_by_tma(dst) && N % 8 == 0) ? 1 : 0;
+    P.c_tma = (q_fmt >= 0 || (dest_by_tma(dst, N) && !o.c_plain)) ? 1 : 0;
+    P.c_vec16 = (dest_by_tma(dst, N) && N % 8 == 0) ? 1 : 0;
     // (a TMA store writes 128 rows: tiles of fewer rows only where there is a single row of tiles, so that what lies
     // below the tile lies below C and is clipped)
-    P.c_tma_last = (!pl.pair && !pl.swap && o.c_tma_last && q_fmt < 0 && dst.n == 1 && dest_by_tma(dst) &&
+    P.c_tma_last = (!pl.pair && !pl.swap && o.c_tma_last && q_fmt < 0 && dst.n == 1 && dest_by_tma(dst, N) &&
                     (pl.p_tile == 128 || pl.tiles_p == 1)) ? 1 : 0;
     P.q_out = (uint8_t*)q_out; P.q_scales = (uint8_t*)q_scales; P.q_fmt = q_fmt;
     P.q_ld = q_fmt < 0 ? 0 : fmt_row_bytes(N, q_fmt);

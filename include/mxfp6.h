@@ -179,8 +179,8 @@ int mxfp6_gemm_multi(const void* a, const void* sfa, const void* b, const void* 
  * peer 737 GB/s, 4 row blocks 708, 16 row blocks 605, 4 x 7 blocks 579), and several copies in flight to the same peer
  * make it worse (16 blocks on two streams per peer 449), so: one stream per peer and strip_tiles large.  scratch: device memory of at least
  * mxfp6_copy_gather_scratch_bytes(M, N, strip_tiles) bytes, 4-byte aligned, owned by this call until `stream` has
- * passed it.  Needs the CTA-pair kernel with TMA stores of C (M > 128, N >= 256, 16-byte aligned destinations and
- * row stride); other problems are refused with MXFP6_ERR_BAD_ARG.  Not capturable into a CUDA graph.  Stands where
+ * passed it.  Needs the CTA-pair kernel with TMA stores of C (M > 128, N >= 256 and a multiple of 8, 16-byte aligned destinations
+ * and row stride); other problems are refused with MXFP6_ERR_BAD_ARG.  Not capturable into a CUDA graph.  Stands where
  * mxfp6_gemm_multi stands (distributed-kernels/bf16_gemm/kernel.cpp:253-265); the reference has no copy-engine path.
  */
 size_t mxfp6_copy_gather_scratch_bytes(int64_t M, int64_t N, int strip_tiles);
