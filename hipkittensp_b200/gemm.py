@@ -113,6 +113,24 @@ def dispatch_micro(A, B, C, scale_A, scale_B, fmt: int = E2M3, fmt_b: int | None
             M, N, K, fmt, fb, _lib.FLAG_B_STATIC if b_static else 0, *ws)
 
 
+def _destinations(A, dests, col_offset: int, M: int, N: int) -> int:
+    """Row stride of the matrices that receive an [M,N] product at a column offset; the first is on A's device, the others on any GPU."""
+    if not 1 <= len(dests) <= 8:
+        raise RuntimeError("1 to 8 destinations")
+    for d in dests:
+        if not isinstance(d, torch.Tensor):
+            raise RuntimeError("Expected a torch.Tensor")
+        if not d.is_cuda:
+            raise RuntimeError("Tensor must be on CUDA device")
+        if d.dtype != torch.bfloat16 or d.dim() != 2 or d.stride(1) != 1 or d.stride(0) != dests[0].stride(0) or d.shape[0] != M:
+            raise RuntimeError("destinations must be bf16 [M, ldc] matrices with one common row stride")
+        if col_offset < 0 or col_offset + N > d.shape[1]:
+            raise RuntimeError("column window outside the destination")
+    if dests[0].get_device() != A.get_device():
+        raise RuntimeError("all tensors must be on the same device")
+    return dests[0].stride(0)
+
+
 def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2M3, workspace=None) -> None:
     """The [M,N] product written into the column window [col_offset, col_offset+N) of every matrix in `dests`.
 
@@ -130,14 +148,7 @@ def dispatch_multi(A, B, dests, col_offset: int, scale_A, scale_B, fmt: int = E2
     if _k_of(B, fmt, "B") != K:
         raise RuntimeError("A and B disagree on K")
     _check_scales(A, B, scale_A, scale_B, K)
-    if not 1 <= len(dests) <= 8:
-        raise RuntimeError("1 to 8 destinations")
-    ldc = dests[0].stride(0)
-    for d in dests:
-        if d.dtype != torch.bfloat16 or d.dim() != 2 or d.stride(1) != 1 or d.stride(0) != ldc or d.shape[0] != M:
-            raise RuntimeError("destinations must be bf16 [M, ldc] matrices with one common row stride")
-        if col_offset < 0 or col_offset + N > d.shape[1]:
-            raise RuntimeError("column window outside the destination")
+    ldc = _destinations(A, dests, col_offset, M, N)
     ptrs = (ctypes.c_void_p * len(dests))(*[d.data_ptr() + 2 * col_offset for d in dests])
     ws = () if workspace is None else _workspace(workspace, A.get_device())
     _launch(A, lib.mxfp6_gemm_multi_ws if ws else lib.mxfp6_gemm_multi, A.data_ptr(), scale_A.data_ptr(), B.data_ptr(), scale_B.data_ptr(), ptrs, len(dests),
@@ -173,15 +184,8 @@ def dispatch_copy_gather(A, B, dests, col_offset: int, scale_A, scale_B, scratch
     if _k_of(B, fmt, "B") != K:
         raise RuntimeError("A and B disagree on K")
     _check_scales(A, B, scale_A, scale_B, K)
-    if not 1 <= len(dests) <= 8:
-        raise RuntimeError("1 to 8 destinations")
-    ldc = dests[0].stride(0)
-    for d in dests:
-        if d.dtype != torch.bfloat16 or d.dim() != 2 or d.stride(1) != 1 or d.stride(0) != ldc or d.shape[0] != M:
-            raise RuntimeError("destinations must be bf16 [M, ldc] matrices with one common row stride")
-        if col_offset < 0 or col_offset + N > d.shape[1]:
-            raise RuntimeError("column window outside the destination")
-    if scratch.device != A.device or not scratch.is_contiguous():
+    ldc = _destinations(A, dests, col_offset, M, N)
+    if not isinstance(scratch, torch.Tensor) or scratch.device != A.device or not scratch.is_contiguous():
         raise RuntimeError("scratch must be a contiguous tensor on the operands' device")
     ptrs = (ctypes.c_void_p * len(dests))(*[d.data_ptr() + 2 * col_offset for d in dests])
     streams = (ctypes.c_void_p * max(len(copy_streams), 1))(*[s.cuda_stream for s in copy_streams])
@@ -262,6 +266,7 @@ def device_status() -> int:
 
 def tma_dump(packed: torch.Tensor, row0: int = 0, k0: int = 0) -> torch.Tensor:
     """Diagnostic: the 16 KiB shared-memory image of one 128x128 operand box as the GEMM loads it."""
+    _accept(packed, "packed", torch.uint8)
     rows, K = packed.shape[0], packed.shape[1] // 3 * 4
     out = torch.empty(16384, dtype=torch.uint8, device=packed.device)
     _launch(packed, lib.mxfp6_debug_tma_dump, packed.data_ptr(), rows, K, row0, k0, out.data_ptr())

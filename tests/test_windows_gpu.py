@@ -72,3 +72,22 @@ def test_a_ragged_window_has_no_completion_flags():
     A, sA, B, sB = _operands(M, 1280, K, R.E2M3)
     hk.dispatch_copy_gather(A, B, [d8], 8, sA, sB, scratch, [])
     assert torch.equal(d8[:, 8:], hk.gemm(A, sA, B, sB)) and torch.isnan(d8[:, :8]).all()
+
+
+def test_destinations_that_are_no_gpu_memory_are_refused():
+    """A matrix in host memory, or no matrix: refused on the host, before anything could write there."""
+    M, N, K = 300, 512, 256
+    A, sA, B, sB = _operands(M, N, K, R.E2M3)
+    good = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    scratch = torch.zeros(1024, dtype=torch.int32, device="cuda")
+    for bad in ([good.cpu()], [good, good.cpu()], [good, good.cpu().pin_memory()], [1], [good, None], [good.float()], [good[:100]], [good[:, 1:]], [], [good] * 9):
+        with pytest.raises(RuntimeError):
+            hk.dispatch_multi(A, B, bad, 0, sA, sB)
+        with pytest.raises(RuntimeError):
+            hk.dispatch_copy_gather(A, B, bad, 0, sA, sB, scratch, [])
+    for bad in (scratch.cpu(), None, scratch[::2]):
+        with pytest.raises(RuntimeError):
+            hk.dispatch_copy_gather(A, B, [good], 0, sA, sB, bad, [])
+    with pytest.raises(RuntimeError, match="Tensor must be on CUDA device"):
+        hk.tma_dump(torch.zeros(128, 96, dtype=torch.uint8))
+    assert not good.any()
