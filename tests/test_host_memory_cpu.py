@@ -36,9 +36,14 @@ for size in (1 << 20, 256 << 10, 120 << 10, 60 << 10, 30 << 10):
             held.append(bytearray(size))
     except MemoryError:
         pass
-rc = call()
-msg = L.mxfp6_last_error()
-held.clear()
+try:
+    rc = call()
+    msg = L.mxfp6_last_error()
+    held.clear()
+except MemoryError:                 # Python itself had nothing left: this run says nothing
+    held.clear()
+    print("HOST_MEMORY_UNDECIDED")
+    sys.exit(0)
 assert rc == _lib.ERR_CUDA and msg == b"out of host memory", (rc, msg)
 assert call() == _lib.ERR_BAD_ARG and b"multiple of 128" in L.mxfp6_last_error()
 print("HOST_MEMORY_OK")
@@ -48,4 +53,6 @@ print("HOST_MEMORY_OK")
 @pytest.mark.parametrize("entry", ["gemm", "gemm_ws", "gemm_ex", "gemm_ex_ws", "gemm_requant", "gemm_scaled", "gemm_multi", "gemm_noalloc"])
 def test_products(entry):
     out = subprocess.run([sys.executable, "-c", _CHILD, ROOT, entry], capture_output=True, text=True, timeout=300)
+    if out.returncode == 0 and "HOST_MEMORY_UNDECIDED" in out.stdout:
+        pytest.skip("the interpreter ran out of memory first")
     assert "HOST_MEMORY_OK" in out.stdout, (out.returncode, out.stdout[-500:], out.stderr[-1000:])

@@ -31,7 +31,7 @@ del used
 torch.cuda.empty_cache()
 side = torch.cuda.Stream()
 for (s, t), out in zip(cases, outs):
-    torch.cuda._sleep(200_000_000)                      # about 0.1 s on the default stream
+    torch.cuda._sleep(1_000_000_000)                    # about 0.5 s on the default stream
     with torch.cuda.stream(side):
         hk.gemm(*t, out=out)
         done = torch.cuda.Event()
