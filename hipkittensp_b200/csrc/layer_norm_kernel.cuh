@@ -217,7 +217,8 @@ __device__ __forceinline__ void mx_store(float2 (&v)[C][4], uint8_t* codes_row, 
 // A row that fp32 statistics cannot carry, by the TPR = 32 * WARPS threads that share it, in 64 bits and straight from memory: the sum
 // or the sum of squares overflows (values past about 1e17), the squares vanish below the range and eps does not cover them, or
 // the row holds an infinity or a NaN (whose mean and rstd come out as the formulas give them).  Not inlined: no
-// register of the usual path is held for it.
+// register of the usual path is held for it.  Three passes with one element per load: 16384 x 8192 bf16, every row of that kind, 0.85 ms
+// against 0.095.
 template <int WARPS>
 __device__ __forceinline__ double row_sum64(double v, double* red) {
 #pragma unroll

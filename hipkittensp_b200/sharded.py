@@ -60,7 +60,11 @@ def assemble_columns(gathered: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 
 def _scratch(M: int, N: int, K: int, device):
     """Scratch of an operator's own for a local product that is split along K: two operators may run side by side."""
-    return gemm_workspace(M, N, K, device) if device is not None and torch.device(device).type == "cuda" else None
+    if device is None or torch.device(device).type != "cuda":
+        return None
+    ws = gemm_workspace(M, N, K, device)
+    torch.cuda.current_stream(ws.device).synchronize()      # zeroed before any stream that the operator is called on
+    return ws
 
 
 class ColumnParallelGemm:

@@ -252,8 +252,12 @@ def test_sharded_operators_side_by_side(kind):
     for seed in (1, 2):
         t, _ = _operands(M, N, K, seed, hk.E2M3, hk.E2M3)
         want = hk.gemm(*t, workspace=hk.gemm_workspace(M, N, K))
-        sides.append((getattr(sharded, kind)(M, N, K, device="cuda"), t, want, torch.cuda.Stream()))
+        sides.append((t, want, torch.cuda.Stream()))
     torch.cuda.synchronize()
+    junk = torch.full((32 << 20,), 0x41, dtype=torch.uint8, device="cuda")
+    del junk
+    torch.cuda._sleep(100_000_000)                     # the operators are made while their constructor's stream is busy
+    sides = [(getattr(sharded, kind)(M, N, K, device="cuda"), *s) for s in sides]
     for _ in range(24):
         for op, t, _, stream in sides:
             with torch.cuda.stream(stream):
